@@ -47,6 +47,8 @@ EXPORTS = [
     "cora_shard_plan", "cora_shard_configure", "cora_shard_info", "cora_shard_exchange_words",
     "cora_shard_search_begin", "cora_shard_probe_words", "cora_shard_search_probe",
     "cora_shard_search_begin_probed", "cora_shard_search_resume", "cora_shard_search_end",
+    "cora_kv4_block_bytes", "cora_kv4_status", "cora_kv4_append", "cora_kv4_attend_workspace",
+    "cora_kv4_attend", "cora_w4_matvec",
 ]
 
 _p = C.c_void_p

@@ -23,24 +23,13 @@
 #include "kernels_query.cuh"
 #include "kernels_refine.cuh"
 #include "kernels_scan.cuh"
+#include "status.hpp"
 
 namespace cora {
-namespace {
 
 thread_local std::string g_last_error;
 
-struct Error : std::runtime_error {
-    int code;
-    Error(int c, const std::string &m) : std::runtime_error(m), code(c) {}
-};
-[[noreturn]] void fail(int code, const std::string &msg) { throw Error(code, msg); }
-
-#define CUDA_TRY(call)                                                                  \
-    do {                                                                                \
-        cudaError_t e_ = (call);                                                        \
-        if (e_ != cudaSuccess)                                                          \
-            ::cora::fail(CORA_ECUDA, std::string(#call) + ": " + cudaGetErrorString(e_)); \
-    } while (0)
+namespace {
 
 // Limits of the reference (include/coraanns/search/parameters.hpp:9-13).
 constexpr uint64_t kDefaultVanguard = 5, kMaxQueryChunk = 65535, kMaxProbeCount = 65536;
@@ -1654,22 +1643,8 @@ struct cora_engine {
 };
 
 namespace {
-template <typename F>
-int guarded(F &&f) {
-    try {
-        f();
-        return CORA_OK;
-    } catch (const cora::Error &e) {
-        cora::g_last_error = e.what();
-        return e.code;
-    } catch (const std::bad_alloc &e) {
-        cora::g_last_error = e.what();
-        return CORA_ENOMEM;
-    } catch (const std::exception &e) {
-        cora::g_last_error = e.what();
-        return CORA_ERUNTIME;
-    }
-}
+using cora::guarded;
+
 Engine &eng(cora_engine *h) {
     if (!h || !h->e) cora::fail(CORA_EINVAL, "null engine");
     return *h->e;

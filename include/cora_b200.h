@@ -302,6 +302,107 @@ uint64_t cora_probe_noalloc_scratch_limit(void);
  * on this device (a bounded wait in the tensor-core kernel that expired): CORA_ERUNTIME. */
 int cora_probe_noalloc_status(cora_engine *engine, void *stream);
 
+/* ---- a reader in 4 bits beside the index (no counterpart in the reference) ---------------
+ *
+ * Operators of a language model that reads what a search retrieved, on the GPU whose memory the
+ * index fills: its attention cache and its weights are kept in 4 bits. All calls need no engine;
+ * they enqueue on `stream` (NULL: the default stream) of the current device and return without
+ * synchronising. All pointers are device memory; 16-bit tensors are bf16 or fp16 (cora_dtype).
+ *
+ * Format. A group of G consecutive values is 4-bit codes c and two fp16 factors (scale, low),
+ * and stands for scale * c + low. Quantising a group x: low = fp16(min x),
+ * scale = fp16((max x - min x) / 15), c = clamp(rne((x - low) * (1 / scale)), 0, 15), c = 0 where
+ * scale is 0, each operation in fp32; factors saturate at the largest fp16, NaN is kept.
+ *
+ * Errors on the device (a slot, position, page or row range outside its tensor, a wait that ran
+ * out) set bits of the cache's status word (1-word device memory, zero at start: bit 1 a wait
+ * timed out, bit 2 bad input); the access is skipped and the results it would have given are
+ * unspecified. cora_kv4_status reads and clears it. */
+typedef enum { CORA_BF16 = 0, CORA_FP16 = 1 } cora_dtype;
+
+/* A paged cache: num_pages x kv_heads blocks of cora_kv4_block_bytes() bytes, 16-byte aligned.
+ * A block holds page_size tokens of one key head, each section token-major: key codes
+ * (head_dim / 2 bytes per token, byte j: dimension 2j low nibble, 2j + 1 high nibble), value
+ * codes, key factors (head_dim / group pairs of fp16 (scale, low)), value factors.
+ * head_dim 64, 128 or 256; group 64 or 128, at most head_dim, at least head_dim / 4; page_size
+ * a power of two from 16 to 1024. */
+typedef struct {
+    uint8_t *pool;
+    uint64_t num_pages;
+    uint32_t kv_heads, head_dim, page_size, group;
+    int32_t *status;
+} cora_kv4_cache;
+
+uint64_t cora_kv4_block_bytes(uint32_t page_size, uint32_t head_dim, uint32_t group);
+/* Synchronises `stream`, reports and clears the status word: CORA_ERUNTIME if a bit is set. */
+int cora_kv4_status(const cora_kv4_cache *cache, void *stream);
+
+/* Rotates keys and queries by position, quantises keys and values, stores them at their slots
+ * (slot = page * page_size + offset; negative: the token is not stored). Pairs (i, i + rotary/2)
+ * of the first `rotary` dimensions are turned, or (2i, 2i + 1) when interleaved, by the row
+ * `positions[token]` of the fp32 tables (rope_rows x rotary / 2); rotary is 0 (no rotation) or a
+ * multiple of 16. Strides are in elements; the dimension's own stride is 1. q may be null; k_out
+ * and v_out (the values the stored codes stand for), each tokens x kv_heads x head_dim, too;
+ * q_out is tokens x q_heads x head_dim. Outputs are contiguous and must not overlap inputs. */
+typedef struct {
+    const void *k, *v, *q;
+    void *k_out, *v_out, *q_out;
+    int64_t k_token, k_head, v_token, v_head, q_token, q_head;
+    const int64_t *slots;
+    const int32_t *positions;
+    const float *rope_cos, *rope_sin;
+    uint64_t tokens, rope_rows;
+    uint32_t q_heads, rotary, interleaved, dtype;
+} cora_kv4_append_args;
+int cora_kv4_append(const cora_kv4_cache *cache, const cora_kv4_append_args *args, void *stream);
+
+/* Softmax attention over the cache. Sequence b holds lens[b] cached tokens, token j in page
+ * page_table[b * table_stride + j / page_size]; its query tokens are rows
+ * [q_start[b], q_start[b + 1]) of q (q_start null: row b), the last ones of the sequence: the
+ * i-th of n is at position lens[b] - n + i. causal: a query sees tokens up to its position;
+ * window w > 0 (causal only): the last w of those. A query that sees none gives zeros (lse
+ * -inf). Query heads h * q_heads / kv_heads .. share key head h. out is q_tokens x q_heads x
+ * head_dim, lse (natural log of the sum of exponentials; may be null) q_tokens x q_heads, both
+ * contiguous. max_queries: an upper bound on the query tokens of a sequence.
+ * workspace: cora_kv4_attend_workspace() bytes, zero before its first use; left ready for the
+ * next call. Calls that overlap in time need workspaces of their own. */
+typedef struct {
+    const void *q;
+    void *out;
+    float *lse;
+    int64_t q_token, q_head;
+    const int32_t *page_table, *lens, *q_start;
+    int64_t table_stride;
+    uint64_t q_tokens, workspace_bytes;
+    void *workspace;
+    float scale;
+    uint32_t seqs, table_width, q_heads, max_queries, window, causal, dtype;
+} cora_kv4_attend_args;
+uint64_t cora_kv4_attend_workspace(const cora_kv4_cache *cache);
+int cora_kv4_attend(const cora_kv4_cache *cache, const cora_kv4_attend_args *args, void *stream);
+
+/* A rows x cols weight matrix in 4 bits. Columns are padded to a multiple of 128 (codes 0,
+ * factors 0); group 32, 64 or 128. codes: rows x padded / 2 bytes, 16-byte aligned; a segment of
+ * 128 columns is 16 words of 32 bits, the word at 4t + j holding columns 32j + 8t .. + 7, of
+ * which column e is nibble {0, 4, 2, 6, 1, 5, 3, 7}[e]. meta: rows x padded / group pairs of
+ * fp16 (scale, low). */
+typedef struct {
+    const uint8_t *codes;
+    const void *meta;
+    uint64_t rows, cols;
+    uint32_t group;
+} cora_w4_weight;
+/* y[m] = weight x[m] (+ bias) for `rows` activation rows (fp32 sums, rounded once); strides in
+ * elements. */
+typedef struct {
+    const void *x, *bias;
+    void *y;
+    int64_t x_stride, y_stride;
+    uint64_t rows;
+    uint32_t dtype;
+} cora_w4_matvec_args;
+int cora_w4_matvec(const cora_w4_weight *weight, const cora_w4_matvec_args *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
