@@ -21,7 +21,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from . import InvalidArgument, _check, _lib
+from . import CoraRuntimeError, InvalidArgument, _check, _lib
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 # Nibble of a 32-bit word that holds column e of its eight (see Weight4).
@@ -71,7 +71,7 @@ def _bind(L):
         f.restype, f.argtypes = C.c_int, list(args)
     L.cora_kv4_block_bytes.restype, L.cora_kv4_block_bytes.argtypes = C.c_uint64, [C.c_uint32] * 3
     L.cora_kv4_attend_workspace.restype = C.c_uint64
-    L.cora_kv4_attend_workspace.argtypes = [C.POINTER(_CacheArg)]
+    L.cora_kv4_attend_workspace.argtypes = [C.POINTER(_CacheArg), C.c_uint32, C.c_uint32]
 
 
 def _need(ok, what):
@@ -145,7 +145,7 @@ class Cache4:
         self._arg = _CacheArg(pool.data_ptr(), num_pages, kv_heads, head_dim, page_size, group,
                               self.status.data_ptr())
         self._ref = C.byref(self._arg)
-        self._work = {}  # stream -> workspace of attend: calls on different streams may overlap
+        self._work = {}  # attend's workspaces, one per stream (calls on different streams may overlap)
 
     def _heads(self, x, what, heads=None):
         _need(x.dim() == 3 and x.shape[2] == self.head_dim and (heads is None or x.shape[1] == heads)
@@ -226,26 +226,34 @@ class Cache4:
             lse = torch.empty(T, Hq, dtype=torch.float32, device=self.device)
             a.lse = lse.data_ptr()
         stream = torch.cuda.current_stream(self.device).cuda_stream
-        work = self._work.get(stream)
-        if work is None:
-            work = self._workspace(stream)
+        key = (stream, Hq, max_queries)
+        work = self._work.get(key) or self._workspace(key)
         a.workspace, a.workspace_bytes = work
         _call(_lib.cora_kv4_attend, self.device, self._ref, C.byref(a))
         return (out, lse) if return_lse else out
 
-    def _workspace(self, stream):
+    def _workspace(self, key):
+        """The stream's workspace, made larger where this shape of call needs more."""
+        stream, heads, queries = key
         with torch.cuda.device(self.device):
-            size = int(_lib.cora_kv4_attend_workspace(self._ref))
-        _need(size > 0, "cache is not valid")
-        buf = torch.zeros(size, dtype=torch.uint8, device=self.device)
-        self._work[stream] = work = (buf.data_ptr(), size)
-        self._work[stream, "tensor"] = buf
+            size = int(_lib.cora_kv4_attend_workspace(self._ref, heads, queries))
+        _need(size > 0, "q_heads must be a multiple of kv_heads")
+        buf = self._work.get(stream)
+        if buf is None or buf.numel() < size:
+            self._work[stream] = buf = torch.zeros(size, dtype=torch.uint8, device=self.device)
+            for k in [k for k in self._work if isinstance(k, tuple) and k[0] == stream]:
+                del self._work[k]
+        self._work[key] = work = (buf.data_ptr(), buf.numel())
         return work
 
     def check(self):
         """Synchronise the current stream; raise if a call met a bad slot, page, position or row
         range, or if a wait ran out, since the last check."""
-        _call(_lib.cora_kv4_status, self.device, self._ref)
+        try:
+            _call(_lib.cora_kv4_status, self.device, self._ref)
+        except CoraRuntimeError:
+            self._work.clear()  # a call that gave up may have left its workspace unready
+            raise
 
 
 class Weight4:

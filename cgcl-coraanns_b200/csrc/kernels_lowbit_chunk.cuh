@@ -1,0 +1,674 @@
+// Attention of many query rows per key head over the paged 4-bit cache: cora_kv4_attend for
+// chunks of a prompt, drafted tokens and wide head groups (more than 8 rows per key head).
+//
+// Bound by the tensor cores and, next to them, by exponentials (16 a clock and SM) and by shared
+// memory. Rows (query token, head of the group) fill tiles of 128; one block takes kNQ = 2 tiles
+// (1 for few rows or head size 256) against the same keys, so each unpacked key tile serves 256
+// rows. Warp roles:
+//   0-3, 4-7  softmax of row tile 0 / 1: one thread per row; sums of q . c from TMEM, the
+//             token's factors from shared memory, running maximum and sum in fp32,
+//             probabilities back to TMEM as the fp16 operand of the second product. One pass:
+//             probabilities refer to the maximum met before; only where it grows by more than
+//             2^8 are the sums (and the tile's earlier probabilities) rescaled, so that they
+//             stay below 2^8, which fp16 holds.
+//   8-15      unpack, into 128-byte swizzled tiles: key codes as the fp16 subnormals c 2^-24 and
+//             c 2^-20, exact (the scores keep fp32 accuracy); value codes to fp16 scale c + low,
+//             one rounding each (2^-12 of the value, as of the probability; values past 65504
+//             do not fit).
+//   16        copies code tiles from the cache's pages (bulk copies into a ring).
+//   17        issues the tcgen05 products: S_g = Q_g C_g^T per factor group (keys K-major) and
+//             O += P V (P in TMEM, values as stored, token-major: the N-major operand).
+// Units (sequence, key head, row tile, token tile) are cut into equal runs, one per block; a job
+// cut over blocks is joined by the last to arrive. Every wait is bounded.
+//
+// Within 8 dimensions, operands and accumulator hold the order 0 4 1 5 2 6 3 7: two nibbles of a
+// word that one AND isolates are neighbours.
+#pragma once
+#include "kernels_lowbit_attend.cuh"
+#include "umma.cuh"
+
+namespace cora {
+
+constexpr int kCkThreads = 576, kCkMinRun = 2;
+
+template <int D, int kNG, int kNQ>
+struct ChunkSmem {
+    static constexpr int kTN = 128 / kNG;                           // tokens of a tile: 128 columns of scores
+    static constexpr uint32_t kQ = 128 * D * 2, kSlot = kTN * D * 2;
+    static constexpr int kSlots = (kNQ * kQ + 4 * kSlot <= 160 * 1024) ? 4 : 3;
+    static constexpr int kRaw = 3;
+    static constexpr uint32_t kCodes = kTN * D / 2, kMeta = kTN * kNG * 4;
+    static constexpr uint32_t kRawBytes = 2 * kCodes + 2 * kMeta;
+    static constexpr uint32_t q = 0;
+    static constexpr uint32_t slot = q + kNQ * kQ;
+    static constexpr uint32_t raw = slot + kSlots * kSlot;
+    static constexpr uint32_t fac = raw + kRaw * kRawBytes;         // [4][scale | low][kNG][kTN] of the keys
+    static constexpr uint32_t poison = fac + 4 * 2 * kNG * kTN * 4; // [4][4] bits: token's value is not finite
+    static constexpr uint32_t misc = poison + 64;                   // tmem slot, last-to-arrive flags
+    static constexpr uint32_t bars = misc + 32;
+    static constexpr uint32_t base = bars + 256;                    // int64[seqs + 1]
+    static constexpr size_t bytes(uint32_t seqs) { return 1024 + base + 8 * (size_t)(seqs + 1); }
+};
+
+// One block's stretch of one job.
+struct Segment {
+    SeqWork s;
+    int seq, head, row0, rows;       // rows: of this job's tiles (<= 128 kNQ)
+    int tok0, tiles;                 // first token and tiles of the stretch
+    int64_t u0, job_u0, job_u1;      // unit of its first tile; units of the whole job
+    bool first, last;                // holds the job's first / last tile
+};
+
+// Walks the stretches of units [u, end); every role of a block sees the same ones.
+template <int kTN, int kRows>
+struct Walker {
+    const AttendParams &p;
+    const int64_t *base;
+    int64_t u, end;
+    int b = -1;
+    SeqWork s{};
+    // tokens that row tile rt's queries see: [lo, hi)
+    __device__ static int2 sees(const AttendParams &p, const SeqWork &s, int rt) {
+        const int heads = p.a.q_heads / p.c.kv_heads;
+        const int i0 = rt * kRows / heads, i1 = min(s.n * heads, (rt + 1) * kRows) - 1;
+        const int first = s.len - s.n + i0, last = s.len - s.n + i1 / heads;
+        const int hi = p.a.causal ? max(0, min(s.len, last + 1)) : s.len;
+        const int lo = p.a.window ? min(hi, max(0, first - (int)p.a.window + 1)) : 0;
+        return make_int2(lo, hi);
+    }
+    __device__ static int tiles(int2 r) { return max(1, (r.y + kTN - 1) / kTN - r.x / kTN); }
+    __device__ static int64_t units_of_head(const AttendParams &p, const SeqWork &s) {
+        int64_t n = 0;
+        for (int rt = 0; rt < s.row_tiles; ++rt) n += tiles(sees(p, s, rt));
+        return n;
+    }
+    __device__ bool next(Segment &g) {
+        if (u >= end) return false;
+        if (b < 0 || u >= base[b + 1]) {
+            int lo = 0, hi = (int)p.seqs - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi) / 2;
+                if (base[mid + 1] > u) hi = mid;
+                else lo = mid + 1;
+            }
+            b = lo;
+            s = seq_work(p, b, kRows);
+        }
+        const int64_t per_head = (base[b + 1] - base[b]) / p.c.kv_heads, r = u - base[b];
+        g.s = s;
+        g.seq = p.seq0 + b;
+        g.head = (int)(r / per_head);
+        int64_t at = base[b] + g.head * per_head;
+        int rt = 0;
+        int2 see = sees(p, s, 0);
+        while (at + tiles(see) <= u) {
+            at += tiles(see);
+            see = sees(p, s, ++rt);
+        }
+        g.row0 = rt * kRows;
+        g.rows = min(kRows, s.n * (int)(p.a.q_heads / p.c.kv_heads) - g.row0);
+        g.job_u0 = at;
+        g.job_u1 = at + tiles(see);
+        g.u0 = u;
+        const int64_t stop = min(end, g.job_u1);
+        g.tok0 = (see.x / kTN + (int)(u - at)) * kTN;
+        g.tiles = (int)(stop - u);
+        g.first = u == at;
+        g.last = stop == g.job_u1;
+        u = stop;
+        return true;
+    }
+};
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<uint64_t &>(d))
+        : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)), "l"(reinterpret_cast<uint64_t &>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t &>(d))
+        : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t &>(d))
+        : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)));
+    return d;
+}
+
+template <typename T, int D, int kNG, int kNQ>
+__global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendParams p) {
+    using S = ChunkSmem<D, kNG, kNQ>;
+    constexpr int kTN = S::kTN, kRows = 128 * kNQ, kG = D / kNG;
+    constexpr uint32_t kQBlock = 128 * 128, kTBlock = kTN * 128;  // bytes of 64 dimensions of a tile
+    constexpr uint32_t kOCol = 0, kSCol = kNQ * D;                // TMEM columns: O tiles, then S buffers
+    constexpr uint32_t kSCols = kNG * kTN;                        // of one buffer: a block per group
+    static_assert(kNQ * D + 2 * kSCols <= 512, "");
+    extern __shared__ unsigned char ck_raw[];
+    unsigned char *sm = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(ck_raw) + 1023) & ~uintptr_t(1023));
+    float *fac = reinterpret_cast<float *>(sm + S::fac);
+    volatile uint32_t *poison = reinterpret_cast<volatile uint32_t *>(sm + S::poison);
+    volatile uint32_t *misc = reinterpret_cast<volatile uint32_t *>(sm + S::misc);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(sm + S::bars);
+    uint64_t *raw_full = bars, *raw_empty = raw_full + S::kRaw;
+    uint64_t *deq_full = raw_empty + S::kRaw, *deq_empty = deq_full + S::kSlots;
+    uint64_t *q_full = deq_empty + S::kSlots, *o_free = q_full + 2;
+    uint64_t *s_full = o_free + 2, *p_full = s_full + 2, *pv_done = p_full + 2, *mma_done = pv_done + 2;
+    static_assert((2 * S::kRaw + 2 * S::kSlots + 11) * 8 <= 256, "");
+    int64_t *base = reinterpret_cast<int64_t *>(sm + S::base);
+    int *err = p.c.status;
+
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int H = p.c.kv_heads, heads = p.a.q_heads / H, P = p.c.page_size;
+    using Walk = Walker<kTN, kRows>;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::kRaw; ++i) mbar_init(raw_full + i, 1), mbar_init(raw_empty + i, 8);
+        for (int i = 0; i < S::kSlots; ++i) mbar_init(deq_full + i, 8), mbar_init(deq_empty + i, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(q_full + i, 128), mbar_init(o_free + i, 128), mbar_init(s_full + i, 1);
+            mbar_init(p_full + i, 128), mbar_init(pv_done + i, 1);
+        }
+        mbar_init(mma_done, 1);
+        fence_barrier_init();
+    }
+    if (warp == 17) tmem_alloc(const_cast<uint32_t *>(misc), 512);
+    if (warp == 0) {  // unit offsets of the sequences
+        int64_t run = 0;
+        if (lane == 0) base[0] = 0;
+        for (int b0 = 0; b0 < (int)p.seqs; b0 += 32) {
+            int64_t v = 0;
+            if (b0 + lane < (int)p.seqs) v = Walk::units_of_head(p, seq_work(p, b0 + lane, kRows)) * H;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const int64_t o = __shfl_up_sync(0xffffffffu, v, off);
+                if (lane >= off) v += o;
+            }
+            if (b0 + lane < (int)p.seqs) base[b0 + lane + 1] = run + v;
+            run += __shfl_sync(0xffffffffu, v, 31);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = misc[0];
+    const int64_t units = base[p.seqs], blocks = max((int64_t)1, min((int64_t)gridDim.x, units / kCkMinRun));
+    const int64_t u0 = blockIdx.x < blocks ? blockIdx.x * units / blocks : 0;
+    const int64_t u1 = blockIdx.x < blocks ? (blockIdx.x + 1) * units / blocks : 0;
+    Walk walk{p, base, u0, u1};
+    Segment g;
+
+    if (warp < 4 * kNQ) {
+        // ---------------- softmax: thread = row of tile q ----------------
+        const int q = warp / 4, row = (warp % 4) * 32 + lane;
+        const uint32_t lanes = tmem + (uint32_t((warp % 4) * 32) << 16);
+        const uint32_t t_o = lanes + kOCol + q * D;
+        unsigned char *sq = sm + S::q + q * S::kQ;
+        const bool vec = reinterpret_cast<uintptr_t>(p.a.q) % 16 == 0 && p.a.q_token % 8 == 0 && p.a.q_head % 8 == 0;
+        const float f0 = fabsf(p.a.scale) * kLog2e;
+        const float sign = p.a.scale < 0.0f ? -1.0f : 1.0f;
+        T *out = static_cast<T *>(p.a.out);
+        uint32_t tile_no = 0;  // tiles this thread has done (phases of the barriers)
+        bool ok = true;
+        while (ok && walk.next(g)) {
+            const int r = q * 128 + row, grow = g.row0 + r;
+            const bool in = r < g.rows;
+            const int i = in ? grow / heads : 0, hh = g.head * heads + (in ? grow % heads : 0);
+            const T *src = static_cast<const T *>(p.a.q) + (int64_t)(g.s.q0 + i) * p.a.q_token + (int64_t)hh * p.a.q_head;
+            // the row under its own power of two, largest |q| in [2^13, 2^14)
+            float big = 0.0f;
+            for (int d = 0; d < D; d += 8) {
+                float x[8];
+                if (vec) load8<T, true>(src + d, x);
+                else load8<T, false>(src + d, x);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) big = fabsf(x[e]) < 3.4e38f ? fmaxf(big, fabsf(x[e])) : big;
+            }
+            const int qe = big > 0.0f ? max(-100, min(126, 13 - ilogbf(big))) : 0;
+            const float qpow = in ? ldexpf(sign, qe) : 0.0f;
+            float qs[kNG];  // sums of q per group, in the units of the products
+#pragma unroll
+            for (int gr = 0; gr < kNG; ++gr) {
+                float sum = 0.0f;
+                for (int d = gr * kG; d < (gr + 1) * kG; d += 8) {
+                    float x[8];
+                    if (vec) load8<T, true>(src + d, x);
+                    else load8<T, false>(src + d, x);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        x[e] *= qpow;
+                        sum += x[e];
+                    }
+                    const float odd = 0.0625f;  // against the odd nibbles' 2^-20
+                    uint4 w;
+                    w.x = pack_half2(x[0], x[4]), w.y = pack_half2(x[1] * odd, x[5] * odd);
+                    w.z = pack_half2(x[2], x[6]), w.w = pack_half2(x[3] * odd, x[7] * odd);
+                    if (!in) w = make_uint4(0, 0, 0, 0);
+                    const int c = (d / 8) & 7;
+                    *reinterpret_cast<uint4 *>(sq + (d / 64) * kQBlock + row * 128 + ((c ^ (row & 7)) << 4)) = w;
+                }
+                qs[gr] = in ? sum * 5.9604644775390625e-8f : 0.0f;  // 2^-24
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(q_full + q);
+            const float f = ldexpf(f0, 24 - qe);
+            const int pos = g.s.len - g.s.n + i;
+            const int hi = !in ? 0x7fffffff : p.a.causal ? max(0, min(g.s.len, pos + 1)) : g.s.len;
+            const int lo = in && p.a.window ? max(0, pos - (int)p.a.window + 1) : 0;
+            const int hi_min = __reduce_min_sync(0xffffffffu, hi), lo_max = __reduce_max_sync(0xffffffffu, lo);
+            float m = -INFINITY, l = 0.0f;
+            for (int j = 0; j < g.tiles && ok; ++j, ++tile_no) {
+                const int buf = kNQ == 2 ? q : (int)(tile_no & 1);
+                const uint32_t sph = kNQ == 2 ? tile_no & 1 : (tile_no >> 1) & 1;
+                const uint32_t t_s = lanes + kSCol + buf * kSCols;
+                const int tok0 = g.tok0 + j * kTN;
+                const bool edge = tok0 + kTN > hi_min || tok0 < lo_max;
+                ok = __all_sync(0xffffffffu, mbar_wait_bounded(s_full + buf, sph, err));
+                if (!ok) break;
+                tc_fence_after();
+                const float *tf = fac + (tile_no & 3) * 2 * kNG * kTN;
+                float2 ls = make_float2(0.0f, 0.0f);
+#pragma unroll 1
+                for (int c = 0; c < kTN / 32; ++c) {
+                    // scores of 32 tokens, in units of 1 / f
+                    uint32_t x[32];
+                    float2 u[16];
+                    tmem_ld32_async(t_s + c * 32, x);
+                    tmem_wait_ld(x);
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) {
+                        const float4 s4 = *reinterpret_cast<const float4 *>(tf + c * 32 + e);
+                        const float4 l4 = *reinterpret_cast<const float4 *>(tf + kNG * kTN + c * 32 + e);
+                        const float2 qq = make_float2(qs[0], qs[0]);
+                        u[e / 2] = fma2(make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), make_float2(s4.x, s4.y),
+                                        mul2(make_float2(l4.x, l4.y), qq));
+                        u[e / 2 + 1] = fma2(make_float2(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])),
+                                            make_float2(s4.z, s4.w), mul2(make_float2(l4.z, l4.w), qq));
+                    }
+#pragma unroll
+                    for (int gr = 1; gr < kNG; ++gr) {
+                        tmem_ld32_async(t_s + gr * kTN + c * 32, x);
+                        tmem_wait_ld(x);
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) {
+                            const float4 s4 = *reinterpret_cast<const float4 *>(tf + gr * kTN + c * 32 + e);
+                            const float4 l4 = *reinterpret_cast<const float4 *>(tf + (kNG + gr) * kTN + c * 32 + e);
+                            const float2 qq = make_float2(qs[gr], qs[gr]);
+                            u[e / 2] = fma2(make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), make_float2(s4.x, s4.y),
+                                            fma2(make_float2(l4.x, l4.y), qq, u[e / 2]));
+                            u[e / 2 + 1] = fma2(make_float2(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])),
+                                                make_float2(s4.z, s4.w), fma2(make_float2(l4.z, l4.w), qq, u[e / 2 + 1]));
+                        }
+                    }
+                    uint32_t hidden = 0;
+                    if (edge) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            const int t0 = tok0 + c * 32 + e;
+                            if (t0 < lo || t0 >= hi) {
+                                (e & 1 ? u[e / 2].y : u[e / 2].x) = -INFINITY;
+                                hidden |= 1u << e;
+                            }
+                        }
+                    }
+                    float tm = -INFINITY, t2 = -INFINITY;
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        tm = fmaxf(fmaxf(tm, u[e].x), u[e].y);
+                        t2 = fmaxf(fmaxf(t2, u[e + 1].x), u[e + 1].y);
+                    }
+                    tm = fmaxf(tm, t2);
+                    tm = tm == -INFINITY ? tm : tm * f;
+                    const bool grew = tm > m + 8.0f || (m == -INFINITY && tm > m);
+                    if (__any_sync(0xffffffffu, grew)) {
+                        // rescale the row's sums, this tile's earlier probabilities among them
+                        const float k = grew ? ex2(m - tm) : 1.0f;
+                        if (grew) m = tm;
+                        l *= k, ls.x *= k, ls.y *= k;
+                        tmem_wait_st();
+#pragma unroll 1
+                        for (int cc = 0; cc < c; ++cc) {
+                            uint32_t w[16];
+                            tmem_ld16(t_s + cc * 16, w);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) {
+                                const float2 h = __half22float2(*reinterpret_cast<__half2 *>(&w[e]));
+                                w[e] = pack_half2(h.x * k, h.y * k);
+                            }
+                            tmem_st16(t_s + cc * 16, w);
+                        }
+                        if (j > 0) {
+                            ok = __all_sync(0xffffffffu, mbar_wait_bounded(pv_done + q, (tile_no - 1) & 1, err));
+                            if (!ok) break;
+                            tc_fence_after();
+#pragma unroll 1
+                            for (int d = 0; d < D; d += 16) {
+                                uint32_t w[16];
+                                tmem_ld16(t_o + d, w);
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) * k);
+                                tmem_st16(t_o + d, w);
+                            }
+                        }
+                        tmem_wait_st();
+                    }
+                    const float mr = m == -INFINITY ? 0.0f : -m;
+                    uint32_t w[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        float2 pr = fma2(u[e], make_float2(f, f), make_float2(mr, mr));
+                        pr.x = ex2(pr.x), pr.y = ex2(pr.y);
+                        if (edge) {
+                            if (hidden >> (2 * e) & 1) pr.x = 0.0f;
+                            if (hidden >> (2 * e + 1) & 1) pr.y = 0.0f;
+                        }
+                        ls = add2(ls, pr);
+                        w[e] = pack_half2(pr.x, pr.y);
+                    }
+                    tmem_st16(t_s + c * 16, w);
+                }
+                if (!ok) break;
+                l += ls.x + ls.y;
+                // values that are not finite are kept out of the product: rows that see one say so here
+                {
+                    const volatile uint32_t *bits = poison + 4 * (tile_no & 3);
+                    uint32_t any = 0;
+#pragma unroll
+                    for (int c = 0; c < kTN / 32; ++c) any |= bits[c];
+                    if (any) {
+                        for (int e = 0; e < kTN; ++e)
+                            if ((bits[e / 32] >> (e % 32) & 1) && tok0 + e >= lo && tok0 + e < hi) l = __int_as_float(0x7fc00000);
+                    }
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(p_full + buf);
+            }
+            if (!ok) break;
+            // ---- the stretch is done: result, or this block's part of it ----
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(pv_done + q, (tile_no - 1) & 1, err));
+            if (!ok) break;
+            tc_fence_after();
+            const bool whole = g.first && g.last;
+            T *dst = out + ((int64_t)(g.s.q0 + i) * p.a.q_heads + hh) * D;
+            const size_t slots = (size_t)2 * gridDim.x * kNQ;
+            const size_t sl = (size_t)(2 * blockIdx.x + (g.first ? 1 : 0)) * kNQ + q;
+            float *po = p.part + sl * D * 128 + row;
+            float2 *ps = reinterpret_cast<float2 *>(p.part + slots * D * 128) + sl * 128 + row;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+                uint32_t x[32];
+                tmem_ld32_async(t_o + c, x);
+                tmem_wait_ld(x);
+                if (!whole) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) __stcg(po + (c + e) * 128, __uint_as_float(x[e]));
+                } else if (in) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        float v[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) v[(k >> 1) + (k & 1) * 4] = l == 0.0f ? 0.0f : __uint_as_float(x[e + k]) * inv;
+                        store8(dst + c + e, v);
+                    }
+                }
+            }
+            tc_fence_before();
+            mbar_arrive(o_free + q);
+            if (whole) {
+                if (in && p.a.lse)
+                    p.a.lse[(int64_t)(g.s.q0 + i) * p.a.q_heads + hh] = l == 0.0f ? -INFINITY : (m + log2f(l)) / kLog2e;
+                continue;
+            }
+            __stcg(ps, make_float2(m, l));
+            __threadfence();
+            named_barrier_sync(1 + q, 128);
+            const int first = (int)(((g.job_u0 + 1) * blocks - 1) / units), last = (int)((g.job_u1 * blocks - 1) / units);
+            uint32_t *count = p.arrived + first * kNQ + q;
+            if (row == 0) misc[1 + q] = atomicAdd(count, 1u) == (uint32_t)(last - first);
+            named_barrier_sync(1 + q, 128);
+            if (misc[1 + q]) {
+                __threadfence();
+                if (row == 0) *count = 0;
+                const float2 *as = reinterpret_cast<const float2 *>(p.part + slots * D * 128) + row;
+                auto at = [&](int bk) { return (size_t)(2 * bk + (bk == first ? 1 : 0)) * kNQ + q; };
+                float jm = -INFINITY, jl = 0.0f;
+                for (int bk = first; bk <= last; ++bk) jm = fmaxf(jm, __ldcg(as + at(bk) * 128).x);
+                for (int bk = first; bk <= last; ++bk) {
+                    const float2 st = __ldcg(as + at(bk) * 128);
+                    jl += st.y * (st.x == -INFINITY ? (st.y == 0.0f ? 0.0f : 1.0f) : ex2(st.x - jm));
+                }
+                const float jinv = jl == 0.0f ? 0.0f : 1.0f / jl;
+#pragma unroll 1
+                for (int c = 0; c < D; c += 8) {
+                    float v[8] = {};
+                    for (int bk = first; bk <= last; ++bk) {
+                        const float sm_ = __ldcg(as + at(bk) * 128).x;
+                        const float k = sm_ == -INFINITY ? 0.0f : ex2(sm_ - jm);
+                        const float *src2 = p.part + at(bk) * D * 128 + (size_t)c * 128 + row;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[(e >> 1) + (e & 1) * 4] = fmaf(k, __ldcg(src2 + e * 128), v[(e >> 1) + (e & 1) * 4]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = jl == 0.0f ? 0.0f : v[e] * jinv;
+                    if (in) store8(dst + c, v);
+                }
+                if (in && p.a.lse)
+                    p.a.lse[(int64_t)(g.s.q0 + i) * p.a.q_heads + hh] = jl == 0.0f ? -INFINITY : (jm + log2f(jl)) / kLog2e;
+            }
+            named_barrier_sync(1 + q, 128);  // misc is free again
+        }
+    } else if (warp >= 8 && warp < 16) {
+        // ---------------- unpack ----------------
+        const int tid = threadIdx.x - 256, t3 = lane & 7, quarter0 = lane >> 3;
+        const int rot = D == 128 ? t3 >> 1 : D == 256 ? t3 : 0;  // 16-byte reads and writes of 8 lanes hit all banks
+        constexpr int kQuads = D / 32;                            // 16-byte pieces of a token's codes
+        uint32_t raw_no = 0, item = 0;
+        bool ok = true;
+        while (ok && walk.next(g)) {
+            int see_lo = 0x7fffffff, see_hi = 0;  // tokens that any row of this job sees
+            {
+                const int2 see = Walk::sees(p, g.s, g.row0 / kRows);
+                see_lo = see.x, see_hi = see.y;
+            }
+            for (int j = 0; j < g.tiles && ok; ++j, ++raw_no) {
+                const int rs = raw_no % S::kRaw, tok0 = g.tok0 + j * kTN;
+                const unsigned char *rw = sm + S::raw + rs * S::kRawBytes;
+                ok = mbar_wait_bounded(raw_full + rs, (raw_no / S::kRaw) & 1, err);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv, ++item) {
+                    const int sl = item % S::kSlots;
+                    ok = mbar_wait_bounded(deq_empty + sl, ((item / S::kSlots) & 1) ^ 1, err);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    unsigned char *dst = sm + S::slot + sl * S::kSlot;
+                    const unsigned char *codes = rw + kv * S::kCodes;
+                    const __half2 *meta = reinterpret_cast<const __half2 *>(rw + 2 * S::kCodes + kv * S::kMeta);
+                    if (kv == 0 && tid < kTN) {  // the keys' factors; which values are not finite
+                        const __half2 *vm = reinterpret_cast<const __half2 *>(rw + 2 * S::kCodes + S::kMeta);
+                        float *tf = fac + (raw_no & 3) * 2 * kNG * kTN;
+                        const int tok = tok0 + tid;
+                        const bool seen = tok >= see_lo && tok < see_hi;
+                        bool bad = false;
+#pragma unroll
+                        for (int gr = 0; gr < kNG; ++gr) {
+                            const float2 kf = __half22float2(meta[tid * kNG + gr]);
+                            tf[gr * kTN + tid] = seen ? kf.x : 0.0f;
+                            tf[(kNG + gr) * kTN + tid] = seen ? kf.y : 0.0f;
+                            const uint32_t u = *reinterpret_cast<const uint32_t *>(vm + tid * kNG + gr);
+                            bad |= (u & 0x7c00u) == 0x7c00u || (u & 0x7c000000u) == 0x7c000000u;
+                        }
+                        const uint32_t bits = __ballot_sync(0xffffffffu, bad && seen);
+                        if (lane == 0) poison[4 * (raw_no & 3) + tid / 32] = bits;
+                    }
+#pragma unroll
+                    for (int it = 0; it < kTN * kQuads / 256; ++it) {
+                        // 8 tokens x 4 pieces per warp and step
+                        const int step = it * 8 + (warp - 8);
+                        constexpr int kParts = kQuads > 4 ? kQuads / 4 : 1;
+                        const int tg8 = step / kParts, part = step % kParts;
+                        int tk, quad;
+                        if (kQuads == 2) {  // 16 tokens x 2 pieces
+                            tk = step * 16 + (quarter0 >> 1) * 8 + t3;
+                            quad = quarter0 & 1;
+                        } else {
+                            tk = tg8 * 8 + t3;
+                            quad = (part * 4 + quarter0 + rot) & (kQuads - 1);
+                        }
+                        const uint4 w4 = *reinterpret_cast<const uint4 *>(codes + tk * (D / 2) + quad * 16);
+                        const uint32_t ws[4] = {w4.x, w4.y, w4.z, w4.w};
+                        __half2 sc, lw;
+                        if (kv) {
+                            const int tok = tok0 + tk;
+                            __half2 f = meta[tk * kNG + quad * 32 / kG];
+                            const uint32_t fu = *reinterpret_cast<const uint32_t *>(&f);
+                            const bool bad = (fu & 0x7c00u) == 0x7c00u || (fu & 0x7c000000u) == 0x7c000000u;
+                            // unseen tokens count as 0, and so do values that are marked above
+                            if (tok < see_lo || tok >= see_hi || bad) f = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
+                            sc = __low2half2(f), lw = __high2half2(f);
+                        }
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t w = ws[k], w8 = w >> 8;
+                            uint32_t o[4] = {w & 0x000f000fu, w & 0x00f000f0u, w8 & 0x000f000fu, w8 & 0x00f000f0u};
+                            if (kv) {
+                                const __half2 k1024 = __half2half2(__ushort_as_half(0x6400)), k64 = __half2half2(__ushort_as_half(0xd400));
+                                const __half2 sixteenth = __half2half2(__ushort_as_half(0x2c00));
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    o[e] |= 0x64006400u;  // 1024 + c or 1024 + 16 c
+                                    __half2 v = *reinterpret_cast<__half2 *>(&o[e]);
+                                    v = e & 1 ? __hfma2(v, sixteenth, k64) : __hsub2(v, k1024);
+                                    v = __hfma2(v, sc, lw);
+                                    o[e] = *reinterpret_cast<uint32_t *>(&v);
+                                }
+                            }
+                            const int chunk = quad * 4 + k, c = chunk & 7;
+                            *reinterpret_cast<uint4 *>(dst + (chunk >> 3) * kTBlock + tk * 128 + ((c ^ (tk & 7)) << 4)) =
+                                make_uint4(o[0], o[1], o[2], o[3]);
+                        }
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(deq_full + sl);
+                        if (kv) mbar_arrive(raw_empty + rs);
+                    }
+                }
+            }
+        }
+    } else if (warp == 16) {
+        // ---------------- copies from the pages ----------------
+        const Kv4Block blk(P, D, kG);
+        const int per = min(P, kTN), piece = lane >> 2, kind = lane & 3;
+        const uint32_t rowb = kind < 2 ? blk.code_row : blk.meta_row;
+        const uint32_t src_at = (kind & 1 ? (kind < 2 ? blk.codes : blk.metas) : 0) + (kind < 2 ? 0 : 2 * blk.codes);
+        const uint32_t dst_at = (kind & 1 ? (kind < 2 ? S::kCodes : S::kMeta) : 0) + (kind < 2 ? 0 : 2 * S::kCodes);
+        uint32_t raw_no = 0;
+        bool ok = true;
+        while (ok && walk.next(g)) {
+            for (int j = 0; j < g.tiles; ++j, ++raw_no) {
+                const int rs = raw_no % S::kRaw, tok0 = g.tok0 + j * kTN;
+                ok = __all_sync(0xffffffffu, mbar_wait_bounded(raw_empty + rs, ((raw_no / S::kRaw) & 1) ^ 1, err));
+                if (!ok) break;
+                const int pieces = max(0, min(kTN / per, (g.s.len - tok0 + per - 1) / per));
+                uint32_t bytes = 0;
+                const unsigned char *src = nullptr;
+                if (piece < pieces) {
+                    const int tok = tok0 + piece * per;
+                    const int page = __ldg(p.a.page_table + (int64_t)g.seq * p.a.table_stride + tok / P);
+                    if (page >= 0 && (uint64_t)page < p.c.num_pages) {
+                        src = p.c.pool + ((uint64_t)page * H + g.head) * blk.bytes + src_at + (uint32_t)(tok % P) * rowb;
+                        bytes = per * rowb;
+                    } else {
+                        atomicOr(err, kDevBadInput);
+                    }
+                }
+                const uint32_t total = __reduce_add_sync(0xffffffffu, bytes);
+                if (lane == 0) mbar_arrive_expect_tx(raw_full + rs, total);
+                __syncwarp();
+                if (bytes) bulk_g2s(sm + S::raw + rs * S::kRawBytes + dst_at + piece * per * rowb, src, bytes, raw_full + rs);
+            }
+        }
+        // the last copy into each stage has landed before the block exits
+        for (uint32_t k = raw_no > S::kRaw ? raw_no - S::kRaw : 0; k < raw_no; ++k)
+            mbar_wait_bounded(raw_full + k % S::kRaw, (k / S::kRaw) & 1, err);
+    } else if (warp == 17 && lane == 0) {
+        // ---------------- products ----------------
+        constexpr uint32_t id_qk = idesc_f16(128, kTN, false), id_pv = idesc_f16(128, D, true);
+        uint32_t seg_no = 0, done = 0;  // stretches and tiles before this one
+        bool ok = true;
+        auto slot_wait = [&](uint32_t item) {
+            const bool w = mbar_wait_bounded(deq_full + item % S::kSlots, (item / S::kSlots) & 1, err);
+            tc_fence_after();
+            return w;
+        };
+        auto buffer = [&](int q, uint32_t tile) { return kNQ == 2 ? q : (int)(tile & 1); };
+        auto qk = [&](int q, uint32_t tile) {  // scores of row tile q against key tile `tile`
+            const unsigned char *kt = sm + S::slot + (2 * tile) % S::kSlots * S::kSlot;
+            const uint64_t a0 = smem_desc_sw128(sm + S::q + q * S::kQ), b0 = smem_desc_sw128(kt);
+            const uint32_t d = tmem + kSCol + buffer(q, tile) * kSCols;
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+                const int gr = k / (kG / 16);
+                mma_f16(d + gr * kTN, a0 + (k / 4) * (kQBlock >> 4) + (k % 4) * 2, b0 + (k / 4) * (kTBlock >> 4) + (k % 4) * 2,
+                        id_qk, k % (kG / 16) != 0);
+            }
+            mma_commit(s_full + buffer(q, tile));
+            if (q == kNQ - 1) mma_commit(deq_empty + (2 * tile) % S::kSlots);
+        };
+        auto pv = [&](int q, uint32_t tile, bool add) {
+            const unsigned char *vt = sm + S::slot + (2 * tile + 1) % S::kSlots * S::kSlot;
+            const uint64_t b0 = smem_desc_sw128_mn(vt, kTBlock);
+            const uint32_t a = tmem + kSCol + buffer(q, tile) * kSCols;
+#pragma unroll
+            for (int k = 0; k < kTN / 16; ++k) mma_f16_ta(tmem + kOCol + q * D, a + k * 8, b0 + k * (2048 >> 4), id_pv, add || k != 0);
+            mma_commit(pv_done + q);
+            if (q == kNQ - 1) mma_commit(deq_empty + (2 * tile + 1) % S::kSlots);
+        };
+        while (ok && walk.next(g)) {
+            for (int q = 0; q < kNQ && ok; ++q) ok = mbar_wait_bounded(q_full + q, seg_no & 1, err);
+            tc_fence_after();
+            constexpr int kAhead = kNQ == 2 ? 1 : 2;  // score tiles issued ahead of the second product
+            for (int a = 0; a < min(kAhead, g.tiles) && ok; ++a) {
+                ok = slot_wait(2 * (done + a));
+                for (int q = 0; q < kNQ && ok; ++q) qk(q, done + a);
+            }
+            for (int j = 0; j < g.tiles && ok; ++j) {
+                const uint32_t tile = done + j;
+                for (int q = 0; q < kNQ && ok; ++q) {
+                    if (q == 0) ok = slot_wait(2 * tile + 1);
+                    if (j == 0 && ok) ok = mbar_wait_bounded(o_free + q, (seg_no & 1) ^ 1, err);
+                    if (ok) ok = mbar_wait_bounded(p_full + buffer(q, tile), kNQ == 2 ? tile & 1 : tile >> 1 & 1, err);
+                    if (!ok) break;
+                    tc_fence_after();
+                    pv(q, tile, j > 0);
+                    if (j + kAhead < g.tiles) {
+                        if (q == 0) ok = slot_wait(2 * (tile + kAhead));
+                        if (ok) qk(q, tile + kAhead);
+                    }
+                }
+            }
+            done += g.tiles;
+            ++seg_no;
+        }
+        mma_commit(mma_done);  // every product has finished before TMEM is freed
+        mbar_wait_bounded(mma_done, 0, err);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 17) tmem_dealloc(tmem, 512);
+}
+
+}  // namespace cora

@@ -4,6 +4,7 @@
 
 #include "kernels_lowbit_append.cuh"
 #include "kernels_lowbit_attend.cuh"
+#include "kernels_lowbit_chunk.cuh"
 #include "kernels_lowbit_matvec.cuh"
 #include "status.hpp"
 
@@ -103,11 +104,18 @@ void append(const cora_kv4_cache *c, const cora_kv4_append_args *a, cudaStream_t
 
 // ---- attend ------------------------------------------------------------------------------
 
-constexpr int kAttendMaxBlocksPerSm = 2;
-// Workspace: the arrival counters first (they are the part that has to start at zero).
-uint64_t attend_workspace(const cora_kv4_cache &c) {
-    const uint64_t blocks = (uint64_t)sm_count() * kAttendMaxBlocksPerSm;
-    return (blocks * 4 + 255) / 256 * 256 + 2 * blocks * 16 * (c.head_dim + 2) * 4;
+// Rows of one key head and sequence: few go to the streaming kernel, more to the tile kernel.
+uint64_t attend_rows(const cora_kv4_cache &c, uint64_t q_heads, uint64_t max_queries) {
+    return std::max<uint64_t>(1, max_queries) * (q_heads / c.kv_heads);
+}
+constexpr uint64_t kFewRows = 8;
+uint64_t attend_counters() { return ((uint64_t)sm_count() * 2 * 4 + 255) / 256 * 256; }
+// Workspace: the arrival counters first (they are the part that has to start at zero), then two
+// partial results per block.
+uint64_t attend_workspace(const cora_kv4_cache &c, uint64_t rows) {
+    const uint64_t blocks = sm_count();
+    const uint64_t parts = rows <= kFewRows ? 2 * (2 * blocks) * 8 : 2 * blocks * (rows <= 128 || c.head_dim == 256 ? 128 : 256);
+    return attend_counters() + parts * (c.head_dim + 2) * 4;
 }
 
 template <typename T, int D, int kNG, int kNT>
@@ -127,6 +135,22 @@ void launch_attend(AttendParams p, cudaStream_t st) {
     }
 }
 
+template <typename T, int D, int kNG, int kNQ>
+void launch_chunk(AttendParams p, cudaStream_t st) {
+    auto *kern = kv4_chunk_kernel<T, D, kNG, kNQ>;
+    using S = ChunkSmem<D, kNG, kNQ>;
+    static_assert(S::bytes(kAtMaxSeqs) <= 232448, "");
+    static int seen[64] = {};
+    allow_smem(kern, S::bytes(kAtMaxSeqs), seen);
+    const uint32_t seqs = p.a.seqs;
+    for (uint32_t s0 = 0; s0 < seqs; s0 += kAtMaxSeqs) {
+        p.seq0 = s0;
+        p.seqs = std::min<uint32_t>(kAtMaxSeqs, seqs - s0);
+        kern<<<sm_count(), kCkThreads, S::bytes(p.seqs), st>>>(p);
+        CUDA_TRY(cudaGetLastError());
+    }
+}
+
 void attend(const cora_kv4_cache *c, const cora_kv4_attend_args *a, cudaStream_t st) {
     check_cache(c);
     need(a, "null arguments");
@@ -138,21 +162,22 @@ void attend(const cora_kv4_cache *c, const cora_kv4_attend_args *a, cudaStream_t
     need((uint64_t)a->table_width * c->page_size <= INT_MAX, "table_width * page_size must fit an int");
     need(!a->window || a->causal, "a window needs causal attention");
     need(a->window <= INT_MAX, "window must fit an int");
-    need(a->workspace && aligned16(a->workspace) && a->workspace_bytes >= attend_workspace(*c),
+    const uint64_t rows = attend_rows(*c, a->q_heads, a->max_queries);
+    need(a->workspace && aligned16(a->workspace) && a->workspace_bytes >= attend_workspace(*c, rows),
          "the workspace is smaller than cora_kv4_attend_workspace()");
     AttendParams p{};
     p.c = *c;
     p.a = *a;
     p.q_tokens = (int64_t)a->q_tokens;
     p.arrived = static_cast<uint32_t *>(a->workspace);
-    p.part = reinterpret_cast<float *>(static_cast<char *>(a->workspace) +
-                                       ((uint64_t)sm_count() * kAttendMaxBlocksPerSm * 4 + 255) / 256 * 256);
-    const uint64_t rows = (uint64_t)std::max(1u, a->max_queries) * (a->q_heads / c->kv_heads);
+    p.part = reinterpret_cast<float *>(static_cast<char *>(a->workspace) + attend_counters());
     by_dtype(a->dtype, [&](auto z) {
         using T = decltype(z);
         auto go = [&](auto d, auto ng) {
-            if (rows <= 8) launch_attend<T, decltype(d)::value, decltype(ng)::value, 1>(p, st);
-            else launch_attend<T, decltype(d)::value, decltype(ng)::value, 2>(p, st);
+            constexpr int D = decltype(d)::value, NG = decltype(ng)::value;
+            if (rows <= kFewRows) launch_attend<T, D, NG, 1>(p, st);
+            else if (rows <= 128 || D == 256) launch_chunk<T, D, NG, 1>(p, st);
+            else launch_chunk<T, D, NG, D == 256 ? 1 : 2>(p, st);
         };
         if (c->head_dim == 64) go(Int<64>{}, Int<1>{});
         else if (c->head_dim == 128 && c->group == 128) go(Int<128>{}, Int<1>{});
@@ -225,11 +250,11 @@ int cora_kv4_append(const cora_kv4_cache *cache, const cora_kv4_append_args *arg
     return cora::guarded([&] { cora::append(cache, args, static_cast<cudaStream_t>(stream)); });
 }
 
-uint64_t cora_kv4_attend_workspace(const cora_kv4_cache *cache) {
+uint64_t cora_kv4_attend_workspace(const cora_kv4_cache *cache, uint32_t q_heads, uint32_t max_queries) {
     uint64_t bytes = 0;
     const int rc = cora::guarded([&] {
         cora::check_cache(cache);
-        bytes = cora::attend_workspace(*cache);
+        bytes = cora::attend_workspace(*cache, cora::attend_rows(*cache, q_heads, max_queries));
     });
     return rc == CORA_OK ? bytes : 0;
 }

@@ -364,8 +364,10 @@ int cora_kv4_append(const cora_kv4_cache *cache, const cora_kv4_append_args *arg
  * -inf). Query heads h * q_heads / kv_heads .. share key head h. out is q_tokens x q_heads x
  * head_dim, lse (natural log of the sum of exponentials; may be null) q_tokens x q_heads, both
  * contiguous. max_queries: an upper bound on the query tokens of a sequence.
- * workspace: cora_kv4_attend_workspace() bytes, zero before its first use; left ready for the
- * next call. Calls that overlap in time need workspaces of their own. */
+ * workspace: cora_kv4_attend_workspace() bytes for this q_heads and max_queries, zero before its
+ * first use; left ready for the next call (of any shape it is large enough for). Calls that
+ * overlap in time need workspaces of their own. With more than 8 rows (query tokens x heads of a
+ * group) per key head, cached values are rounded to fp16 (past 65504 they become infinite). */
 typedef struct {
     const void *q;
     void *out;
@@ -378,7 +380,7 @@ typedef struct {
     float scale;
     uint32_t seqs, table_width, q_heads, max_queries, window, causal, dtype;
 } cora_kv4_attend_args;
-uint64_t cora_kv4_attend_workspace(const cora_kv4_cache *cache);
+uint64_t cora_kv4_attend_workspace(const cora_kv4_cache *cache, uint32_t q_heads, uint32_t max_queries);
 int cora_kv4_attend(const cora_kv4_cache *cache, const cora_kv4_attend_args *args, void *stream);
 
 /* A rows x cols weight matrix in 4 bits. Columns are padded to a multiple of 128 (codes 0,
