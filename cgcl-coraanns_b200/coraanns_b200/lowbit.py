@@ -17,11 +17,12 @@ reported by ``Cache4.check``. There is no CPU fallback.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import NamedTuple, Optional
 
 import torch
 
-from . import CoraRuntimeError, InvalidArgument, _check, _lib
+from . import CoraRuntimeError, InvalidArgument, _check, load_library
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 # Nibble of a 32-bit word that holds column e of its eight (see Weight4).
@@ -34,44 +35,49 @@ class _CacheArg(C.Structure):
                 ("status", C.c_void_p)]
 
 
-class _AppendArg(C.Structure):
-    _fields_ = ([(n, C.c_void_p) for n in ("k", "v", "q", "k_out", "v_out", "q_out")]
-                + [(n, C.c_int64) for n in ("k_token", "k_head", "v_token", "v_head", "q_token", "q_head")]
-                + [(n, C.c_void_p) for n in ("slots", "positions", "rope_cos", "rope_sin")]
-                + [("tokens", C.c_uint64), ("rope_rows", C.c_uint64)]
-                + [(n, C.c_uint32) for n in ("q_heads", "rotary", "interleaved", "dtype")])
-
-
-class _AttendArg(C.Structure):
-    _fields_ = ([(n, C.c_void_p) for n in ("q", "out", "lse")]
-                + [("q_token", C.c_int64), ("q_head", C.c_int64)]
-                + [(n, C.c_void_p) for n in ("page_table", "lens", "q_start")]
-                + [("table_stride", C.c_int64), ("q_tokens", C.c_uint64), ("workspace_bytes", C.c_uint64),
-                   ("workspace", C.c_void_p), ("scale", C.c_float)]
-                + [(n, C.c_uint32) for n in ("seqs", "table_width", "q_heads", "max_queries", "window",
-                                             "causal", "dtype")])
-
-
 class _WeightArg(C.Structure):
     _fields_ = [("codes", C.c_void_p), ("meta", C.c_void_p), ("rows", C.c_uint64), ("cols", C.c_uint64),
                 ("group", C.c_uint32)]
 
 
-class _MatvecArg(C.Structure):
-    _fields_ = [("x", C.c_void_p), ("bias", C.c_void_p), ("y", C.c_void_p), ("x_stride", C.c_int64),
-                ("y_stride", C.c_int64), ("rows", C.c_uint64), ("dtype", C.c_uint32)]
+# The per-call argument structs, packed in one go (field by field through ctypes costs several
+# microseconds a call): cora_kv4_append_args, cora_kv4_attend_args, cora_w4_matvec_args.
+_APPEND = struct.Struct("6Q6q4Q2Q4I").pack
+_ATTEND = struct.Struct("3Q2q3Qq3Qf7I").pack
+_MATVEC = struct.Struct("3Q2qQI4x").pack
 
 
 def _bind(L):
-    for name, args in (("cora_kv4_append", (C.POINTER(_CacheArg), C.POINTER(_AppendArg), C.c_void_p)),
-                       ("cora_kv4_attend", (C.POINTER(_CacheArg), C.POINTER(_AttendArg), C.c_void_p)),
-                       ("cora_w4_matvec", (C.POINTER(_WeightArg), C.POINTER(_MatvecArg), C.c_void_p)),
-                       ("cora_kv4_status", (C.POINTER(_CacheArg), C.c_void_p))):
+    ref, args = C.c_void_p, C.c_char_p
+    for name, types in (("cora_kv4_append", (ref, args, C.c_void_p)), ("cora_kv4_attend", (ref, args, C.c_void_p)),
+                        ("cora_w4_matvec", (ref, args, C.c_void_p)), ("cora_kv4_status", (ref, C.c_void_p))):
         f = getattr(L, name)
-        f.restype, f.argtypes = C.c_int, list(args)
+        f.restype, f.argtypes = C.c_int, list(types)
     L.cora_kv4_block_bytes.restype, L.cora_kv4_block_bytes.argtypes = C.c_uint64, [C.c_uint32] * 3
     L.cora_kv4_attend_workspace.restype = C.c_uint64
-    L.cora_kv4_attend_workspace.argtypes = [C.POINTER(_CacheArg), C.c_uint32, C.c_uint32]
+    L.cora_kv4_attend_workspace.argtypes = [ref, C.c_uint32, C.c_uint32]
+    return L
+
+
+_bound = None
+
+
+def _library():
+    global _bound
+    if _bound is None:
+        _bound = _bind(load_library())
+    return _bound
+
+
+try:  # the current stream's handle without a Stream object around it
+    from torch._C import _cuda_getCurrentRawStream as _stream
+except ImportError:
+    def _stream(index):
+        return torch.cuda.current_stream(index).cuda_stream
+
+
+def _refuse(what):
+    raise InvalidArgument(what)
 
 
 def _need(ok, what):
@@ -79,18 +85,20 @@ def _need(ok, what):
         raise InvalidArgument(what)
 
 
-def _call(f, device, *args):
-    """f(*args, stream) on the tensors' device and its current stream."""
-    if device.index == torch.cuda.current_device():
-        _check(f(*args, torch.cuda.current_stream(device).cuda_stream))
+def _call(f, index, *args):
+    """f(*args, stream) on device `index` and its current stream."""
+    if index == torch.cuda.current_device():
+        rc = f(*args, _stream(index))
     else:
-        with torch.cuda.device(device):
-            _check(f(*args, torch.cuda.current_stream(device).cuda_stream))
+        with torch.cuda.device(index):
+            rc = f(*args, _stream(index))
+    if rc:
+        _check(rc)
 
 
 def _index(t, what, dtype, shape, device):
-    _need(t.dtype == dtype and tuple(t.shape) == shape and t.device == device and t.is_contiguous(),
-          f"{what} must be a contiguous {dtype} tensor of shape {shape} on {device}")
+    if t.dtype is not dtype or t.shape != shape or t.device != device or not t.is_contiguous():
+        _refuse(f"{what} must be a contiguous {dtype} tensor of shape {shape} on {device}")
     return t.data_ptr()
 
 
@@ -128,13 +136,13 @@ class Cache4:
         return self
 
     def _setup(self, pool, num_pages, kv_heads, head_dim, page_size, group, device):
-        _bind(_lib)
+        self._lib = _library()
         _need(head_dim in (64, 128, 256), "head_dim must be 64, 128 or 256")
         _need(group in (64, 128) and group <= head_dim <= 4 * group, "group must be 64 or 128 and at most head_dim")
         _need(16 <= page_size <= 1024 and page_size & (page_size - 1) == 0,
               "page_size must be a power of two from 16 to 1024")
         _need(num_pages >= 1 and kv_heads >= 1, "num_pages and kv_heads must be positive")
-        block = int(_lib.cora_kv4_block_bytes(page_size, head_dim, group))
+        block = int(self._lib.cora_kv4_block_bytes(page_size, head_dim, group))
         if pool is None:
             pool = torch.zeros(num_pages, kv_heads, block, dtype=torch.uint8, device=device)
         _need(pool.shape[2] == block, f"a block of this shape has {block} bytes, the pool's have {pool.shape[2]}")
@@ -144,13 +152,14 @@ class Cache4:
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._arg = _CacheArg(pool.data_ptr(), num_pages, kv_heads, head_dim, page_size, group,
                               self.status.data_ptr())
-        self._ref = C.byref(self._arg)
+        self._ref = C.addressof(self._arg)
+        self._dev = self.device.index
         self._work = {}  # attend's workspaces, one per stream (calls on different streams may overlap)
 
-    def _heads(self, x, what, heads=None):
-        _need(x.dim() == 3 and x.shape[2] == self.head_dim and (heads is None or x.shape[1] == heads)
-              and x.device == self.device and x.stride(2) == 1,
-              f"{what} must be (tokens, {heads or 'heads'}, {self.head_dim}) on {self.device}, its last stride 1")
+    def _heads(self, x, what, shape):
+        """The type code of a (tokens, heads, head_dim) tensor."""
+        if x.shape != shape or x.device != self.device or x.stride(2) != 1:
+            _refuse(f"{what} must be {shape} on {self.device}, its last stride 1")
         return _DTYPES.get(x.dtype, 99)
 
     def append(self, k, v, slots, q=None, rope=None, positions=None, interleaved=False, values=False) -> Appended:
@@ -163,30 +172,38 @@ class Cache4:
         (tokens, heads, head_dim), returned rotated. values: also return the keys and values that
         the stored codes stand for, as k and v of the result. A slot may appear once.
         """
-        dt = self._heads(k, "k", self.kv_heads)
+        D, dev = self.head_dim, self.device
+        if k.dim() != 3:
+            _refuse(f"k must be (tokens, {self.kv_heads}, {D})")
         T = k.shape[0]
-        _need(self._heads(v, "v", self.kv_heads) == dt and v.shape[0] == T, "k and v must be alike")
-        a = _AppendArg(k=k.data_ptr(), v=v.data_ptr(), k_token=k.stride(0), k_head=k.stride(1),
-                       v_token=v.stride(0), v_head=v.stride(1), tokens=T, dtype=dt,
-                       slots=_index(slots, "slots", torch.int64, (T,), self.device))
+        shape = (T, self.kv_heads, D)
+        dt = self._heads(k, "k", shape)
+        if self._heads(v, "v", shape) != dt:
+            _refuse("k and v must be of one type")
         qo = ko = vo = None
+        qp = qop = kop = vop = qt = qh = heads = pos = cosp = sinp = rows = rotary = 0
         if q is not None:
-            _need(self._heads(q, "q") == dt and q.shape[0] == T, "q must have k's tokens and type")
-            qo = torch.empty(q.shape, dtype=q.dtype, device=self.device)
-            a.q, a.q_out, a.q_token, a.q_head, a.q_heads = q.data_ptr(), qo.data_ptr(), q.stride(0), q.stride(1), q.shape[1]
+            if q.dim() != 3 or self._heads(q, "q", (T, q.shape[1], D)) != dt:
+                _refuse("q must be (tokens, heads, head_dim) of k's type")
+            heads = q.shape[1]
+            qo = torch.empty((T, heads, D), dtype=q.dtype, device=dev)
+            qp, qop, (qt, qh, _) = q.data_ptr(), qo.data_ptr(), q.stride()
         if rope is not None:
             cos, sin = rope
-            _need(positions is not None and cos.dim() == 2, "rope is (cos, sin), each (positions, rotary / 2), and needs positions")
-            shape = tuple(cos.shape)
-            a.rope_cos = _index(cos, "cos", torch.float32, shape, self.device)
-            a.rope_sin = _index(sin, "sin", torch.float32, shape, self.device)
-            a.positions = _index(positions, "positions", torch.int32, (T,), self.device)
-            a.rope_rows, a.rotary, a.interleaved = shape[0], 2 * shape[1], int(interleaved)
+            if positions is None or cos.dim() != 2:
+                _refuse("rope is (cos, sin), each (positions, rotary / 2), and needs positions")
+            rows, rotary = cos.shape
+            cosp = _index(cos, "cos", torch.float32, cos.shape, dev)
+            sinp = _index(sin, "sin", torch.float32, cos.shape, dev)
+            pos = _index(positions, "positions", torch.int32, (T,), dev)
         if values:
-            ko = torch.empty(T, self.kv_heads, self.head_dim, dtype=k.dtype, device=self.device)
-            vo = torch.empty_like(ko)
-            a.k_out, a.v_out = ko.data_ptr(), vo.data_ptr()
-        _call(_lib.cora_kv4_append, self.device, self._ref, C.byref(a))
+            ko, vo = torch.empty(shape, dtype=k.dtype, device=dev), torch.empty(shape, dtype=k.dtype, device=dev)
+            kop, vop = ko.data_ptr(), vo.data_ptr()
+        kt, kh, _ = k.stride()
+        vt, vh, _ = v.stride()
+        _call(self._lib.cora_kv4_append, self._dev, self._ref, _APPEND(
+            k.data_ptr(), v.data_ptr(), qp, kop, vop, qop, kt, kh, vt, vh, qt, qh,
+            _index(slots, "slots", torch.int64, (T,), dev), pos, cosp, sinp, T, rows, heads, 2 * rotary, bool(interleaved), dt))
         return Appended(qo, ko, vo)
 
     def attend(self, q, page_table, lens, q_start=None, max_queries: int = 1, causal=True, window: int = 0,
@@ -200,43 +217,44 @@ class Cache4:
         last `window` of them. scale: of the scores, default head_dim ** -0.5. A token that sees
         nothing gets zeros (and lse -inf). Returns out, or (out, lse): lse is fp32 (rows, heads).
         """
-        dt = self._heads(q, "q")
-        T, Hq, D = q.shape
-        _need(page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.device == self.device
-              and page_table.stride(1) == 1, f"page_table must be int32 (sequences, width) on {self.device}")
-        B = page_table.shape[0]
-        a = _AttendArg(q=q.data_ptr(), q_token=q.stride(0), q_head=q.stride(1), page_table=page_table.data_ptr(),
-                       table_stride=page_table.stride(0), table_width=page_table.shape[1],
-                       lens=_index(lens, "lens", torch.int32, (B,), self.device), q_tokens=T, q_heads=Hq, seqs=B,
-                       scale=D ** -0.5 if scale is None else scale, window=window, causal=int(causal),
-                       max_queries=max_queries, dtype=dt)
-        _need(window >= 0 and max_queries >= 1, "window and max_queries must not be negative")
+        dev = self.device
+        if q.dim() != 3 or page_table.dim() != 2:
+            _refuse("q must be (rows, heads, head_dim), page_table (sequences, width)")
+        T, Hq, D = shape = q.shape
+        dt = self._heads(q, "q", (T, Hq, self.head_dim))
+        B, width = page_table.shape
+        stride, last = page_table.stride()
+        if page_table.dtype is not torch.int32 or page_table.device != dev or last != 1:
+            _refuse(f"page_table must be int32 (sequences, width) on {dev}")
+        if window < 0 or max_queries < 1:
+            _refuse("window must not be negative, max_queries must be positive")
+        qs = 0
         if q_start is not None:
-            a.q_start = _index(q_start, "q_start", torch.int32, (B + 1,), self.device)
-        else:
-            _need(T == B, "q has one row per sequence where q_start is not given")
+            qs = _index(q_start, "q_start", torch.int32, (B + 1,), dev)
+        elif T != B:
+            _refuse("q has one row per sequence where q_start is not given")
         if out is None:
-            out = torch.empty(T, Hq, D, dtype=q.dtype, device=self.device)
-        else:
-            _need(out.shape == q.shape and out.dtype == q.dtype and out.device == self.device and out.is_contiguous(),
-                  "out must be contiguous, of q's shape and type")
-        a.out = out.data_ptr()
-        lse = None
+            out = torch.empty(shape, dtype=q.dtype, device=dev)
+        elif out.shape != shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
+            _refuse("out must be contiguous, of q's shape and type")
+        lse, lp = None, 0
         if return_lse:
-            lse = torch.empty(T, Hq, dtype=torch.float32, device=self.device)
-            a.lse = lse.data_ptr()
-        stream = torch.cuda.current_stream(self.device).cuda_stream
-        key = (stream, Hq, max_queries)
-        work = self._work.get(key) or self._workspace(key)
-        a.workspace, a.workspace_bytes = work
-        _call(_lib.cora_kv4_attend, self.device, self._ref, C.byref(a))
+            lse = torch.empty((T, Hq), dtype=torch.float32, device=dev)
+            lp = lse.data_ptr()
+        key = (_stream(self._dev), Hq, max_queries)
+        work, size = self._work.get(key) or self._workspace(key)
+        qt, qh, _ = q.stride()
+        _call(self._lib.cora_kv4_attend, self._dev, self._ref, _ATTEND(
+            q.data_ptr(), out.data_ptr(), lp, qt, qh, page_table.data_ptr(),
+            _index(lens, "lens", torch.int32, (B,), dev), qs, stride, T, size, work,
+            D ** -0.5 if scale is None else scale, B, width, Hq, max_queries, window, bool(causal), dt))
         return (out, lse) if return_lse else out
 
     def _workspace(self, key):
         """The stream's workspace, made larger where this shape of call needs more."""
         stream, heads, queries = key
         with torch.cuda.device(self.device):
-            size = int(_lib.cora_kv4_attend_workspace(self._ref, heads, queries))
+            size = int(self._lib.cora_kv4_attend_workspace(self._ref, heads, queries))
         _need(size > 0, "q_heads must be a multiple of kv_heads")
         buf = self._work.get(stream)
         if buf is None or buf.numel() < size:
@@ -250,7 +268,7 @@ class Cache4:
         """Synchronise the current stream; raise if a call met a bad slot, page, position or row
         range, or if a wait ran out, since the last check."""
         try:
-            _call(_lib.cora_kv4_status, self.device, self._ref)
+            _call(self._lib.cora_kv4_status, self._dev, self._ref)
         except CoraRuntimeError:
             self._work.clear()  # a call that gave up may have left its workspace unready
             raise
@@ -262,7 +280,7 @@ class Weight4:
     128 columns is that of the matrix instruction's operands (include/cora_b200.h)."""
 
     def __init__(self, codes: torch.Tensor, meta: torch.Tensor, cols: int):
-        _bind(_lib)
+        self._lib = _library()
         padded = -(-cols // 128) * 128
         _need(codes.dtype == torch.uint8 and codes.dim() == 2 and codes.is_contiguous() and codes.is_cuda
               and codes.shape[1] * 2 == padded, f"codes must be contiguous CUDA uint8 (rows, {padded // 2})")
@@ -274,9 +292,9 @@ class Weight4:
         _need(groups * group == padded and group in (32, 64, 128) and meta.numel() == rows * groups * 2,
               "meta must hold a pair for each group of 32, 64 or 128 columns")
         self.codes, self.meta, self.rows, self.cols, self.group = codes, meta, rows, cols, group
-        self.device = codes.device
+        self.device, self._dev = codes.device, codes.device.index
         self._arg = _WeightArg(codes.data_ptr(), meta.data_ptr(), rows, cols, group)
-        self._ref = C.byref(self._arg)
+        self._ref = C.addressof(self._arg)
 
     @classmethod
     def quantize(cls, dense: torch.Tensor, group: int = 128) -> "Weight4":
@@ -289,7 +307,7 @@ class Weight4:
         for r in range(0, rows, step):
             x = torch.nn.functional.pad(dense[r:r + step].float(), (0, pad)).unflatten(1, (-1, group))
             low = x.amin(-1, keepdim=True)
-            scale = ((x.amax(-1, keepdim=True) - low) / 15.0).clamp(max=65504.0).half().float()
+            scale = ((x.amax(-1, keepdim=True) - low) * (1 / 15)).clamp(max=65504.0).half().float()
             low = low.clamp(-65504.0, 65504.0).half().float()
             inv = torch.where(scale > 0, 1.0 / scale, torch.zeros_like(scale))
             c = ((x - low) * inv).round().clamp(0, 15).to(torch.int32)
@@ -307,19 +325,19 @@ def matvec(x: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = None
            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x (..., cols) times the 4-bit weight, plus bias: (..., rows) in x's type. Meant for the few
     rows of decoding (1 to 64); more are correct, 32 rows at a time."""
-    _need(x.dim() >= 1 and x.shape[-1] == weight.cols and x.device == weight.device and x.stride(-1) == 1,
-          f"x must be (..., {weight.cols}) on {weight.device}, its last stride 1")
-    x2 = x if x.dim() == 2 else x.reshape(-1, weight.cols)
-    M, N = x2.shape[0], weight.rows
+    dev, N, dims = weight.device, weight.rows, x.dim()
+    if not dims or x.shape[-1] != weight.cols or x.device != dev or x.stride(-1) != 1:
+        _refuse(f"x must be (..., {weight.cols}) on {dev}, its last stride 1")
+    x2 = x if dims == 2 else x.reshape(-1, weight.cols)
+    M = x2.shape[0]
+    shape = (M, N) if dims == 2 else (*x.shape[:-1], N)
+    bp = 0
     if bias is not None:
-        _need(bias.dtype == x.dtype and tuple(bias.shape) == (N,) and bias.device == x.device and bias.is_contiguous(),
-              f"bias must be contiguous ({N},) of x's type")
+        bp = _index(bias, "bias", x.dtype, (N,), dev)
     if out is None:
-        out = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
-    else:
-        _need(tuple(out.shape) == (*x.shape[:-1], N) and out.dtype == x.dtype and out.device == x.device and out.is_contiguous(),
-              "out must be contiguous, of x's type, (..., rows)")
-    a = _MatvecArg(x2.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), x2.stride(0), N, M,
-                   _DTYPES.get(x.dtype, 99))
-    _call(_lib.cora_w4_matvec, x.device, weight._ref, C.byref(a))
+        out = torch.empty(shape, dtype=x.dtype, device=dev)
+    elif out.shape != shape or out.dtype != x.dtype or out.device != dev or not out.is_contiguous():
+        _refuse("out must be contiguous, of x's type, (..., rows)")
+    _call(weight._lib.cora_w4_matvec, weight._dev, weight._ref, _MATVEC(
+        x2.data_ptr(), bp, out.data_ptr(), x2.stride(0), N, M, _DTYPES.get(x.dtype, 99)))
     return out

@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(kAtThreads, kNT * D <= 128 ? 2 : 1) kv4_attend
     const int64_t u0 = cut(blockIdx.x), u1 = cut(blockIdx.x + 1);
     if (u0 >= u1) return;
 
-    // The sequence that holds unit u (base is ascending).
+    // The sequence that holds unit u (base is ascending; units of one sequence fit 32 bits).
     auto find = [&](int64_t u) {
         int lo = 0, hi = (int)p.seqs - 1;
         while (lo < hi) {
@@ -188,44 +188,59 @@ __global__ void __launch_bounds__(kAtThreads, kNT * D <= 128 ? 2 : 1) kv4_attend
     };
 
     // ---- the warp's stream of tiles: units u0 + warp, + kAtWarps, ... ----
-    int fb = -1;
+    // Copies of one tile: lane 4 i + k copies section k of the tile's i-th page piece.
+    const int per = min(P, kAtTile), shift = 31 - __clz(P);  // tokens of a piece
+    const int piece = lane >> 2, kind = lane & 3;
+    const uint32_t rowb = kind < 2 ? D / 2 : kNG * 4;
+    const uint32_t src_at = (kind & 1 ? (kind < 2 ? blk.codes : blk.metas) : 0) + (kind < 2 ? 0 : 2 * blk.codes);
+    const uint32_t dst_at = (kind & 1 ? (kind < 2 ? S::kCodes : S::kMeta) : 0) + (kind < 2 ? 0 : 2 * S::kCodes) +
+                            piece * per * rowb;
+    int fb = -1, ftile = 0, frt = 0, fhead = 0, fpage = 0;  // the next tile to fetch
     SeqWork fs{};
-    auto fetch = [&](int64_t u, int stage) {  // warp-uniform
-        if (fb < 0 || u >= base[fb + 1]) {
-            fb = find(u);
-            fs = seq_work(p, fb, kRows);
-        }
-        const int64_t r = u - base[fb];
-        const int tile = (int)(r % fs.tiles);
-        const int head = (int)(r / fs.tiles / fs.row_tiles);
-        const int tok0 = fs.first + tile * kAtTile;
-        const int per = min(P, kAtTile);                       // tokens of one piece
-        const int pieces = max(0, min(kAtTile / per, (fs.len - tok0 + per - 1) / per));
-        const int piece = lane >> 2, kind = lane & 3;
-        bool ok = false;
-        const unsigned char *src = nullptr;
-        unsigned char *dst = nullptr;
-        uint32_t bytes = 0;
-        if (piece < pieces) {
-            const int tok = tok0 + piece * per;
-            const int page = __ldg(p.a.page_table + (int64_t)(p.seq0 + fb) * p.a.table_stride + tok / P);
-            ok = page >= 0 && (uint64_t)page < p.c.num_pages;
-            if (!ok) atomicOr(p.c.status, kDevBadInput);
-            const uint32_t row = kind < 2 ? blk.code_row : blk.meta_row;
-            const uint32_t at = (kind & 1 ? (kind < 2 ? blk.codes : blk.metas) : 0) + (kind < 2 ? 0 : 2 * blk.codes);
-            src = p.c.pool + ((uint64_t)(ok ? page : 0) * H + head) * blk.bytes + at + (uint32_t)(tok % P) * row;
-            dst = ring + stage * S::kStage + (kind & 1 ? (kind < 2 ? S::kCodes : S::kMeta) : 0) +
-                  (kind < 2 ? 0 : 2 * S::kCodes) + piece * per * row;
-            bytes = ok ? per * row : 0;
-        }
-        const uint32_t total = __reduce_add_sync(0xffffffffu, bytes);
-        if (lane == 0) mbar_arrive_expect_tx(bars + stage, total);
+    const int *ftable = nullptr;
+    auto fetch_page = [&]() {  // its page's number, early: the copy needs it one tile later
+        const int tok = fs.first + ftile * kAtTile + piece * per;
+        fpage = piece * per < kAtTile && tok < fs.len ? __ldg(ftable + (tok >> shift)) : -2;
+    };
+    auto fetch_seek = [&](int64_t u) {  // warp-uniform
+        fb = find(u);
+        fs = seq_work(p, fb, kRows);
+        ftable = p.a.page_table + (int64_t)(p.seq0 + fb) * p.a.table_stride;
+        const uint32_t r = (uint32_t)(u - base[fb]), job = r / (uint32_t)fs.tiles;
+        ftile = (int)(r - job * fs.tiles);
+        fhead = (int)(job / fs.row_tiles);
+        frt = (int)(job - fhead * fs.row_tiles);
+        fetch_page();
+    };
+    auto fetch = [&](int64_t u, int stage) {
+        const bool got = fpage != -2, ok = got && fpage >= 0 && (uint32_t)fpage < p.c.num_pages;
+        const uint32_t lanes = __ballot_sync(0xffffffffu, ok);
+        if (got && !ok) atomicOr(p.c.status, kDevBadInput);
+        const uint32_t bytes = per * rowb;
+        // sections of a piece are copied by four neighbouring lanes, all or none
+        if (lane == 0) mbar_arrive_expect_tx(bars + stage, __popc(lanes) / 4 * per * (D + 8 * kNG));
         __syncwarp();
-        if (bytes) bulk_g2s(dst, src, bytes, bars + stage);
+        if (ok) {
+            const int tok = fs.first + ftile * kAtTile + piece * per;
+            bulk_g2s(ring + stage * S::kStage + dst_at,
+                     p.c.pool + ((uint64_t)fpage * H + fhead) * blk.bytes + src_at + (uint32_t)(tok & (P - 1)) * rowb, bytes,
+                     bars + stage);
+        }
+        // on to the tile after next of this block
+        u += kAtWarps;
+        if (u >= u1) return;
+        if (u >= base[fb + 1]) return fetch_seek(u);
+        ftile += kAtWarps;
+        while (ftile >= fs.tiles) {
+            ftile -= fs.tiles;
+            if (++frt == fs.row_tiles) frt = 0, ++fhead;
+        }
+        fetch_page();
     };
 
     int64_t ahead = u0 + warp;   // next unit to fetch
     int fstage = 0, pending = 0;  // tiles in flight
+    if (ahead < u1) fetch_seek(ahead);
     for (; pending < kAtStages && ahead < u1; ++pending, ahead += kAtWarps) fetch(ahead, pending);
     int stage = 0;
     uint32_t phase = 0;

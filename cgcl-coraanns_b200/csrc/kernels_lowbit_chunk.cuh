@@ -224,10 +224,13 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
             const T *src = static_cast<const T *>(p.a.q) + (int64_t)(g.s.q0 + i) * p.a.q_token + (int64_t)hh * p.a.q_head;
             // the row under its own power of two, largest |q| in [2^13, 2^14)
             float big = 0.0f;
+#pragma unroll 8
             for (int d = 0; d < D; d += 8) {
-                float x[8];
-                if (vec) load8<T, true>(src + d, x);
-                else load8<T, false>(src + d, x);
+                float x[8] = {};
+                if (in) {
+                    if (vec) load8<T, true>(src + d, x);
+                    else load8<T, false>(src + d, x);
+                }
 #pragma unroll
                 for (int e = 0; e < 8; ++e) big = fabsf(x[e]) < 3.4e38f ? fmaxf(big, fabsf(x[e])) : big;
             }
@@ -237,10 +240,13 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
 #pragma unroll
             for (int gr = 0; gr < kNG; ++gr) {
                 float sum = 0.0f;
+#pragma unroll 8
                 for (int d = gr * kG; d < (gr + 1) * kG; d += 8) {
-                    float x[8];
-                    if (vec) load8<T, true>(src + d, x);
-                    else load8<T, false>(src + d, x);
+                    float x[8] = {};
+                    if (in) {
+                        if (vec) load8<T, true>(src + d, x);
+                        else load8<T, false>(src + d, x);
+                    }
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         x[e] *= qpow;
@@ -250,11 +256,10 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
                     uint4 w;
                     w.x = pack_half2(x[0], x[4]), w.y = pack_half2(x[1] * odd, x[5] * odd);
                     w.z = pack_half2(x[2], x[6]), w.w = pack_half2(x[3] * odd, x[7] * odd);
-                    if (!in) w = make_uint4(0, 0, 0, 0);
                     const int c = (d / 8) & 7;
                     *reinterpret_cast<uint4 *>(sq + (d / 64) * kQBlock + row * 128 + ((c ^ (row & 7)) << 4)) = w;
                 }
-                qs[gr] = in ? sum * 5.9604644775390625e-8f : 0.0f;  // 2^-24
+                qs[gr] = sum * 5.9604644775390625e-8f;  // 2^-24
             }
             fence_proxy_async_smem();
             mbar_arrive(q_full + q);

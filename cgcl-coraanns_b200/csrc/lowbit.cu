@@ -64,9 +64,9 @@ void allow_smem(K kernel, size_t bytes, int (&seen)[64]) {
 
 // ---- append ------------------------------------------------------------------------------
 
-template <typename T, int D, bool kVec>
+template <typename T, int D, bool kOne, bool kVec>
 void launch_append(const cora_kv4_cache &c, const cora_kv4_append_args &a, cudaStream_t st) {
-    const uint64_t per = kAppendThreads / (D / 8), bx = (a.tokens + per - 1) / per;
+    const uint64_t per = kAppendThreads / (D / 16), bx = (a.tokens + per - 1) / per;
     const uint64_t heads = 2ull * c.kv_heads + (a.q ? a.q_heads : 0);
     // Few tokens: one head per thread, for latency. Many: runs of heads share one read of the
     // rotation's factors, as long as 16 blocks per SM remain to hide the loads.
@@ -74,7 +74,9 @@ void launch_append(const cora_kv4_cache &c, const cora_kv4_append_args &a, cudaS
     uint64_t run = bx * heads <= want ? 1 : std::min(heads, bx * heads / want);
     while ((heads + run - 1) / run > kMaxGrid) ++run;
     need(bx <= INT_MAX, "too many tokens");
-    kv4_append_kernel<T, D, kVec><<<dim3((unsigned)bx, (unsigned)((heads + run - 1) / run)), kAppendThreads, 0, st>>>(c, a, (int)run);
+    const int turn = !a.rotary ? kTurnNone : a.interleaved ? kTurnInterleaved : a.rotary == D ? kTurnFull : kTurnPart;
+    kv4_append_kernel<T, D, kOne, kVec><<<dim3((unsigned)bx, (unsigned)((heads + run - 1) / run)), kAppendThreads, 0, st>>>(
+        c, a, (int)run, turn);
     CUDA_TRY(cudaGetLastError());
 }
 
@@ -93,8 +95,10 @@ void append(const cora_kv4_cache *c, const cora_kv4_append_args *a, cudaStream_t
     by_dtype(a->dtype, [&](auto z) {
         using T = decltype(z);
         auto go = [&](auto d) {
-            if (vec) launch_append<T, decltype(d)::value, true>(*c, *a, st);
-            else launch_append<T, decltype(d)::value, false>(*c, *a, st);
+            constexpr int D = decltype(d)::value;
+            const bool one = c->group == c->head_dim;
+            if (vec) one ? launch_append<T, D, true, true>(*c, *a, st) : launch_append<T, D, false, true>(*c, *a, st);
+            else one ? launch_append<T, D, true, false>(*c, *a, st) : launch_append<T, D, false, false>(*c, *a, st);
         };
         if (c->head_dim == 64) go(Int<64>{});
         else if (c->head_dim == 128) go(Int<128>{});

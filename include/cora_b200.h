@@ -311,7 +311,7 @@ int cora_probe_noalloc_status(cora_engine *engine, void *stream);
  *
  * Format. A group of G consecutive values is 4-bit codes c and two fp16 factors (scale, low),
  * and stands for scale * c + low. Quantising a group x: low = fp16(min x),
- * scale = fp16((max x - min x) / 15), c = clamp(rne((x - low) * (1 / scale)), 0, 15), c = 0 where
+ * scale = fp16((max x - min x) * (1 / 15)), c = clamp(rne((x - low) * (1 / scale)), 0, 15), c = 0 where
  * scale is 0, each operation in fp32; factors saturate at the largest fp16, NaN is kept.
  *
  * Errors on the device (a slot, position, page or row range outside its tensor, a wait that ran

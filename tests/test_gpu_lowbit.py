@@ -39,7 +39,7 @@ def quantize32(x, G):
     g = x.astype(np.float32).reshape(*x.shape[:-1], -1, G)
     lo, hi = g.min(-1, keepdims=True), g.max(-1, keepdims=True)
     with np.errstate(all="ignore"):
-        s = ((hi - lo) / np.float32(15)).astype(np.float32)
+        s = ((hi - lo) * np.float32(1 / 15)).astype(np.float32)
         s = np.minimum(s, np.float32(65504)).astype(np.float16)
         b = np.clip(lo, -65504, 65504).astype(np.float16)
         sf, bf = s.astype(np.float32), b.astype(np.float32)
