@@ -79,6 +79,12 @@ __device__ __forceinline__ void store8(T *p, const float (&x)[8]) {
     *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(t);
 }
 
+template <typename T>
+__device__ __forceinline__ void store4(T *p, float a, float b, float c, float d) {
+    alignas(8) T t[4] = {from_f32<T>(a), from_f32<T>(b), from_f32<T>(c), from_f32<T>(d)};
+    *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(t);
+}
+
 constexpr int kAppendThreads = 256;
 enum AppendTurn { kTurnNone, kTurnFull, kTurnInterleaved, kTurnPart };
 

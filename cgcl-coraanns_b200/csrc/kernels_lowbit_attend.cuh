@@ -18,10 +18,13 @@
 //    their group's range; so the sum is taken as sum w (c' - 7.5) + sum p (low' + 7.5 scale'),
 //    sum w by one more product with ones: the loss is then 2^-12 of |value - middle|.
 //    Statistics, sums and accumulators are fp32;
-//  - each warp streams its own tiles of kTile tokens through a private ring of bulk copies, and
-//    keeps its own running maximum and sum; a block's warps join in shared memory;
-//  - (sequence, key head, row tile, token tile) units are cut into equal runs, one per block,
-//    so ragged batches balance; a job cut over several blocks is joined by the last to arrive.
+//  - each warp streams tiles of kAtTile tokens through a private ring of bulk copies and keeps its
+//    own running maximum and sum: warps wait for one another only where they share a job;
+//  - the work, (sequence, key head, row tile) jobs of token tiles plus one unit for a job's own
+//    cost, is cut into equal runs, one per warp, so that long, short and ragged batches balance.
+//    A job inside one run is written by its warp; one cut over the warps of a block is joined in
+//    shared memory; one cut over blocks by the last block to arrive, from partial results in
+//    the workspace. Where all jobs are short, each block takes one instead (no join over blocks).
 #pragma once
 #include <cuda_fp16.h>
 
@@ -33,8 +36,10 @@
 namespace cora {
 
 constexpr int kAtWarps = 8, kAtThreads = kAtWarps * 32, kAtTile = 32, kAtStages = 2;
-constexpr int kAtMinRun = 4;       // units of a block, at least
-constexpr int kAtMaxSeqs = 1024;   // sequences of one launch (their unit offsets are in smem)
+constexpr int kAtRows = 8;         // query rows of a job
+constexpr int kAtMinRun = 2;       // units of a warp, at least
+constexpr int kAtShort = 40;       // tiles of a job that one block takes whole
+constexpr int kAtMaxSeqs = 512;    // sequences of one launch (their work is kept in smem)
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttendParams {
@@ -42,28 +47,28 @@ struct AttendParams {
     cora_kv4_attend_args a;
     uint32_t seq0, seqs;      // this launch's sequences
     int64_t q_tokens;         // rows of q
-    float *part;              // partial results: [2 * blocks][rows][D] then [2 * blocks][rows][2]
+    float *part;              // partial results
     uint32_t *arrived;        // per block, zero between launches
 };
 
+// A partial result of 8 rows: unnormalised outputs, then (maximum, sum) per row.
+template <int D>
+constexpr int kAtPart = kAtRows * (D + 2);
+
 // The shared memory of a block, in order (each part a multiple of 16 bytes).
-template <int D, int kNG, int kNT>
+template <int D, int kNG>
 struct AttendSmem {
-    static constexpr int kRows = 8 * kNT;
     static constexpr uint32_t kCodes = kAtTile * D / 2, kMeta = kAtTile * kNG * 4;
     static constexpr uint32_t kStage = 2 * kCodes + 2 * kMeta;
+    static constexpr uint32_t kRing = kAtStages * kStage;   // of a warp; at the end its partial result
+    static_assert(kRing >= kAtPart<D> * 4, "");
     static constexpr uint32_t ring = 0;
-    static constexpr uint32_t qfrag = ring + kAtWarps * kAtStages * kStage;  // D / 32 * kNT * 512
-    static constexpr uint32_t red = qfrag + (D / 32) * kNT * 512;            // [warp][row][64]
-    static constexpr uint32_t qsum = red + kAtWarps * kRows * 64 * 4;        // [row][kNG]
-    static constexpr uint32_t lim = qsum + kRows * kNG * 4;                  // [row] {lo, hi}
-    static constexpr uint32_t stat = lim + kRows * 8;                        // [warp][row] {m, l}
-    static constexpr uint32_t om = stat + kAtWarps * kRows * 8;              // [warp][row][kNG]
-    static constexpr uint32_t fin = om + kAtWarps * kRows * kNG * 4;         // [row] {m, l}
-    static constexpr uint32_t misc = fin + kRows * 8;                        // max |q|, last to arrive
+    static constexpr uint32_t qfrag = ring + kAtWarps * kRing;       // [warp][D / 32][32] x 16 bytes
+    static constexpr uint32_t keys = qfrag + kAtWarps * (D / 32) * 512;  // [2 warps] job of each partial result
+    static constexpr uint32_t misc = keys + kAtWarps * 2 * 8;
     static constexpr uint32_t bars = misc + 32;
-    static constexpr uint32_t base = bars + kAtWarps * kAtStages * 8;        // int64[seqs + 1]
-    static constexpr size_t bytes(uint32_t seqs) { return base + 8 * (size_t)(seqs + 1); }
+    static constexpr uint32_t work = bars + kAtWarps * kAtStages * 8;    // int4[seqs], int64[seqs + 1]
+    static constexpr size_t bytes(uint32_t seqs) { return work + 24 * (size_t)seqs + 8; }
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -122,60 +127,70 @@ __device__ __forceinline__ SeqWork seq_work(const AttendParams &p, int b, int ro
     return s;
 }
 
-template <typename T, int D, int kNG, int kNT>
-__global__ void __launch_bounds__(kAtThreads, kNT * D <= 128 ? 2 : 1) kv4_attend_kernel(const AttendParams p) {
-    using S = AttendSmem<D, kNG, kNT>;
-    constexpr int kRows = 8 * kNT, kG = D / kNG;
-    constexpr int kWords = kG / 32;         // words of one lane and group
-    constexpr int kVB = D / 64;             // 64-dimension blocks of the values
+template <typename T, int D, int kNG>
+__global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kernel(const AttendParams p) {
+    using S = AttendSmem<D, kNG>;
+    constexpr int kG = D / kNG, kWords = kG / 32;  // words of one lane and group
+    constexpr int kVB = D / 64;                    // 64-dimension blocks of the values
     extern __shared__ __align__(128) unsigned char at_smem[];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
-    unsigned char *ring = at_smem + S::ring + warp * kAtStages * S::kStage;
-    uint4 *qfrag = reinterpret_cast<uint4 *>(at_smem + S::qfrag);
-    float *red = reinterpret_cast<float *>(at_smem + S::red);
-    float *qsum = reinterpret_cast<float *>(at_smem + S::qsum);
-    int2 *lim = reinterpret_cast<int2 *>(at_smem + S::lim);
-    float2 *stat = reinterpret_cast<float2 *>(at_smem + S::stat);
-    float *omw = reinterpret_cast<float *>(at_smem + S::om);
-    float2 *fin = reinterpret_cast<float2 *>(at_smem + S::fin);
+    unsigned char *ring = at_smem + S::ring + warp * S::kRing;
+    uint4 *qfrag = reinterpret_cast<uint4 *>(at_smem + S::qfrag) + warp * (D / 32) * 32;
+    int64_t *keys = reinterpret_cast<int64_t *>(at_smem + S::keys);
     volatile int *misc = reinterpret_cast<volatile int *>(at_smem + S::misc);
     uint64_t *bars = reinterpret_cast<uint64_t *>(at_smem + S::bars) + warp * kAtStages;
-    int64_t *base = reinterpret_cast<int64_t *>(at_smem + S::base);
+    int4 *work = reinterpret_cast<int4 *>(at_smem + S::work);
+    int64_t *base = reinterpret_cast<int64_t *>(work + p.seqs);
 
     const int H = p.c.kv_heads, heads = p.a.q_heads / H, P = p.c.page_size;
     const Kv4Block blk(P, D, kG);
 
     if (lane == 0) {
         for (int s = 0; s < kAtStages; ++s) mbar_init(bars + s, 1);
+        keys[2 * warp] = keys[2 * warp + 1] = -1;
         fence_barrier_init();
     }
-    // unit offsets of the sequences: inclusive sums by warp 0, 32 sequences at a time
-    if (warp == 0) {
-        int64_t run = 0;
-        if (lane == 0) base[0] = 0;
-        for (int b0 = 0; b0 < (int)p.seqs; b0 += 32) {
-            int64_t v = 0;
-            if (b0 + lane < (int)p.seqs) {
-                const SeqWork s = seq_work(p, b0 + lane, kRows);
-                v = (int64_t)s.tiles * s.row_tiles * H;
-            }
-#pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-                const int64_t o = __shfl_up_sync(0xffffffffu, v, off);
-                if (lane >= off) v += o;
-            }
-            if (b0 + lane < (int)p.seqs) base[b0 + lane + 1] = run + v;
-            run += __shfl_sync(0xffffffffu, v, 31);
-        }
+    for (int b = threadIdx.x; b < (int)p.seqs; b += kAtThreads) {
+        const SeqWork s = seq_work(p, b, kAtRows);
+        work[b] = make_int4(s.q0, s.n, s.len, s.first);
     }
     __syncthreads();
-    // Equal runs of at least kAtMinRun units: block i holds units [i U / B, (i + 1) U / B).
-    const int64_t units = base[p.seqs], blocks = max((int64_t)1, min((int64_t)gridDim.x, units / kAtMinRun));
-    if (blockIdx.x >= blocks) return;
-    auto cut = [&](int64_t i) { return i * units / blocks; };
-    const int64_t u0 = cut(blockIdx.x), u1 = cut(blockIdx.x + 1);
-    if (u0 >= u1) return;
-
+    auto seq = [&](int b) {
+        const int4 w = work[b];
+        SeqWork s;
+        s.q0 = w.x, s.n = w.y, s.len = w.z, s.first = w.w;
+        s.tiles = max(1, (s.len - s.first + kAtTile - 1) / kAtTile);
+        s.row_tiles = (s.n * heads + kAtRows - 1) / kAtRows;
+        return s;
+    };
+    if (warp == 0) {  // first units of the sequences, 32 at a time; jobs and the longest
+        int64_t run = 0, jobs = 0;
+        int longest = 0;
+        if (lane == 0) base[0] = 0;
+        for (int b0 = 0; b0 < (int)p.seqs; b0 += 32) {
+            int64_t v = 0, j = 0;
+            if (b0 + lane < (int)p.seqs) {
+                const SeqWork s = seq(b0 + lane);
+                j = (int64_t)s.row_tiles * H;
+                v = (s.tiles + 1) * j;
+                if (j) longest = max(longest, s.tiles);
+            }
+            int64_t all = v;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const int64_t o = __shfl_up_sync(0xffffffffu, all, off);
+                if (lane >= off) all += o;
+                j += __shfl_xor_sync(0xffffffffu, j, off);
+            }
+            if (b0 + lane < (int)p.seqs) base[b0 + lane + 1] = run + all;
+            run += __shfl_sync(0xffffffffu, all, 31);
+            jobs += j;
+        }
+        longest = __reduce_max_sync(0xffffffffu, longest);
+        if (lane == 0) misc[2] = longest <= kAtShort && jobs <= gridDim.x ? (int)jobs : 0;
+    }
+    __syncthreads();
+    const int64_t units = base[p.seqs];
     // The sequence that holds unit u (base is ascending; units of one sequence fit 32 bits).
     auto find = [&](int64_t u) {
         int lo = 0, hi = (int)p.seqs - 1;
@@ -186,8 +201,31 @@ __global__ void __launch_bounds__(kAtThreads, kNT * D <= 128 ? 2 : 1) kv4_attend
         }
         return lo;
     };
+    // Equal runs: warp i of B blocks holds units [i U / 8 B, (i + 1) U / 8 B).
+    const bool aligned = misc[2] != 0;
+    const int64_t blocks = aligned ? misc[2] : max((int64_t)1, min((int64_t)gridDim.x, units / (kAtMinRun * kAtWarps)));
+    if (blockIdx.x >= blocks || !units) return;
+    int64_t b0 = 0, b1 = 0;  // this block's units
+    if (aligned) {  // one job per block: the block's number counts jobs
+        int64_t job = blockIdx.x;
+        for (int b = 0;; ++b) {
+            const SeqWork s = seq(b);
+            const int64_t n = (int64_t)s.row_tiles * H;
+            if (job < n) {
+                b0 = base[b] + job * (s.tiles + 1), b1 = b0 + s.tiles + 1;
+                break;
+            }
+            job -= n;
+        }
+    } else {
+        b0 = blockIdx.x * units / blocks, b1 = (blockIdx.x + 1) * units / blocks;
+    }
+    auto cut = [&](int64_t w) {
+        return aligned ? w * (b1 - b0) / kAtWarps + b0 : (blockIdx.x * kAtWarps + w) * units / (blocks * kAtWarps);
+    };
+    const int64_t u0 = cut(warp), u1 = cut(warp + 1);
 
-    // ---- the warp's stream of tiles: units u0 + warp, + kAtWarps, ... ----
+    // ---- the warp's stream of tiles ----
     // Copies of one tile: lane 4 i + k copies section k of the tile's i-th page piece.
     const int per = min(P, kAtTile), shift = 31 - __clz(P);  // tokens of a piece
     const int piece = lane >> 2, kind = lane & 3;
@@ -195,183 +233,168 @@ __global__ void __launch_bounds__(kAtThreads, kNT * D <= 128 ? 2 : 1) kv4_attend
     const uint32_t src_at = (kind & 1 ? (kind < 2 ? blk.codes : blk.metas) : 0) + (kind < 2 ? 0 : 2 * blk.codes);
     const uint32_t dst_at = (kind & 1 ? (kind < 2 ? S::kCodes : S::kMeta) : 0) + (kind < 2 ? 0 : 2 * S::kCodes) +
                             piece * per * rowb;
-    int fb = -1, ftile = 0, frt = 0, fhead = 0, fpage = 0;  // the next tile to fetch
+    int64_t ahead = u0;                                // the unit that the next tile to fetch is
+    int fb = -1, ftile = 0, frt = 0, fhead = 0, fpage = 0;
     SeqWork fs{};
     const int *ftable = nullptr;
     auto fetch_page = [&]() {  // its page's number, early: the copy needs it one tile later
         const int tok = fs.first + ftile * kAtTile + piece * per;
         fpage = piece * per < kAtTile && tok < fs.len ? __ldg(ftable + (tok >> shift)) : -2;
     };
-    auto fetch_seek = [&](int64_t u) {  // warp-uniform
-        fb = find(u);
-        fs = seq_work(p, fb, kRows);
+    auto fetch_seek = [&]() {  // to unit `ahead`, or past it where that is a job's first (no tile)
+        if (ahead >= u1) return;
+        fb = find(ahead);
+        fs = seq(fb);
         ftable = p.a.page_table + (int64_t)(p.seq0 + fb) * p.a.table_stride;
-        const uint32_t r = (uint32_t)(u - base[fb]), job = r / (uint32_t)fs.tiles;
-        ftile = (int)(r - job * fs.tiles);
+        const uint32_t r = (uint32_t)(ahead - base[fb]), n = fs.tiles + 1, job = r / n;
+        ftile = (int)(r - job * n) - 1;
         fhead = (int)(job / fs.row_tiles);
         frt = (int)(job - fhead * fs.row_tiles);
-        fetch_page();
+        if (ftile < 0) ++ahead, ftile = 0;
+        if (ahead < u1) fetch_page();
     };
-    auto fetch = [&](int64_t u, int stage) {
+    auto fetch = [&](int stage) {
         const bool got = fpage != -2, ok = got && fpage >= 0 && (uint32_t)fpage < p.c.num_pages;
         const uint32_t lanes = __ballot_sync(0xffffffffu, ok);
         if (got && !ok) atomicOr(p.c.status, kDevBadInput);
-        const uint32_t bytes = per * rowb;
         // sections of a piece are copied by four neighbouring lanes, all or none
         if (lane == 0) mbar_arrive_expect_tx(bars + stage, __popc(lanes) / 4 * per * (D + 8 * kNG));
         __syncwarp();
         if (ok) {
             const int tok = fs.first + ftile * kAtTile + piece * per;
             bulk_g2s(ring + stage * S::kStage + dst_at,
-                     p.c.pool + ((uint64_t)fpage * H + fhead) * blk.bytes + src_at + (uint32_t)(tok & (P - 1)) * rowb, bytes,
-                     bars + stage);
+                     p.c.pool + ((uint64_t)fpage * H + fhead) * blk.bytes + src_at + (uint32_t)(tok & (P - 1)) * rowb,
+                     per * rowb, bars + stage);
         }
-        // on to the tile after next of this block
-        u += kAtWarps;
-        if (u >= u1) return;
-        if (u >= base[fb + 1]) return fetch_seek(u);
-        ftile += kAtWarps;
-        while (ftile >= fs.tiles) {
-            ftile -= fs.tiles;
-            if (++frt == fs.row_tiles) frt = 0, ++fhead;
-        }
-        fetch_page();
+        if (++ahead >= u1) return;
+        if (++ftile < fs.tiles) return fetch_page();
+        if (ahead >= base[fb + 1]) return fetch_seek();
+        ++ahead, ftile = 0;  // the next job's own unit
+        if (++frt == fs.row_tiles) frt = 0, ++fhead;
+        if (ahead < u1) fetch_page();
     };
-
-    int64_t ahead = u0 + warp;   // next unit to fetch
     int fstage = 0, pending = 0;  // tiles in flight
-    if (ahead < u1) fetch_seek(ahead);
-    for (; pending < kAtStages && ahead < u1; ++pending, ahead += kAtWarps) fetch(ahead, pending);
+    fetch_seek();
+    for (; pending < kAtStages && ahead < u1; ++pending) fetch(pending);
     int stage = 0;
     uint32_t phase = 0;
-    int64_t u = u0 + warp;       // next unit to consume
+    bool alive = true;
 
+    // partial results: two per block, then one per warp (a first job that goes on before it ends)
+    float *const part_warp = p.part + (size_t)2 * gridDim.x * kAtPart<D> + (size_t)(blockIdx.x * kAtWarps + warp) * kAtPart<D>;
+
+    T *const out = static_cast<T *>(p.a.out);
+    float acc[kVB][4][4], mx[2], ls[2];
     int b = -1;
     SeqWork sw{};
-    bool alive = true;
-    for (int64_t seg = u0; seg < u1;) {
-        // ---- one job (sequence, key head, row tile), units [seg, seg_end) of it are ours ----
-        if (b < 0 || seg >= base[b + 1]) {
-            b = find(seg);
-            sw = seq_work(p, b, kRows);
+    for (int64_t u = u0; u < u1;) {
+        // ---- one job: tiles [tile0, tile1) of it are this warp's ----
+        if (b < 0 || u >= base[b + 1]) {
+            b = find(u);
+            sw = seq(b);
         }
-        const int64_t job = (seg - base[b]) / sw.tiles;
-        const int64_t job_u0 = base[b] + job * sw.tiles, job_u1 = job_u0 + sw.tiles;
+        const uint32_t jr = (uint32_t)(u - base[b]), jn = sw.tiles + 1, job = jr / jn;
+        const int64_t job_u0 = base[b] + (int64_t)job * jn, job_u1 = job_u0 + jn;
         const int64_t seg_end = min(u1, job_u1);
-        const int rt = (int)(job % sw.row_tiles), head = (int)(job / sw.row_tiles);
-        const int row0 = rt * kRows, nrows = min(kRows, sw.n * heads - row0);
-
+        const int head = (int)(job / sw.row_tiles), rt = (int)(job - head * sw.row_tiles);
+        const int row0 = rt * kAtRows, nrows = min(kAtRows, sw.n * heads - row0);
+        int tile = max(0, (int)(u - job_u0) - 1);
+        const int tile_end = (int)(seg_end - job_u0) - 1;
+        if (tile_end <= tile) {  // only the job's own unit
+            u = seg_end;
+            continue;
+        }
         // queries: rows are (token, head of the group); fp16 under a common power of two
-        if (threadIdx.x == 0) misc[0] = 0;
-        __syncthreads();
-        float qv[(kRows + kAtWarps - 1) / kAtWarps][D / 32];
+        constexpr int kPer = D / 32;  // dimensions of a lane
+        float qv[kAtRows][kPer];
         float big = 0.0f;
 #pragma unroll
-        for (int i = 0; i < (kRows + kAtWarps - 1) / kAtWarps; ++i) {
-            const int r = warp + i * kAtWarps;
-            const int row = row0 + r;
-            const bool in = r < nrows;
-            const T *src = static_cast<const T *>(p.a.q) + (int64_t)(sw.q0 + (in ? row / heads : 0)) * p.a.q_token +
-                           (int64_t)(head * heads + (in ? row % heads : 0)) * p.a.q_head;
+        for (int r = 0; r < kAtRows; ++r) {
+            const int row = row0 + min(r, nrows - 1), tk = row / heads;
+            const T *src = static_cast<const T *>(p.a.q) + (int64_t)(sw.q0 + tk) * p.a.q_token +
+                           (int64_t)(head * heads + row - tk * heads) * p.a.q_head;
 #pragma unroll
-            for (int d = 0; d < D / 32; ++d) {
-                qv[i][d] = in ? to_f32(src[d * 32 + lane]) : 0.0f;
-                const float m = fabsf(qv[i][d]);
-                if (m < 3.4e38f) big = fmaxf(big, m);  // infinities and NaN keep to their rows
-            }
-            if (lane == 0 && r < kRows) {
-                const int pos = sw.len - sw.n + row / heads;
-                const int hi = p.a.causal ? max(0, min(sw.len, pos + 1)) : sw.len;
-                const int lo = p.a.window ? max(0, pos - (int)p.a.window + 1) : 0;
-                lim[r] = in ? make_int2(lo, hi) : make_int2(0, 0);
-            }
+            for (int d = 0; d < kPer; ++d) qv[r][d] = to_f32(src[d * 32 + lane]);
         }
 #pragma unroll
-        for (int m = 16; m; m >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, m));
-        if (lane == 0) atomicMax(const_cast<int *>(&misc[0]), __float_as_int(big));
-        __syncthreads();
+        for (int r = 0; r < kAtRows; ++r)
+#pragma unroll
+            for (int d = 0; d < kPer; ++d) {
+                if (r >= nrows) qv[r][d] = 0.0f;
+                const float m = fabsf(qv[r][d]);
+                big = m < 3.4e38f ? fmaxf(big, m) : big;  // infinities and NaN keep to their rows
+            }
+        big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));
         // 2^qe brings the largest |q| into [2^13, 2^14)
-        const float qmax = __int_as_float(misc[0]);
-        const int qe = qmax > 0.0f ? max(-114, min(126, 13 - ilogbf(qmax))) : 0;
-        const float qpow = ldexpf(1.0f, qe);
-        const float qf = p.a.scale * kLog2e;
-#pragma unroll
-        for (int i = 0; i < (kRows + kAtWarps - 1) / kAtWarps; ++i) {
-            const int r = warp + i * kAtWarps;
-            if (r < kRows) {
-                __half *dst = reinterpret_cast<__half *>(qfrag);
-#pragma unroll
-                for (int d = 0; d < D / 32; ++d) {
-                    // dimension -> (word of 8, nibble) -> (group, lane t, word of the lane)
-                    const int dim = d * 32 + lane, word = dim / 8, nib = dim % 8;
-                    const int gr = dim / kG, wi = word - gr * (kG / 8), tt = wi / kWords, j = wi % kWords;
-                    // registers: {0,4} {1,5} {2,6} {3,7}; odd nibbles carry 2^-4
-                    const int reg = nib & 3, half = nib >> 2;
-                    const int frag = ((r / 8) * (D / 32) + gr * kWords + j) * 32 + (r % 8) * 4 + tt;
-                    dst[frag * 8 + reg * 2 + half] = __float2half_rn(qv[i][d] * qpow * (nib & 1 ? 0.0625f : 1.0f));
-                }
-#pragma unroll
-                for (int gr = 0; gr < kNG; ++gr) {
-                    float s = 0.0f;
-#pragma unroll
-                    for (int d = gr * (kG / 32); d < (gr + 1) * (kG / 32); ++d) s += qv[i][d];
-#pragma unroll
-                    for (int m = 16; m; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
-                    if (lane == 0) qsum[r * kNG + gr] = s * qf;
-                }
-            }
-        }
-        __syncthreads();
+        const int qe = big > 0.0f ? max(-100, min(126, 13 - ilogbf(big))) : 0;
+        const float qpow = ldexpf(1.0f, qe), qf = p.a.scale * kLog2e;
         const float raw = ldexpf(qf, 24 - qe);  // of q . c as the tensor core sums it
-        float qs[kNT][2][kNG];
-        int2 lm[kNT][2];
-        int lo_max = 0, hi_min = sw.len;
-        for (int r = 0; r < nrows; ++r) {
-            lo_max = max(lo_max, lim[r].x);
-            hi_min = min(hi_min, lim[r].y);
-        }
+        float qs[2][kNG];
 #pragma unroll
-        for (int n = 0; n < kNT; ++n)
+        for (int gr = 0; gr < kNG; ++gr) qs[0][gr] = qs[1][gr] = 0.0f;
+        __syncwarp();
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                lm[n][c] = lim[n * 8 + 2 * t + c];
+        for (int r = 0; r < kAtRows; ++r) {
+            __half *dst = reinterpret_cast<__half *>(qfrag);
 #pragma unroll
-                for (int gr = 0; gr < kNG; ++gr) qs[n][c][gr] = qsum[(n * 8 + 2 * t + c) * kNG + gr];
+            for (int d = 0; d < kPer; ++d) {
+                // dimension -> (word of 8, nibble) -> (group, lane t, word of the lane)
+                const int dim = d * 32 + lane, word = dim / 8, nib = dim % 8;
+                const int gr = dim / kG, wi = word - gr * (kG / 8), tt = wi / kWords, j = wi % kWords;
+                // registers: {0,4} {1,5} {2,6} {3,7}; odd nibbles carry 2^-4
+                dst[((gr * kWords + j) * 32 + r * 4 + tt) * 8 + (nib & 3) * 2 + (nib >> 2)] =
+                    __float2half_rn(qv[r][d] * qpow * (nib & 1 ? 0.0625f : 1.0f));
             }
+#pragma unroll
+            for (int gr = 0; gr < kNG; ++gr) {
+                float s = 0.0f;
+#pragma unroll
+                for (int d = gr * (kG / 32); d < (gr + 1) * (kG / 32); ++d) s += qv[r][d];
+#pragma unroll
+                for (int m = 16; m; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
+                if (r / 2 == t) qs[r & 1][gr] = s * qf;
+            }
+        }
+        __syncwarp();
+        int2 lm[2];  // tokens that rows 2 t and 2 t + 1 see
+        int lo_max = 0, hi_min = 0x7fffffff;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int r = 2 * t + c, pos = sw.len - sw.n + (row0 + r) / heads;
+            lm[c].y = p.a.causal ? max(0, min(sw.len, pos + 1)) : sw.len;
+            lm[c].x = p.a.window ? max(0, pos - (int)p.a.window + 1) : 0;
+            if (r < nrows) lo_max = max(lo_max, lm[c].x), hi_min = min(hi_min, lm[c].y);
+        }
+        lo_max = __reduce_max_sync(0xffffffffu, lo_max);
+        hi_min = __reduce_min_sync(0xffffffffu, hi_min);
 
-        float acc[kVB][4][kNT][4];
-        float mx[kNT][2], ls[kNT][2], om[kNT][2][kNG];
-        float ws[kNG][kNT][4];  // sum w (rows of the accumulator are alike)
+        float om[2][kNG], ws[kNG][4];  // sum p (low' + 7.5 scale'); sum w (rows of the accumulator are alike)
 #pragma unroll
         for (int v = 0; v < kVB; ++v)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int n = 0; n < kNT; ++n)
+                for (int c = 0; c < 4; ++c) acc[v][i][c] = 0.0f;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) acc[v][i][n][c] = 0.0f;
+        for (int c = 0; c < 2; ++c) {
+            mx[c] = -INFINITY;
+            ls[c] = 0.0f;
 #pragma unroll
-        for (int n = 0; n < kNT; ++n)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                mx[n][c] = -INFINITY;
-                ls[n][c] = 0.0f;
-#pragma unroll
-                for (int gr = 0; gr < kNG; ++gr) om[n][c][gr] = ws[gr][n][c] = ws[gr][n][c + 2] = 0.0f;
-            }
+            for (int gr = 0; gr < kNG; ++gr) om[c][gr] = ws[gr][c] = ws[gr][c + 2] = 0.0f;
+        }
         int vexp = 126;  // 2^-vexp bounds the value scales met: operands are p scale' 2^(15 + vexp)
         float vbound = 0.0f, vmul = 0.0f;
 
-        for (; u < seg_end; u += kAtWarps) {
-            const int tok0 = sw.first + (int)(u - job_u0) * kAtTile;
+        for (; tile < tile_end; ++tile) {
+            const int tok0 = sw.first + tile * kAtTile;
             if (pending) {  // (0 only after a wait ran out: nothing more is fetched then)
                 alive = __all_sync(0xffffffffu, mbar_wait_bounded(bars + stage, phase, p.c.status)) && alive;
                 --pending;
             }
             const unsigned char *st = ring + stage * S::kStage;
             const bool edge = tok0 + kAtTile > hi_min || tok0 < lo_max;
-            // ---- scores: two tiles of 16 tokens x 8 kNT rows ----
-            float s[2][kNT][4];
+            // ---- scores: two tiles of 16 tokens x 8 rows ----
+            float s[2][4];
             const int tg = g ^ ((g >> 1) & 1);  // the token of operand row g (and + 8): see below
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt) {
@@ -386,72 +409,58 @@ __global__ void __launch_bounds__(kAtThreads, kNT * D <= 128 ? 2 : 1) kv4_attend
                         *reinterpret_cast<uint2 *>(wa) = *reinterpret_cast<const uint2 *>(ka);
                         *reinterpret_cast<uint2 *>(wb) = *reinterpret_cast<const uint2 *>(ka + 8 * (D / 2));
                     }
-                    float d[kNT][4];
-#pragma unroll
-                    for (int n = 0; n < kNT; ++n)
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) d[n][c] = 0.0f;
+                    float d[4] = {};
 #pragma unroll
                     for (int j = 0; j < kWords; ++j) {
                         const uint32_t a8 = wa[j] >> 8, b8 = wb[j] >> 8;
-#pragma unroll
-                        for (int n = 0; n < kNT; ++n) {
-                            const uint4 q = qfrag[(n * (D / 32) + gr * kWords + j) * 32 + lane];
-                            mma16816<__half>(d[n], wa[j] & 0x000f000fu, wb[j] & 0x000f000fu, wa[j] & 0x00f000f0u,
-                                             wb[j] & 0x00f000f0u, q.x, q.y);
-                            mma16816<__half>(d[n], a8 & 0x000f000fu, b8 & 0x000f000fu, a8 & 0x00f000f0u,
-                                             b8 & 0x00f000f0u, q.z, q.w);
-                        }
+                        const uint4 q = qfrag[(gr * kWords + j) * 32 + lane];
+                        mma16816<__half>(d, wa[j] & 0x000f000fu, wb[j] & 0x000f000fu, wa[j] & 0x00f000f0u,
+                                         wb[j] & 0x00f000f0u, q.x, q.y);
+                        mma16816<__half>(d, a8 & 0x000f000fu, b8 & 0x000f000fu, a8 & 0x00f000f0u, b8 & 0x00f000f0u,
+                                         q.z, q.w);
                     }
                     const __half2 *km = reinterpret_cast<const __half2 *>(st + 2 * S::kCodes);
                     const float2 f0 = __half22float2(km[(mt * 16 + tg) * kNG + gr]);
                     const float2 f1 = __half22float2(km[(mt * 16 + 8 + tg) * kNG + gr]);
                     const float r0 = f0.x * raw, r1 = f1.x * raw;
 #pragma unroll
-                    for (int n = 0; n < kNT; ++n)
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            const float low = (c < 2 ? f0.y : f1.y) * qs[n][c & 1][gr];
-                            const float v = fmaf(c < 2 ? r0 : r1, d[n][c], low);
-                            s[mt][n][c] = gr ? s[mt][n][c] + v : v;
-                        }
+                    for (int c = 0; c < 4; ++c) {
+                        const float low = (c < 2 ? f0.y : f1.y) * qs[c & 1][gr];
+                        const float v = fmaf(c < 2 ? r0 : r1, d[c], low);
+                        s[mt][c] = gr ? s[mt][c] + v : v;
+                    }
                 }
             }
-            uint32_t hidden = 0;  // bit (mt * kNT + n) * 4 + c
+            uint32_t hidden = 0;  // bit 4 mt + c
             if (edge) {
 #pragma unroll
                 for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-                    for (int n = 0; n < kNT; ++n)
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            const int tok = tok0 + mt * 16 + tg + (c >> 1) * 8;
-                            const int2 l = lm[n][c & 1];
-                            if (tok < l.x || tok >= l.y) {
-                                s[mt][n][c] = -INFINITY;
-                                hidden |= 1u << ((mt * kNT + n) * 4 + c);
-                            }
+                    for (int c = 0; c < 4; ++c) {
+                        const int tok = tok0 + mt * 16 + tg + (c >> 1) * 8;
+                        if (tok < lm[c & 1].x || tok >= lm[c & 1].y) {
+                            s[mt][c] = -INFINITY;
+                            hidden |= 1u << (mt * 4 + c);
                         }
+                    }
             }
             // ---- running maximum ----
-            float al[kNT][2];
+            float al[2];
             bool moved = false;
 #pragma unroll
-            for (int n = 0; n < kNT; ++n)
+            for (int c = 0; c < 2; ++c) {
+                float m = fmaxf(fmaxf(s[0][c], s[0][c + 2]), fmaxf(s[1][c], s[1][c + 2]));
+                m = fmaxf(mx[c], max_over_g(m));
+                const float ref = m == -INFINITY ? 0.0f : m;
+                al[c] = ex2(mx[c] - ref);
+                moved |= m != mx[c];
+                mx[c] = m;
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    float m = fmaxf(fmaxf(s[0][n][c], s[0][n][c + 2]), fmaxf(s[1][n][c], s[1][n][c + 2]));
-                    m = fmaxf(mx[n][c], max_over_g(m));
-                    const float ref = m == -INFINITY ? 0.0f : m;
-                    al[n][c] = ex2(mx[n][c] - ref);
-                    moved |= m != mx[n][c];
-                    mx[n][c] = m;
-#pragma unroll
-                    for (int mt = 0; mt < 2; ++mt) {
-                        s[mt][n][c] = ex2(s[mt][n][c] - ref);
-                        s[mt][n][c + 2] = ex2(s[mt][n][c + 2] - ref);
-                    }
+                for (int mt = 0; mt < 2; ++mt) {
+                    s[mt][c] = ex2(s[mt][c] - ref);
+                    s[mt][c + 2] = ex2(s[mt][c + 2] - ref);
                 }
+            }
             // ---- value factors; the bound on their scales ----
             const __half2 *vm = reinterpret_cast<const __half2 *>(st + 2 * S::kCodes + S::kMeta);
             float2 vf[2][2][kNG];
@@ -481,48 +490,41 @@ __global__ void __launch_bounds__(kAtThreads, kNT * D <= 128 ? 2 : 1) kv4_attend
             }
             if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-                for (int n = 0; n < kNT; ++n)
+                for (int c = 0; c < 2; ++c) {
+                    ls[c] *= al[c];
+                    const float f = al[c] * shrink;
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        ls[n][c] *= al[n][c];
+                    for (int gr = 0; gr < kNG; ++gr) om[c][gr] *= al[c], ws[gr][c] *= f;
 #pragma unroll
-                        for (int gr = 0; gr < kNG; ++gr) om[n][c][gr] *= al[n][c];
-                        const float f = al[n][c] * shrink;
+                    for (int v = 0; v < kVB; ++v)
 #pragma unroll
-                        for (int gr = 0; gr < kNG; ++gr) ws[gr][n][c] *= f;
-#pragma unroll
-                        for (int v = 0; v < kVB; ++v)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                acc[v][i][n][c] *= f;
-                                acc[v][i][n][c + 2] *= f;
-                            }
-                    }
+                        for (int i = 0; i < 4; ++i) {
+                            acc[v][i][c] *= f;
+                            acc[v][i][c + 2] *= f;
+                        }
+                }
             }
             // ---- values: per 16 tokens, p scale' transposed into the 16-deep operand ----
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt) {
-                uint32_t pb[kNG][kNT][2];
+                uint32_t pb[kNG][2];
 #pragma unroll
-                for (int n = 0; n < kNT; ++n) {
+                for (int c = 0; c < 4; ++c) ls[c & 1] += s[mt][c];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) ls[n][c & 1] += s[mt][n][c];
+                for (int gr = 0; gr < kNG; ++gr) {
+                    float x[4];
 #pragma unroll
-                    for (int gr = 0; gr < kNG; ++gr) {
-                        float x[4];
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            const float2 f = vf[mt][c >> 1][gr];
-                            x[c] = s[mt][n][c] * (f.x * vmul);
-                            float y = s[mt][n][c] * f.y;
-                            if (edge && (hidden >> ((mt * kNT + n) * 4 + c) & 1)) x[c] = y = 0.0f;
-                            om[n][c & 1][gr] += y;
-                        }
-                        pb[gr][n][0] = transpose8x8(pack_half2(x[0], x[1]));
-                        pb[gr][n][1] = transpose8x8(pack_half2(x[2], x[3]));
-                        constexpr uint32_t one = 0x3c003c00u;
-                        mma16816<__half>(ws[gr][n], one, one, one, one, pb[gr][n][0], pb[gr][n][1]);
+                    for (int c = 0; c < 4; ++c) {
+                        const float2 f = vf[mt][c >> 1][gr];
+                        x[c] = s[mt][c] * (f.x * vmul);
+                        float y = s[mt][c] * f.y;
+                        if (edge && (hidden >> (mt * 4 + c) & 1)) x[c] = y = 0.0f;
+                        om[c & 1][gr] += y;
                     }
+                    pb[gr][0] = transpose8x8(pack_half2(x[0], x[1]));
+                    pb[gr][1] = transpose8x8(pack_half2(x[2], x[3]));
+                    constexpr uint32_t one = 0x3c003c00u;
+                    mma16816<__half>(ws[gr], one, one, one, one, pb[gr][0], pb[gr][1]);
                 }
                 // Operand row r of a 16-token tile is token r ^ (r >> 1 & 1): the four lanes t of
                 // a value load then read rows of both parities, two bank halves instead of one.
@@ -541,17 +543,14 @@ __global__ void __launch_bounds__(kAtThreads, kNT * D <= 128 ? 2 : 1) kv4_attend
                     const int gr = v * 64 / kG;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int n = 0; n < kNT; ++n)
-                            mma16816<__half>(acc[v][i][n], x[i] & 0x000f000fu, x[i] & 0x00f000f0u,
-                                             y[i] & 0x000f000fu, y[i] & 0x00f000f0u, pb[gr][n][0], pb[gr][n][1]);
+                        mma16816<__half>(acc[v][i], x[i] & 0x000f000fu, x[i] & 0x00f000f0u, y[i] & 0x000f000fu,
+                                         y[i] & 0x00f000f0u, pb[gr][0], pb[gr][1]);
                 }
             }
             // ---- the stage is read: refill it ----
             __syncwarp();
             if (ahead < u1 && alive) {
-                fetch(ahead, fstage);
-                ahead += kAtWarps;
+                fetch(fstage);
                 ++pending;
             }
             if (++fstage == kAtStages) fstage = 0;
@@ -560,152 +559,194 @@ __global__ void __launch_bounds__(kAtThreads, kNT * D <= 128 ? 2 : 1) kv4_attend
                 phase ^= 1;
             }
         }
+        u = seg_end;
 
-        // ---- join the warps ----
+        // ---- the warp's result of this job: acc becomes sum p v, ls the sum over its tokens ----
         const float opow = ldexpf(1.0f, 9 - vexp);  // 2^24 of the codes, 2^-(15 + vexp) of the operand
 #pragma unroll
-        for (int n = 0; n < kNT; ++n)
+        for (int c = 0; c < 2; ++c) {
+            ls[c] = sum_over_g(ls[c]);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const float l = sum_over_g(ls[n][c]);
-                const int r = n * 8 + 2 * t + c;
-                if (g == 0) stat[warp * kRows + r] = make_float2(mx[n][c], l);
+            for (int gr = 0; gr < kNG; ++gr) {
+                const float o = fmaf(ws[gr][c], -7.5f * 5.9604644775390625e-8f * opow, sum_over_g(om[c][gr]));
 #pragma unroll
-                for (int gr = 0; gr < kNG; ++gr) {
-                    const float o = fmaf(ws[gr][n][c], -7.5f * 5.9604644775390625e-8f * opow, sum_over_g(om[n][c][gr]));
-                    if (g == 0) omw[(warp * kRows + r) * kNG + gr] = o;
-                }
+                for (int v = gr * (kG / 64); v < (gr + 1) * (kG / 64); ++v)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        acc[v][i][c] = fmaf(acc[v][i][c], opow, o);
+                        acc[v][i][c + 2] = fmaf(acc[v][i][c + 2], opow * 0.0625f, o);
+                    }
             }
-        __syncthreads();
-        if (threadIdx.x < kRows) {
-            float m = -INFINITY, l = 0.0f;
-            for (int w = 0; w < kAtWarps; ++w) m = fmaxf(m, stat[w * kRows + threadIdx.x].x);
-            for (int w = 0; w < kAtWarps; ++w) {
-                const float2 f = stat[w * kRows + threadIdx.x];
-                l += f.y * ex2(f.x == -INFINITY ? -INFINITY : f.x - m);
-            }
-            fin[threadIdx.x] = make_float2(m, l);
         }
-        const bool whole = seg == job_u0 && seg_end == job_u1;
-        // A block's first job may have begun in an earlier block (slot 0); its last may go on (1).
-        const int slot = 2 * blockIdx.x + (seg == job_u0 ? 1 : 0);
-        float *po = p.part + (size_t)slot * kRows * D;
-        float *ps = p.part + (size_t)2 * gridDim.x * kRows * D + (size_t)slot * kRows * 2;
-        __syncthreads();
-        float wf[kNT][2];
-#pragma unroll
-        for (int n = 0; n < kNT; ++n)
+        const bool whole = u0 <= job_u0 + 1 && seg_end == job_u1;  // all its tiles are ours
+        if (whole) {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const float m = fin[n * 8 + 2 * t + c].x;
-                wf[n][c] = mx[n][c] == -INFINITY ? 0.0f : ex2(mx[n][c] - m);
-            }
-        T *out = static_cast<T *>(p.a.out);
-        for (int v = 0; v < kVB; ++v) {
+                const int r = 2 * t + c, row = row0 + r;
+                if (r < nrows) {
+                    const int tk = row / heads;
+                    const int64_t at = (int64_t)(sw.q0 + tk) * p.a.q_heads + head * heads + row - tk * heads;
+                    const float inv = ls[c] == 0.0f ? 0.0f : 1.0f / ls[c];
 #pragma unroll
-            for (int n = 0; n < kNT; ++n)
+                    for (int v = 0; v < kVB; ++v) {
+                        float x[8];
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int r = n * 8 + 2 * t + c;
-                    const float o = omw[(warp * kRows + r) * kNG + v * 64 / kG];
-                    float x[8];
-#pragma unroll
-                    for (int vv = 0; vv < kVB; ++vv)
-                        if (vv == v) {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                x[2 * i] = wf[n][c] * fmaf(acc[vv][i][n][c], opow, o);
-                                x[2 * i + 1] = wf[n][c] * fmaf(acc[vv][i][n][c + 2], opow * 0.0625f, o);
-                            }
+                        for (int i = 0; i < 4; ++i) {
+                            x[2 * i] = ls[c] == 0.0f ? 0.0f : acc[v][i][c] * inv;
+                            x[2 * i + 1] = ls[c] == 0.0f ? 0.0f : acc[v][i][c + 2] * inv;
                         }
-                    if (wf[n][c] == 0.0f) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) x[i] = 0.0f;
+                        store8(out + at * D + v * 64 + g * 8, x);
                     }
-                    float4 *dst = reinterpret_cast<float4 *>(red + (warp * kRows + r) * 64 + g * 8);
-                    dst[0] = make_float4(x[0], x[1], x[2], x[3]);
-                    dst[1] = make_float4(x[4], x[5], x[6], x[7]);
-                }
-            __syncthreads();
-            for (int e = threadIdx.x; e < kRows * 64; e += kAtThreads) {
-                const int r = e / 64, d = v * 64 + e % 64;
-                float sum = 0.0f;
-#pragma unroll
-                for (int w = 0; w < kAtWarps; ++w) sum += red[w * kRows * 64 + e];
-                if (!whole) {
-                    __stcg(po + r * D + d, sum);
-                } else if (r < nrows) {
-                    const float l = fin[r].y;
-                    const int row = row0 + r;
-                    out[((int64_t)(sw.q0 + row / heads) * p.a.q_heads + head * heads + row % heads) * D + d] =
-                        from_f32<T>(l == 0.0f ? 0.0f : sum / l);
+                    if (p.a.lse && g == 0) p.a.lse[at] = ls[c] == 0.0f ? -INFINITY : (mx[c] + log2f(ls[c])) / kLog2e;
                 }
             }
-            __syncthreads();
+            continue;
         }
-        if (threadIdx.x < nrows) {
-            const float2 f = fin[threadIdx.x];
+        // Not whole: it waits for the other warps. The last job's part goes to shared memory (the
+        // ring has run dry), an earlier one's (the run's first job) to the workspace.
+        const bool last = u >= u1;
+        if (lane == 0) keys[2 * warp + (last ? 1 : 0)] = job_u0;
+        float *dst = last ? reinterpret_cast<float *>(ring) : part_warp;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int r = 2 * t + c;
+#pragma unroll
+            for (int v = 0; v < kVB; ++v) {
+                float4 *at = reinterpret_cast<float4 *>(dst + r * D + v * 64 + g * 8);
+                at[0] = make_float4(acc[v][0][c], acc[v][0][c + 2], acc[v][1][c], acc[v][1][c + 2]);
+                at[1] = make_float4(acc[v][2][c], acc[v][2][c + 2], acc[v][3][c], acc[v][3][c + 2]);
+            }
+            if (g == 0) *reinterpret_cast<float2 *>(dst + kAtRows * D + 2 * r) = make_float2(mx[c], ls[c]);
+        }
+    }
+
+    // ---- jobs cut over this block's warps ----
+    __syncthreads();
+    for (int e0 = 0; e0 < 2 * kAtWarps;) {
+        const int64_t job_u0 = keys[e0];
+        if (job_u0 < 0) {
+            ++e0;
+            continue;
+        }
+        int e1 = e0 + 1;  // entries [e0, e1) are this job's, or empty
+        while (e1 < 2 * kAtWarps && (keys[e1] < 0 || keys[e1] == job_u0)) ++e1;
+        const int bb = find(job_u0);
+        const SeqWork s = seq(bb);
+        const uint32_t jn = s.tiles + 1, job = (uint32_t)(job_u0 - base[bb]) / jn;
+        const int head = (int)(job / s.row_tiles), row0 = (int)(job - head * s.row_tiles) * kAtRows;
+        const int nrows = min(kAtRows, s.n * heads - row0);
+        const int64_t job_u1 = job_u0 + jn;
+        const bool starts = b0 <= job_u0 + 1, whole = starts && b1 >= job_u1;
+        float *slot = p.part + (size_t)(2 * blockIdx.x + (starts ? 1 : 0)) * kAtPart<D>;
+        for (int i = threadIdx.x; i < nrows * (D / 4); i += kAtThreads) {
+            const int r = i / (D / 4), d = i % (D / 4) * 4;
+            auto entry = [&](int e) {
+                return e & 1 ? reinterpret_cast<const float *>(at_smem + S::ring + (e >> 1) * S::kRing)
+                             : p.part + (size_t)2 * gridDim.x * kAtPart<D> + (size_t)(blockIdx.x * kAtWarps + (e >> 1)) * kAtPart<D>;
+            };
+            float m = -INFINITY, l = 0.0f;
+            for (int e = e0; e < e1; ++e)
+                if (keys[e] >= 0) m = fmaxf(m, entry(e)[kAtRows * D + 2 * r]);
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int e = e0; e < e1; ++e) {
+                if (keys[e] < 0) continue;
+                const float *en = entry(e);
+                const float2 f = *reinterpret_cast<const float2 *>(en + kAtRows * D + 2 * r);
+                const float4 x = *reinterpret_cast<const float4 *>(en + r * D + d);
+                const float k = f.x == -INFINITY ? 0.0f : ex2(f.x - m);
+                l += f.y * (f.x == -INFINITY && f.y != 0.0f ? 1.0f : k);
+                if (k != 0.0f) {
+                    sum.x = fmaf(k, x.x, sum.x), sum.y = fmaf(k, x.y, sum.y);
+                    sum.z = fmaf(k, x.z, sum.z), sum.w = fmaf(k, x.w, sum.w);
+                }
+            }
             if (!whole) {
-                __stcg(reinterpret_cast<float2 *>(ps) + threadIdx.x, f);
-            } else if (p.a.lse) {
-                const int row = row0 + threadIdx.x;
-                p.a.lse[(int64_t)(sw.q0 + row / heads) * p.a.q_heads + head * heads + row % heads] =
-                    f.y == 0.0f ? -INFINITY : (f.x + log2f(f.y)) / kLog2e;
+                __stcg(reinterpret_cast<float4 *>(slot + r * D + d), sum);
+                if (d == 0) __stcg(reinterpret_cast<float2 *>(slot + kAtRows * D + 2 * r), make_float2(m, l));
+                continue;
             }
+            const int row = row0 + r, tk = row / heads;
+            const int64_t at = (int64_t)(s.q0 + tk) * p.a.q_heads + head * heads + row - tk * heads;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            store4(out + at * D + d, sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+            if (d == 0 && p.a.lse) p.a.lse[at] = l == 0.0f ? -INFINITY : (m + log2f(l)) / kLog2e;
         }
-        if (!whole) {
-            // the blocks that hold parts of this job: the first is named by the job's first unit
-            // (the run that holds unit x is the last i with i U / B < x + 1)
-            auto owner = [&](int64_t x) { return (int)(((x + 1) * blocks - 1) / units); };
-            const int first = owner(job_u0), last = owner(job_u1 - 1);
-            __threadfence();
-            __syncthreads();
-            if (threadIdx.x == 0) misc[1] = (int)atomicAdd(p.arrived + first, 1u) == last - first;
-            __syncthreads();
-            if (misc[1]) {
-                __threadfence();
-                if (threadIdx.x == 0) p.arrived[first] = 0;
-                const float *ap = p.part, *as = p.part + (size_t)2 * gridDim.x * kRows * D;
-                // the first block's part is in its slot 1, the others' in their slot 0
-                if (threadIdx.x < nrows) {
-                    float m = -INFINITY, l = 0.0f;
-                    for (int i = first; i <= last; ++i)
-                        m = fmaxf(m, __ldcg(as + ((size_t)(2 * i + (i == first)) * kRows + threadIdx.x) * 2));
-                    for (int i = first; i <= last; ++i) {
-                        const float2 f = __ldcg(reinterpret_cast<const float2 *>(as) + (size_t)(2 * i + (i == first)) * kRows + threadIdx.x);
-                        l += f.y * ex2(f.x == -INFINITY ? -INFINITY : f.x - m);
-                    }
-                    fin[threadIdx.x] = make_float2(m, l);
-                    if (p.a.lse) {
-                        const int row = row0 + threadIdx.x;
-                        p.a.lse[(int64_t)(sw.q0 + row / heads) * p.a.q_heads + head * heads + row % heads] =
-                            l == 0.0f ? -INFINITY : (m + log2f(l)) / kLog2e;
-                    }
-                }
-                __syncthreads();
-                for (int e = threadIdx.x; e < nrows * (D / 4); e += kAtThreads) {
-                    const int r = e / (D / 4), d = e % (D / 4) * 4;
-                    const float2 f = fin[r];
-                    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-                    for (int i = first; i <= last; ++i) {
-                        const size_t sl = (size_t)(2 * i + (i == first)) * kRows + r;
-                        const float m = __ldcg(as + sl * 2);
-                        const float4 x = __ldcg(reinterpret_cast<const float4 *>(ap + sl * D + d));
-                        const float k = m == -INFINITY ? 0.0f : ex2(m - f.x);
-                        sum.x = fmaf(k, x.x, sum.x), sum.y = fmaf(k, x.y, sum.y);
-                        sum.z = fmaf(k, x.z, sum.z), sum.w = fmaf(k, x.w, sum.w);
-                    }
-                    const float inv = f.y == 0.0f ? 0.0f : 1.0f / f.y;
-                    const int row = row0 + r;
-                    T *dst = out + ((int64_t)(sw.q0 + row / heads) * p.a.q_heads + head * heads + row % heads) * D + d;
-                    dst[0] = from_f32<T>(sum.x * inv), dst[1] = from_f32<T>(sum.y * inv);
-                    dst[2] = from_f32<T>(sum.z * inv), dst[3] = from_f32<T>(sum.w * inv);
+        e0 = e1;
+        if (whole) continue;
+
+        // ---- cut over blocks: the last to arrive joins (unit x is in block (x B + B - 1) / U) ----
+        const int first = (int)(((job_u0 + 2) * blocks - 1) / units), last = (int)((job_u1 * blocks - 1) / units);
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) misc[1] = (int)atomicAdd(p.arrived + first, 1u) == last - first;
+        __syncthreads();
+        if (!misc[1]) continue;
+        __threadfence();
+        if (threadIdx.x == 0) p.arrived[first] = 0;
+        // the first block's part is in its slot 1, the others' in their slot 0
+        auto slot_of = [&](int i) { return p.part + (size_t)(2 * i + (i == first ? 1 : 0)) * kAtPart<D>; };
+        const int parts = last - first + 1;
+        float2 *fin = reinterpret_cast<float2 *>(at_smem + S::qfrag);  // [row] (maximum, 1 / sum)
+        float4 *red = reinterpret_cast<float4 *>(at_smem + S::qfrag + 128);
+        __syncthreads();
+        {  // a warp per row, a lane per part
+            const int r = warp;
+            float m = -INFINITY, l = 0.0f;
+            for (int i = lane; i < parts; i += 32) m = fmaxf(m, __ldcg(slot_of(first + i) + kAtRows * D + 2 * r));
+#pragma unroll
+            for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            for (int i = lane; i < parts; i += 32) {
+                const float2 f = __ldcg(reinterpret_cast<const float2 *>(slot_of(first + i) + kAtRows * D) + r);
+                l += f.y * (f.x == -INFINITY ? (f.y != 0.0f ? 1.0f : 0.0f) : ex2(f.x - m));
+            }
+#pragma unroll
+            for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+            if (lane == 0) {
+                fin[r] = make_float2(m, l == 0.0f ? 0.0f : 1.0f / l);
+                if (r < nrows && p.a.lse) {
+                    const int row = row0 + r, tk = row / heads;
+                    p.a.lse[(int64_t)(s.q0 + tk) * p.a.q_heads + head * heads + row - tk * heads] =
+                        l == 0.0f ? -INFINITY : (m + log2f(l)) / kLog2e;
                 }
             }
         }
         __syncthreads();
-        seg = seg_end;
+        // threads: (a share of the parts, if there are threads to spare) x (row, 4 dimensions)
+        const int items = nrows * (D / 4), groups = max(1, kAtThreads / items);
+        for (int i0 = 0; i0 < items; i0 += kAtThreads) {
+            const int gi = threadIdx.x / items, i = groups > 1 ? threadIdx.x % items : i0 + threadIdx.x;
+            const bool on = i < items && gi < groups;
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            const int r = i / (D / 4), d = i % (D / 4) * 4;
+            if (on) {
+#pragma unroll 8
+                for (int k = groups > 1 ? gi : 0; k < parts; k += groups) {
+                    const float4 x = __ldcg(reinterpret_cast<const float4 *>(slot_of(first + k) + r * D + d));
+                    const float pm = __ldcg(slot_of(first + k) + kAtRows * D + 2 * r);
+                    const float w = pm == -INFINITY ? 0.0f : ex2(pm - fin[r].x);
+                    if (w != 0.0f) {
+                        sum.x = fmaf(w, x.x, sum.x), sum.y = fmaf(w, x.y, sum.y);
+                        sum.z = fmaf(w, x.z, sum.z), sum.w = fmaf(w, x.w, sum.w);
+                    }
+                }
+            }
+            if (groups > 1) {
+                if (on) red[gi * items + i] = sum;
+                __syncthreads();
+                if (on && gi == 0)
+                    for (int k = 1; k < groups; ++k) {
+                        const float4 x = red[k * items + i];
+                        sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+                    }
+            }
+            if (on && gi == 0) {
+                const float inv = fin[r].y;
+                const int row = row0 + r, tk = row / heads;
+                store4(out + ((int64_t)(s.q0 + tk) * p.a.q_heads + head * heads + row - tk * heads) * D + d, sum.x * inv,
+                       sum.y * inv, sum.z * inv, sum.w * inv);
+            }
+        }
+        __syncthreads();
     }
 }
 

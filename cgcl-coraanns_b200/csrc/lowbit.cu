@@ -112,29 +112,30 @@ void append(const cora_kv4_cache *c, const cora_kv4_append_args *a, cudaStream_t
 uint64_t attend_rows(const cora_kv4_cache &c, uint64_t q_heads, uint64_t max_queries) {
     return std::max<uint64_t>(1, max_queries) * (q_heads / c.kv_heads);
 }
-constexpr uint64_t kFewRows = 8;
+constexpr uint64_t kFewRows = kAtRows;
 uint64_t attend_counters() { return ((uint64_t)sm_count() * 2 * 4 + 255) / 256 * 256; }
 // Workspace: the arrival counters first (they are the part that has to start at zero), then two
 // partial results per block.
 uint64_t attend_workspace(const cora_kv4_cache &c, uint64_t rows) {
     const uint64_t blocks = sm_count();
-    const uint64_t parts = rows <= kFewRows ? 2 * (2 * blocks) * 8 : 2 * blocks * (rows <= 128 || c.head_dim == 256 ? 128 : 256);
+    // few rows: two parts of 8 rows per block and one per warp, two blocks per SM
+    const uint64_t parts = rows <= kFewRows ? (2 * blocks) * (2 + kAtWarps) * kAtRows
+                                            : 2 * blocks * (rows <= 128 || c.head_dim == 256 ? 128 : 256);
     return attend_counters() + parts * (c.head_dim + 2) * 4;
 }
 
-template <typename T, int D, int kNG, int kNT>
+template <typename T, int D, int kNG>
 void launch_attend(AttendParams p, cudaStream_t st) {
-    auto *kern = kv4_attend_kernel<T, D, kNG, kNT>;
-    using S = AttendSmem<D, kNG, kNT>;
+    auto *kern = kv4_attend_kernel<T, D, kNG>;
+    using S = AttendSmem<D, kNG>;
+    static_assert(S::bytes(kAtMaxSeqs) <= (D <= 128 ? 115 : 227) * 1024, "");
     static int seen[64] = {};
-    const size_t sm = S::bytes(kAtMaxSeqs);
-    allow_smem(kern, sm, seen);
+    allow_smem(kern, S::bytes(kAtMaxSeqs), seen);
     const uint32_t seqs = p.a.seqs;
     for (uint32_t s0 = 0; s0 < seqs; s0 += kAtMaxSeqs) {
         p.seq0 = s0;
         p.seqs = std::min<uint32_t>(kAtMaxSeqs, seqs - s0);
-        const unsigned blocks = sm_count() * (kNT * D <= 128 ? 2 : 1);
-        kern<<<blocks, kAtThreads, S::bytes(p.seqs), st>>>(p);
+        kern<<<sm_count() * (D <= 128 ? 2 : 1), kAtThreads, S::bytes(p.seqs), st>>>(p);
         CUDA_TRY(cudaGetLastError());
     }
 }
@@ -160,6 +161,7 @@ void attend(const cora_kv4_cache *c, const cora_kv4_attend_args *a, cudaStream_t
     need(a, "null arguments");
     if (a->seqs == 0 || a->q_tokens == 0) return;
     need(a->q && a->out && a->page_table && a->lens, "q, out, page_table and lens are needed");
+    need(aligned16(a->out), "out must be 16-byte aligned");
     need(a->q_heads >= 1 && a->q_heads % c->kv_heads == 0, "q_heads must be a multiple of kv_heads");
     need(a->q_tokens <= INT_MAX && a->seqs <= INT_MAX, "too many rows");
     need(a->q_start || a->q_tokens >= a->seqs, "q needs a row per sequence where q_start is null");
@@ -179,7 +181,7 @@ void attend(const cora_kv4_cache *c, const cora_kv4_attend_args *a, cudaStream_t
         using T = decltype(z);
         auto go = [&](auto d, auto ng) {
             constexpr int D = decltype(d)::value, NG = decltype(ng)::value;
-            if (rows <= kFewRows) launch_attend<T, D, NG, 1>(p, st);
+            if (rows <= kFewRows) launch_attend<T, D, NG>(p, st);
             else if (rows <= 128 || D == 256) launch_chunk<T, D, NG, 1>(p, st);
             else launch_chunk<T, D, NG, D == 256 ? 1 : 2>(p, st);
         };
