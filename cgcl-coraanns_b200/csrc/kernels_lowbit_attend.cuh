@@ -201,10 +201,14 @@ __global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kerne
         }
         return lo;
     };
-    // Equal runs: warp i of B blocks holds units [i U / 8 B, (i + 1) U / 8 B).
+    // Equal runs: with W warps, warp i holds units [cut(i), cut(i + 1)), cut(i) = floor(i U / W).
     const bool aligned = misc[2] != 0;
-    const int64_t blocks = aligned ? misc[2] : max((int64_t)1, min((int64_t)gridDim.x, units / (kAtMinRun * kAtWarps)));
+    const int blocks = aligned ? misc[2] : (int)max((int64_t)1, min((int64_t)gridDim.x, units / (kAtMinRun * kAtWarps)));
     if (blockIdx.x >= blocks || !units) return;
+    const uint32_t workers = blocks * kAtWarps;
+    const int64_t each = units >> 32 ? units / workers : (uint32_t)units / workers;
+    const uint32_t more = (uint32_t)(units - each * workers);
+    auto even = [&](uint32_t i) { return each * i + more * i / workers; };  // more i < 2368^2
     int64_t b0 = 0, b1 = 0;  // this block's units
     if (aligned) {  // one job per block: the block's number counts jobs
         int64_t job = blockIdx.x;
@@ -218,10 +222,10 @@ __global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kerne
             job -= n;
         }
     } else {
-        b0 = blockIdx.x * units / blocks, b1 = (blockIdx.x + 1) * units / blocks;
+        b0 = even(blockIdx.x * kAtWarps), b1 = even((blockIdx.x + 1) * kAtWarps);
     }
-    auto cut = [&](int64_t w) {
-        return aligned ? w * (b1 - b0) / kAtWarps + b0 : (blockIdx.x * kAtWarps + w) * units / (blocks * kAtWarps);
+    auto cut = [&](uint32_t w) {
+        return aligned ? b0 + w * (uint32_t)(b1 - b0) / kAtWarps : even(blockIdx.x * kAtWarps + w);
     };
     const int64_t u0 = cut(warp), u1 = cut(warp + 1);
 
@@ -241,6 +245,14 @@ __global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kerne
         const int tok = fs.first + ftile * kAtTile + piece * per;
         fpage = piece * per < kAtTile && tok < fs.len ? __ldg(ftable + (tok >> shift)) : -2;
     };
+    auto fetch_q = [&]() {  // the job's queries, into L2 ahead of the copies that crowd the memory
+        constexpr int kLines = D / 64;  // 128-byte lines of a row
+        const int row = frt * kAtRows + lane / kLines, tk = row / heads;
+        if (lane < kAtRows * kLines && row < fs.n * heads)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const T *>(p.a.q) + (int64_t)(fs.q0 + tk) * p.a.q_token +
+                                                          (int64_t)(fhead * heads + row - tk * heads) * p.a.q_head +
+                                                          lane % kLines * 64));
+    };
     auto fetch_seek = [&]() {  // to unit `ahead`, or past it where that is a job's first (no tile)
         if (ahead >= u1) return;
         fb = find(ahead);
@@ -251,7 +263,10 @@ __global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kerne
         fhead = (int)(job / fs.row_tiles);
         frt = (int)(job - fhead * fs.row_tiles);
         if (ftile < 0) ++ahead, ftile = 0;
-        if (ahead < u1) fetch_page();
+        if (ahead < u1) {
+            fetch_page();
+            fetch_q();
+        }
     };
     auto fetch = [&](int stage) {
         const bool got = fpage != -2, ok = got && fpage >= 0 && (uint32_t)fpage < p.c.num_pages;
@@ -271,7 +286,10 @@ __global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kerne
         if (ahead >= base[fb + 1]) return fetch_seek();
         ++ahead, ftile = 0;  // the next job's own unit
         if (++frt == fs.row_tiles) frt = 0, ++fhead;
-        if (ahead < u1) fetch_page();
+        if (ahead < u1) {
+            fetch_page();
+            fetch_q();
+        }
     };
     int fstage = 0, pending = 0;  // tiles in flight
     fetch_seek();
@@ -284,6 +302,7 @@ __global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kerne
     float *const part_warp = p.part + (size_t)2 * gridDim.x * kAtPart<D> + (size_t)(blockIdx.x * kAtWarps + warp) * kAtPart<D>;
 
     T *const out = static_cast<T *>(p.a.out);
+    const bool q_vec = reinterpret_cast<uintptr_t>(p.a.q) % 8 == 0 && p.a.q_token % 4 == 0 && p.a.q_head % 4 == 0;
     float acc[kVB][4][4], mx[2], ls[2];
     int b = -1;
     SeqWork sw{};
@@ -304,24 +323,29 @@ __global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kerne
             u = seg_end;
             continue;
         }
-        // queries: rows are (token, head of the group); fp16 under a common power of two
-        constexpr int kPer = D / 32;  // dimensions of a lane
-        float qv[kAtRows][kPer];
+        // queries: rows are (token, head of the group); fp16 under a common power of two. A lane
+        // loads 4 dimensions of a row at a time.
+        constexpr int kLoads = kAtRows * D / 4 / 32;
+        T qv[kLoads][4];
         float big = 0.0f;
 #pragma unroll
-        for (int r = 0; r < kAtRows; ++r) {
+        for (int i = 0; i < kLoads; ++i) {
+            const int r = (i * 32 + lane) / (D / 4), d = (i * 32 + lane) % (D / 4) * 4;
             const int row = row0 + min(r, nrows - 1), tk = row / heads;
             const T *src = static_cast<const T *>(p.a.q) + (int64_t)(sw.q0 + tk) * p.a.q_token +
-                           (int64_t)(head * heads + row - tk * heads) * p.a.q_head;
+                           (int64_t)(head * heads + row - tk * heads) * p.a.q_head + d;
+            if (q_vec) {
+                *reinterpret_cast<uint2 *>(qv[i]) = *reinterpret_cast<const uint2 *>(src);
+            } else {
 #pragma unroll
-            for (int d = 0; d < kPer; ++d) qv[r][d] = to_f32(src[d * 32 + lane]);
+                for (int e = 0; e < 4; ++e) qv[i][e] = src[e];
+            }
         }
 #pragma unroll
-        for (int r = 0; r < kAtRows; ++r)
+        for (int i = 0; i < kLoads; ++i)
 #pragma unroll
-            for (int d = 0; d < kPer; ++d) {
-                if (r >= nrows) qv[r][d] = 0.0f;
-                const float m = fabsf(qv[r][d]);
+            for (int e = 0; e < 4; ++e) {
+                const float m = fabsf(to_f32(qv[i][e]));
                 big = m < 3.4e38f ? fmaxf(big, m) : big;  // infinities and NaN keep to their rows
             }
         big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));
@@ -329,33 +353,40 @@ __global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kerne
         const int qe = big > 0.0f ? max(-100, min(126, 13 - ilogbf(big))) : 0;
         const float qpow = ldexpf(1.0f, qe), qf = p.a.scale * kLog2e;
         const float raw = ldexpf(qf, 24 - qe);  // of q . c as the tensor core sums it
-        float qs[2][kNG];
-#pragma unroll
-        for (int gr = 0; gr < kNG; ++gr) qs[0][gr] = qs[1][gr] = 0.0f;
         __syncwarp();
 #pragma unroll
-        for (int r = 0; r < kAtRows; ++r) {
-            __half *dst = reinterpret_cast<__half *>(qfrag);
+        for (int i = 0; i < kLoads; ++i) {
+            const int r = (i * 32 + lane) / (D / 4), d = (i * 32 + lane) % (D / 4) * 4;
+            // Dimensions d .. d + 3 are nibbles 0..3 (even lanes) or 4..7 (odd ones) of their
+            // word of 8; the operand pairs nibbles {0,4} {1,5} {2,6} {3,7}, the odd ones under
+            // 2^-4: neighbouring lanes swap halves, and each stores two pairs.
+            float x[4];
 #pragma unroll
-            for (int d = 0; d < kPer; ++d) {
-                // dimension -> (word of 8, nibble) -> (group, lane t, word of the lane)
-                const int dim = d * 32 + lane, word = dim / 8, nib = dim % 8;
-                const int gr = dim / kG, wi = word - gr * (kG / 8), tt = wi / kWords, j = wi % kWords;
-                // registers: {0,4} {1,5} {2,6} {3,7}; odd nibbles carry 2^-4
-                dst[((gr * kWords + j) * 32 + r * 4 + tt) * 8 + (nib & 3) * 2 + (nib >> 2)] =
-                    __float2half_rn(qv[r][d] * qpow * (nib & 1 ? 0.0625f : 1.0f));
-            }
-#pragma unroll
-            for (int gr = 0; gr < kNG; ++gr) {
-                float s = 0.0f;
-#pragma unroll
-                for (int d = gr * (kG / 32); d < (gr + 1) * (kG / 32); ++d) s += qv[r][d];
-#pragma unroll
-                for (int m = 16; m; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
-                if (r / 2 == t) qs[r & 1][gr] = s * qf;
-            }
+            for (int e = 0; e < 4; ++e) x[e] = r < nrows ? to_f32(qv[i][e]) * qpow * (e & 1 ? 0.0625f : 1.0f) : 0.0f;
+            const uint32_t lo = pack_half2(x[0], x[1]), hi = pack_half2(x[2], x[3]);
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, lane & 1 ? lo : hi, 1);
+            uint2 w;
+            w.x = lane & 1 ? __byte_perm(other, hi, 0x5410) : __byte_perm(lo, other, 0x5410);
+            w.y = lane & 1 ? __byte_perm(other, hi, 0x7632) : __byte_perm(lo, other, 0x7632);
+            // word -> (group, lane t, word of the lane)
+            const int word = d / 8, gr = d / kG, wi = word - gr * (kG / 8), tt = wi / kWords, j = wi % kWords;
+            reinterpret_cast<uint2 *>(qfrag + (gr * kWords + j) * 32 + r * 4 + tt)[lane & 1] = w;
         }
         __syncwarp();
+        float qs[2][kNG];  // sums of q per group, by the same operands against ones (and 16s)
+#pragma unroll
+        for (int gr = 0; gr < kNG; ++gr) {
+            float d[4] = {};
+            constexpr uint32_t one = 0x3c003c00u, sixteen = 0x4c004c00u;
+#pragma unroll
+            for (int j = 0; j < kWords; ++j) {
+                const uint4 q = qfrag[(gr * kWords + j) * 32 + lane];
+                mma16816<__half>(d, one, one, sixteen, sixteen, q.x, q.y);
+                mma16816<__half>(d, one, one, sixteen, sixteen, q.z, q.w);
+            }
+            const float f = ldexpf(qf, -qe);
+            qs[0][gr] = d[0] * f, qs[1][gr] = d[1] * f;
+        }
         int2 lm[2];  // tokens that rows 2 t and 2 t + 1 see
         int lo_max = 0, hi_min = 0x7fffffff;
 #pragma unroll
@@ -620,16 +651,19 @@ __global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kerne
         }
     }
 
-    // ---- jobs cut over this block's warps ----
+    // ---- jobs cut over this block's warps: entries 2 w, 2 w + 1 are warp w's parts ----
     __syncthreads();
-    for (int e0 = 0; e0 < 2 * kAtWarps;) {
-        const int64_t job_u0 = keys[e0];
-        if (job_u0 < 0) {
-            ++e0;
-            continue;
-        }
-        int e1 = e0 + 1;  // entries [e0, e1) are this job's, or empty
-        while (e1 < 2 * kAtWarps && (keys[e1] < 0 || keys[e1] == job_u0)) ++e1;
+    float *const wt = reinterpret_cast<float *>(at_smem + S::qfrag);  // [row][16] weights of the entries
+    float2 *const fin = reinterpret_cast<float2 *>(wt + kAtRows * 16);  // [row] (maximum, sum or 1 / sum)
+    const int64_t key = lane < 2 * kAtWarps ? keys[lane] : -1;
+    auto entry = [&](int e) -> const float * {
+        return e & 1 ? reinterpret_cast<const float *>(at_smem + S::ring + (e >> 1) * S::kRing)
+                     : p.part + (size_t)2 * gridDim.x * kAtPart<D> + (size_t)(blockIdx.x * kAtWarps + (e >> 1)) * kAtPart<D>;
+    };
+    for (uint32_t left = __ballot_sync(0xffffffffu, key >= 0); left;) {
+        const int64_t job_u0 = __shfl_sync(0xffffffffu, key, __ffs(left) - 1);
+        const uint32_t mine = __ballot_sync(0xffffffffu, key == job_u0);
+        left &= ~mine;
         const int bb = find(job_u0);
         const SeqWork s = seq(bb);
         const uint32_t jn = s.tiles + 1, job = (uint32_t)(job_u0 - base[bb]) / jn;
@@ -638,44 +672,62 @@ __global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kerne
         const int64_t job_u1 = job_u0 + jn;
         const bool starts = b0 <= job_u0 + 1, whole = starts && b1 >= job_u1;
         float *slot = p.part + (size_t)(2 * blockIdx.x + (starts ? 1 : 0)) * kAtPart<D>;
+        auto row_at = [&](int r) {  // of out and lse
+            const int row = row0 + r, tk = row / heads;
+            return (int64_t)(s.q0 + tk) * p.a.q_heads + head * heads + row - tk * heads;
+        };
+        auto write_lse = [&](int r, float m, float l) {
+            if (r < nrows && p.a.lse) p.a.lse[row_at(r)] = l == 0.0f ? -INFINITY : (m + log2f(l)) / kLog2e;
+        };
+        // Warp r weighs row r's parts, a lane each. A part that saw nothing has maximum -inf, sum
+        // 0; a sum that is not 0 there is NaN and must show.
+        auto weigh = [&](float2 f, float m) { return f.x == -INFINITY ? 0.0f : ex2(f.x - m); };
+        auto share = [&](float2 f, float k) { return f.y * (f.x == -INFINITY && f.y != 0.0f ? 1.0f : k); };
+        {
+            const bool on = mine >> lane & 1;
+            const float2 f = on ? *reinterpret_cast<const float2 *>(entry(lane) + kAtRows * D + 2 * warp) : make_float2(-INFINITY, 0.0f);
+            float m = f.x;
+#pragma unroll
+            for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const float k = weigh(f, m);
+            float l = share(f, k);
+#pragma unroll
+            for (int o = 8; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+            if (lane < 16) wt[warp * 16 + lane] = k;
+            if (lane == 0) {
+                fin[warp] = make_float2(m, whole ? (l == 0.0f ? 0.0f : 1.0f / l) : l);
+                if (whole) write_lse(warp, m, l);
+            }
+        }
+        __syncthreads();
         for (int i = threadIdx.x; i < nrows * (D / 4); i += kAtThreads) {
             const int r = i / (D / 4), d = i % (D / 4) * 4;
-            auto entry = [&](int e) {
-                return e & 1 ? reinterpret_cast<const float *>(at_smem + S::ring + (e >> 1) * S::kRing)
-                             : p.part + (size_t)2 * gridDim.x * kAtPart<D> + (size_t)(blockIdx.x * kAtWarps + (e >> 1)) * kAtPart<D>;
-            };
-            float m = -INFINITY, l = 0.0f;
-            for (int e = e0; e < e1; ++e)
-                if (keys[e] >= 0) m = fmaxf(m, entry(e)[kAtRows * D + 2 * r]);
             float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (int e = e0; e < e1; ++e) {
-                if (keys[e] < 0) continue;
-                const float *en = entry(e);
-                const float2 f = *reinterpret_cast<const float2 *>(en + kAtRows * D + 2 * r);
-                const float4 x = *reinterpret_cast<const float4 *>(en + r * D + d);
-                const float k = f.x == -INFINITY ? 0.0f : ex2(f.x - m);
-                l += f.y * (f.x == -INFINITY && f.y != 0.0f ? 1.0f : k);
-                if (k != 0.0f) {
-                    sum.x = fmaf(k, x.x, sum.x), sum.y = fmaf(k, x.y, sum.y);
-                    sum.z = fmaf(k, x.z, sum.z), sum.w = fmaf(k, x.w, sum.w);
-                }
+#pragma unroll
+            for (int e = 0; e < 2 * kAtWarps; ++e) {
+                if (!(mine >> e & 1)) continue;
+                const float4 x = *reinterpret_cast<const float4 *>(entry(e) + r * D + d);
+                const float k = wt[r * 16 + e];
+                sum.x += k != 0.0f ? k * x.x : 0.0f, sum.y += k != 0.0f ? k * x.y : 0.0f;
+                sum.z += k != 0.0f ? k * x.z : 0.0f, sum.w += k != 0.0f ? k * x.w : 0.0f;
             }
-            if (!whole) {
+            if (whole) {
+                const float inv = fin[r].y;
+                store4(out + row_at(r) * D + d, sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+            } else {
                 __stcg(reinterpret_cast<float4 *>(slot + r * D + d), sum);
-                if (d == 0) __stcg(reinterpret_cast<float2 *>(slot + kAtRows * D + 2 * r), make_float2(m, l));
-                continue;
+                if (d == 0) __stcg(reinterpret_cast<float2 *>(slot + kAtRows * D + 2 * r), fin[r]);
             }
-            const int row = row0 + r, tk = row / heads;
-            const int64_t at = (int64_t)(s.q0 + tk) * p.a.q_heads + head * heads + row - tk * heads;
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            store4(out + at * D + d, sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
-            if (d == 0 && p.a.lse) p.a.lse[at] = l == 0.0f ? -INFINITY : (m + log2f(l)) / kLog2e;
         }
-        e0 = e1;
-        if (whole) continue;
+        if (whole) {
+            __syncthreads();
+            continue;
+        }
 
-        // ---- cut over blocks: the last to arrive joins (unit x is in block (x B + B - 1) / U) ----
-        const int first = (int)(((job_u0 + 2) * blocks - 1) / units), last = (int)((job_u1 * blocks - 1) / units);
+        // ---- cut over blocks: the last to arrive joins. Unit x is the run of worker i, the last
+        // with cut(i) <= x, that is i U < (x + 1) W ----
+        auto owner = [&](int64_t x) { return (int)(((x + 1) * workers - 1) / units) / kAtWarps; };
+        const int first = owner(job_u0 + 1), last = owner(job_u1 - 1), parts = last - first + 1;
         __threadfence();
         __syncthreads();
         if (threadIdx.x == 0) misc[1] = (int)atomicAdd(p.arrived + first, 1u) == last - first;
@@ -684,50 +736,52 @@ __global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kerne
         __threadfence();
         if (threadIdx.x == 0) p.arrived[first] = 0;
         // the first block's part is in its slot 1, the others' in their slot 0
-        auto slot_of = [&](int i) { return p.part + (size_t)(2 * i + (i == first ? 1 : 0)) * kAtPart<D>; };
-        const int parts = last - first + 1;
-        float2 *fin = reinterpret_cast<float2 *>(at_smem + S::qfrag);  // [row] (maximum, 1 / sum)
-        float4 *red = reinterpret_cast<float4 *>(at_smem + S::qfrag + 128);
-        __syncthreads();
-        {  // a warp per row, a lane per part
-            const int r = warp;
+        auto slot_of = [&](int i) { return p.part + (size_t)(2 * (first + i) + (i == 0 ? 1 : 0)) * kAtPart<D>; };
+        {
+            constexpr int kOf = (2 * 148 + 31) / 32;  // parts of a lane, read at once
+            float2 f[kOf];
             float m = -INFINITY, l = 0.0f;
-            for (int i = lane; i < parts; i += 32) m = fmaxf(m, __ldcg(slot_of(first + i) + kAtRows * D + 2 * r));
+#pragma unroll
+            for (int i = 0; i < kOf; ++i)
+                f[i] = i * 32 + lane < parts ? __ldcg(reinterpret_cast<const float2 *>(slot_of(i * 32 + lane) + kAtRows * D) + warp)
+                                             : make_float2(-INFINITY, 0.0f);
+            for (int i = kOf * 32 + lane; i < parts; i += 32)  // (a larger device)
+                m = fmaxf(m, __ldcg(slot_of(i) + kAtRows * D + 2 * warp));
+#pragma unroll
+            for (int i = 0; i < kOf; ++i) m = fmaxf(m, f[i].x);
 #pragma unroll
             for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            for (int i = lane; i < parts; i += 32) {
-                const float2 f = __ldcg(reinterpret_cast<const float2 *>(slot_of(first + i) + kAtRows * D) + r);
-                l += f.y * (f.x == -INFINITY ? (f.y != 0.0f ? 1.0f : 0.0f) : ex2(f.x - m));
+#pragma unroll
+            for (int i = 0; i < kOf; ++i) l += share(f[i], weigh(f[i], m));
+            for (int i = kOf * 32 + lane; i < parts; i += 32) {
+                const float2 x = __ldcg(reinterpret_cast<const float2 *>(slot_of(i) + kAtRows * D) + warp);
+                l += share(x, weigh(x, m));
             }
 #pragma unroll
             for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
             if (lane == 0) {
-                fin[r] = make_float2(m, l == 0.0f ? 0.0f : 1.0f / l);
-                if (r < nrows && p.a.lse) {
-                    const int row = row0 + r, tk = row / heads;
-                    p.a.lse[(int64_t)(s.q0 + tk) * p.a.q_heads + head * heads + row - tk * heads] =
-                        l == 0.0f ? -INFINITY : (m + log2f(l)) / kLog2e;
-                }
+                fin[warp] = make_float2(m, l == 0.0f ? 0.0f : 1.0f / l);
+                write_lse(warp, m, l);
             }
         }
         __syncthreads();
         // threads: (a share of the parts, if there are threads to spare) x (row, 4 dimensions)
         const int items = nrows * (D / 4), groups = max(1, kAtThreads / items);
+        float4 *red = reinterpret_cast<float4 *>(at_smem + S::qfrag + 1024);
         for (int i0 = 0; i0 < items; i0 += kAtThreads) {
             const int gi = threadIdx.x / items, i = groups > 1 ? threadIdx.x % items : i0 + threadIdx.x;
             const bool on = i < items && gi < groups;
             float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             const int r = i / (D / 4), d = i % (D / 4) * 4;
             if (on) {
+                const float m = fin[r].x;
 #pragma unroll 8
                 for (int k = groups > 1 ? gi : 0; k < parts; k += groups) {
-                    const float4 x = __ldcg(reinterpret_cast<const float4 *>(slot_of(first + k) + r * D + d));
-                    const float pm = __ldcg(slot_of(first + k) + kAtRows * D + 2 * r);
-                    const float w = pm == -INFINITY ? 0.0f : ex2(pm - fin[r].x);
-                    if (w != 0.0f) {
-                        sum.x = fmaf(w, x.x, sum.x), sum.y = fmaf(w, x.y, sum.y);
-                        sum.z = fmaf(w, x.z, sum.z), sum.w = fmaf(w, x.w, sum.w);
-                    }
+                    const float4 x = __ldcg(reinterpret_cast<const float4 *>(slot_of(k) + r * D + d));
+                    const float pm = __ldcg(slot_of(k) + kAtRows * D + 2 * r);
+                    const float w = pm == -INFINITY ? 0.0f : ex2(pm - m);
+                    sum.x += w != 0.0f ? w * x.x : 0.0f, sum.y += w != 0.0f ? w * x.y : 0.0f;
+                    sum.z += w != 0.0f ? w * x.z : 0.0f, sum.w += w != 0.0f ? w * x.w : 0.0f;
                 }
             }
             if (groups > 1) {
@@ -741,9 +795,7 @@ __global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kerne
             }
             if (on && gi == 0) {
                 const float inv = fin[r].y;
-                const int row = row0 + r, tk = row / heads;
-                store4(out + ((int64_t)(s.q0 + tk) * p.a.q_heads + head * heads + row - tk * heads) * D + d, sum.x * inv,
-                       sum.y * inv, sum.z * inv, sum.w * inv);
+                store4(out + row_at(r) * D + d, sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
             }
         }
         __syncthreads();
