@@ -18,6 +18,11 @@
 //    their group's range; so the sum is taken as sum w (c' - 7.5) + sum p (low' + 7.5 scale'),
 //    sum w by one more product with ones: the loss is then 2^-12 of |value - middle|.
 //    Statistics, sums and accumulators are fp32;
+//  - scores are taken relative to the maximum met before, and only where one exceeds it by more
+//    than 2^8 (or value scales outgrow their bound) are maxima exchanged and sums rescaled: p
+//    stays below 2^8, w below 2^15;
+//  - a value factor that is not finite is left out of the products and makes the rows that see
+//    the token NaN (0 times it would reach the rows that do not);
 //  - each warp streams tiles of kAtTile tokens through a private ring of bulk copies and keeps its
 //    own running maximum and sum: warps wait for one another only where they share a job;
 //  - the work, (sequence, key head, row tile) jobs of token tiles plus one unit for a job's own
@@ -35,7 +40,11 @@
 
 namespace cora {
 
-constexpr int kAtWarps = 8, kAtThreads = kAtWarps * 32, kAtTile = 32, kAtStages = 2;
+// One block per SM, of as many warps as leave a thread the registers it needs: spilled variables
+// would go past the little L1 that the ring leaves (they cost 10 of 40 us at 131072 tokens).
+constexpr int at_warps(int D) { return D == 256 ? 8 : 12; }
+constexpr int at_stages(int D) { return D == 256 ? 2 : 3; }  // tiles of a warp's ring
+constexpr int kAtTile = 32;
 constexpr int kAtRows = 8;         // query rows of a job
 constexpr int kAtMinRun = 2;       // units of a warp, at least
 constexpr int kAtShort = 40;       // tiles of a job that one block takes whole
@@ -58,6 +67,7 @@ constexpr int kAtPart = kAtRows * (D + 2);
 // The shared memory of a block, in order (each part a multiple of 16 bytes).
 template <int D, int kNG>
 struct AttendSmem {
+    static constexpr int kAtWarps = at_warps(D), kAtStages = at_stages(D);
     static constexpr uint32_t kCodes = kAtTile * D / 2, kMeta = kAtTile * kNG * 4;
     static constexpr uint32_t kStage = 2 * kCodes + 2 * kMeta;
     static constexpr uint32_t kRing = kAtStages * kStage;   // of a warp; at the end its partial result
@@ -65,7 +75,8 @@ struct AttendSmem {
     static constexpr uint32_t ring = 0;
     static constexpr uint32_t qfrag = ring + kAtWarps * kRing;       // [warp][D / 32][32] x 16 bytes
     static constexpr uint32_t keys = qfrag + kAtWarps * (D / 32) * 512;  // [2 warps] job of each partial result
-    static constexpr uint32_t misc = keys + kAtWarps * 2 * 8;
+    static constexpr uint32_t info = keys + kAtWarps * 2 * 8;            // [2 warps] int4: q0, head, row0 << 4 | rows, units
+    static constexpr uint32_t misc = info + kAtWarps * 2 * 16;
     static constexpr uint32_t bars = misc + 32;
     static constexpr uint32_t work = bars + kAtWarps * kAtStages * 8;    // int4[seqs], int64[seqs + 1]
     static constexpr size_t bytes(uint32_t seqs) { return work + 24 * (size_t)seqs + 8; }
@@ -128,8 +139,9 @@ __device__ __forceinline__ SeqWork seq_work(const AttendParams &p, int b, int ro
 }
 
 template <typename T, int D, int kNG>
-__global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kernel(const AttendParams p) {
+__global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const AttendParams p) {
     using S = AttendSmem<D, kNG>;
+    constexpr int kAtWarps = at_warps(D), kAtThreads = kAtWarps * 32, kAtStages = at_stages(D);
     constexpr int kG = D / kNG, kWords = kG / 32;  // words of one lane and group
     constexpr int kVB = D / 64;                    // 64-dimension blocks of the values
     extern __shared__ __align__(128) unsigned char at_smem[];
@@ -137,6 +149,7 @@ __global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kerne
     unsigned char *ring = at_smem + S::ring + warp * S::kRing;
     uint4 *qfrag = reinterpret_cast<uint4 *>(at_smem + S::qfrag) + warp * (D / 32) * 32;
     int64_t *keys = reinterpret_cast<int64_t *>(at_smem + S::keys);
+    int4 *info = reinterpret_cast<int4 *>(at_smem + S::info);
     volatile int *misc = reinterpret_cast<volatile int *>(at_smem + S::misc);
     uint64_t *bars = reinterpret_cast<uint64_t *>(at_smem + S::bars) + warp * kAtStages;
     int4 *work = reinterpret_cast<int4 *>(at_smem + S::work);
@@ -208,7 +221,7 @@ __global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kerne
     const uint32_t workers = blocks * kAtWarps;
     const int64_t each = units >> 32 ? units / workers : (uint32_t)units / workers;
     const uint32_t more = (uint32_t)(units - each * workers);
-    auto even = [&](uint32_t i) { return each * i + more * i / workers; };  // more i < 2368^2
+    auto even = [&](uint32_t i) { return each * i + more * i / workers; };  // more i < 2^32
     int64_t b0 = 0, b1 = 0;  // this block's units
     if (aligned) {  // one job per block: the block's number counts jobs
         int64_t job = blockIdx.x;
@@ -238,12 +251,13 @@ __global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kerne
     const uint32_t dst_at = (kind & 1 ? (kind < 2 ? S::kCodes : S::kMeta) : 0) + (kind < 2 ? 0 : 2 * S::kCodes) +
                             piece * per * rowb;
     int64_t ahead = u0;                                // the unit that the next tile to fetch is
-    int fb = -1, ftile = 0, frt = 0, fhead = 0, fpage = 0;
+    int fb = -1, ftile = 0, frt = 0, fhead = 0;
     SeqWork fs{};
     const int *ftable = nullptr;
-    auto fetch_page = [&]() {  // its page's number, early: the copy needs it one tile later
-        const int tok = fs.first + ftile * kAtTile + piece * per;
-        fpage = piece * per < kAtTile && tok < fs.len ? __ldg(ftable + (tok >> shift)) : -2;
+    int pages = 0, pbase = 0;  // lane i holds the number of the sequence's page pbase + i
+    auto load_pages = [&](int first) {
+        pbase = first;
+        pages = (first + lane) << shift < fs.len ? __ldg(ftable + first + lane) : -1;
     };
     auto fetch_q = [&]() {  // the job's queries, into L2 ahead of the copies that crowd the memory
         constexpr int kLines = D / 64;  // 128-byte lines of a row
@@ -253,48 +267,45 @@ __global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kerne
                                                           (int64_t)(fhead * heads + row - tk * heads) * p.a.q_head +
                                                           lane % kLines * 64));
     };
-    auto fetch_seek = [&]() {  // to unit `ahead`, or past it where that is a job's first (no tile)
-        if (ahead >= u1) return;
-        fb = find(ahead);
-        fs = seq(fb);
-        ftable = p.a.page_table + (int64_t)(p.seq0 + fb) * p.a.table_stride;
-        const uint32_t r = (uint32_t)(ahead - base[fb]), n = fs.tiles + 1, job = r / n;
-        ftile = (int)(r - job * n) - 1;
-        fhead = (int)(job / fs.row_tiles);
-        frt = (int)(job - fhead * fs.row_tiles);
-        if (ftile < 0) ++ahead, ftile = 0;
-        if (ahead < u1) {
-            fetch_page();
-            fetch_q();
-        }
-    };
+    // Copies the tile that is next (if there is one yet) and moves on to the one after.
     auto fetch = [&](int stage) {
-        const bool got = fpage != -2, ok = got && fpage >= 0 && (uint32_t)fpage < p.c.num_pages;
-        const uint32_t lanes = __ballot_sync(0xffffffffu, ok);
-        if (got && !ok) atomicOr(p.c.status, kDevBadInput);
-        // sections of a piece are copied by four neighbouring lanes, all or none
-        if (lane == 0) mbar_arrive_expect_tx(bars + stage, __popc(lanes) / 4 * per * (D + 8 * kNG));
-        __syncwarp();
-        if (ok) {
+        if (fb >= 0) {
             const int tok = fs.first + ftile * kAtTile + piece * per;
-            bulk_g2s(ring + stage * S::kStage + dst_at,
-                     p.c.pool + ((uint64_t)fpage * H + fhead) * blk.bytes + src_at + (uint32_t)(tok & (P - 1)) * rowb,
-                     per * rowb, bars + stage);
+            if (((fs.first + ftile * kAtTile + kAtTile - 1) >> shift) - pbase >= 32) load_pages((fs.first + ftile * kAtTile) >> shift);
+            const int page = __shfl_sync(0xffffffffu, pages, (tok >> shift) - pbase);
+            const bool got = piece * per < kAtTile && tok < fs.len, ok = got && page >= 0 && (uint32_t)page < p.c.num_pages;
+            const uint32_t lanes = __ballot_sync(0xffffffffu, ok);
+            if (got && !ok) atomicOr(p.c.status, kDevBadInput);
+            // sections of a piece are copied by four neighbouring lanes, all or none
+            if (lane == 0) mbar_arrive_expect_tx(bars + stage, __popc(lanes) / 4 * per * (D + 8 * kNG));
+            __syncwarp();
+            if (ok)
+                bulk_g2s(ring + stage * S::kStage + dst_at,
+                         p.c.pool + ((uint64_t)page * H + fhead) * blk.bytes + src_at + (uint32_t)(tok & (P - 1)) * rowb,
+                         per * rowb, bars + stage);
+            ++ahead, ++ftile;
         }
-        if (++ahead >= u1) return;
-        if (++ftile < fs.tiles) return fetch_page();
-        if (ahead >= base[fb + 1]) return fetch_seek();
-        ++ahead, ftile = 0;  // the next job's own unit
-        if (++frt == fs.row_tiles) frt = 0, ++fhead;
-        if (ahead < u1) {
-            fetch_page();
+        if (ahead >= u1) return;
+        if (fb < 0 || ftile == fs.tiles) {  // another job
+            if (fb < 0 || ahead >= base[fb + 1]) {  // of another sequence
+                fb = find(ahead);
+                fs = seq(fb);
+                ftable = p.a.page_table + (int64_t)(p.seq0 + fb) * p.a.table_stride;
+                const uint32_t r = (uint32_t)(ahead - base[fb]), n = fs.tiles + 1, job = r / n;
+                ftile = (int)(r - job * n) - 1;
+                fhead = (int)(job / fs.row_tiles);
+                frt = (int)(job - fhead * fs.row_tiles);
+            } else {
+                ftile = -1;
+                if (++frt == fs.row_tiles) frt = 0, ++fhead;
+            }
+            if (ftile < 0) ++ahead, ftile = 0;  // past the job's own unit
+            if (ahead >= u1) return;
+            load_pages((fs.first + ftile * kAtTile) >> shift);
             fetch_q();
         }
     };
-    int fstage = 0, pending = 0;  // tiles in flight
-    fetch_seek();
-    for (; pending < kAtStages && ahead < u1; ++pending) fetch(pending);
-    int stage = 0;
+    int fstage = 0, stage = 0, pending = 0;  // next stage to fill, to read; tiles in flight
     uint32_t phase = 0;
     bool alive = true;
 
@@ -303,31 +314,40 @@ __global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kerne
 
     T *const out = static_cast<T *>(p.a.out);
     const bool q_vec = reinterpret_cast<uintptr_t>(p.a.q) % 8 == 0 && p.a.q_token % 4 == 0 && p.a.q_head % 4 == 0;
-    float acc[kVB][4][4], mx[2], ls[2];
-    int b = -1;
+    float acc[kVB][4][4], om[2][kNG], ws[kNG][4];  // sum w c'; sum p (low' + 7.5 scale'); sum w (rows alike)
+    float mx[2], ref[2], over[2], ls[2];           // per row: maximum, what scores are relative to, how far
+                                                   // they may exceed it, sum of p
+    float qs[2][kNG], raw = 0.0f;                  // sums of q; the unit of q . c
+    int2 lm[2];                                    // tokens that rows 2 t and 2 t + 1 see
+    int lo_max = 0, hi_min = 0;
+    int vexp = 0;                                  // 2^-vexp bounds the value scales met
+    float vbound = 0.0f, vmul = 0.0f;              // w = p scale' vmul = p scale' 2^(7 + vexp)
+    int b = -1, head = 0, row0 = 0, nrows = 0, tile = 0, tile_end = 0;
+    int64_t u = u0, seg_end = 0, job_u0 = 0, job_u1 = 0;
     SeqWork sw{};
-    for (int64_t u = u0; u < u1;) {
-        // ---- one job: tiles [tile0, tile1) of it are this warp's ----
-        if (b < 0 || u >= base[b + 1]) {
-            b = find(u);
-            sw = seq(b);
+    const int tg = g ^ ((g >> 1) & 1);  // the token of operand row g (and + 8): see the values below
+
+    constexpr int kLoads = kAtRows * D / 4 / 32;
+    T qv[kLoads][4];
+    for (bool fresh = true;;) {
+        if (fresh) {
+        // ---- the next job: tiles [tile, tile_end) of it are this warp's ----
+        for (tile = 0, tile_end = 0; u < u1 && tile_end <= tile; u = tile_end <= tile ? seg_end : u) {
+            if (b < 0 || u >= base[b + 1]) {
+                b = find(u);
+                sw = seq(b);
+            }
+            const uint32_t jr = (uint32_t)(u - base[b]), jn = sw.tiles + 1, job = jr / jn;
+            job_u0 = base[b] + (int64_t)job * jn, job_u1 = job_u0 + jn;
+            seg_end = min(u1, job_u1);
+            head = (int)(job / sw.row_tiles);
+            row0 = (int)(job - head * sw.row_tiles) * kAtRows;
+            nrows = min(kAtRows, sw.n * heads - row0);
+            tile = max(0, (int)(u - job_u0) - 1);
+            tile_end = (int)(seg_end - job_u0) - 1;  // (none: only the job's own unit)
         }
-        const uint32_t jr = (uint32_t)(u - base[b]), jn = sw.tiles + 1, job = jr / jn;
-        const int64_t job_u0 = base[b] + (int64_t)job * jn, job_u1 = job_u0 + jn;
-        const int64_t seg_end = min(u1, job_u1);
-        const int head = (int)(job / sw.row_tiles), rt = (int)(job - head * sw.row_tiles);
-        const int row0 = rt * kAtRows, nrows = min(kAtRows, sw.n * heads - row0);
-        int tile = max(0, (int)(u - job_u0) - 1);
-        const int tile_end = (int)(seg_end - job_u0) - 1;
-        if (tile_end <= tile) {  // only the job's own unit
-            u = seg_end;
-            continue;
-        }
-        // queries: rows are (token, head of the group); fp16 under a common power of two. A lane
-        // loads 4 dimensions of a row at a time.
-        constexpr int kLoads = kAtRows * D / 4 / 32;
-        T qv[kLoads][4];
-        float big = 0.0f;
+        if (u >= u1) break;
+        // its queries, 4 dimensions of a row a lane and load, ahead of the copies
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int r = (i * 32 + lane) / (D / 4), d = (i * 32 + lane) % (D / 4) * 4;
@@ -341,6 +361,19 @@ __global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kerne
                 for (int e = 0; e < 4; ++e) qv[i][e] = src[e];
             }
         }
+        }
+        while (pending < kAtStages && ahead < u1 && alive) {
+            const bool copies = fb >= 0;
+            fetch(fstage);
+            if (copies) {
+                ++pending;
+                fstage = fstage + 1 == kAtStages ? 0 : fstage + 1;
+            }
+        }
+        if (fresh) {
+        fresh = false;
+        // queries: rows are (token, head of the group); fp16 under a common power of two
+        float big = 0.0f;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i)
 #pragma unroll
@@ -352,7 +385,7 @@ __global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kerne
         // 2^qe brings the largest |q| into [2^13, 2^14)
         const int qe = big > 0.0f ? max(-100, min(126, 13 - ilogbf(big))) : 0;
         const float qpow = ldexpf(1.0f, qe), qf = p.a.scale * kLog2e;
-        const float raw = ldexpf(qf, 24 - qe);  // of q . c as the tensor core sums it
+        raw = ldexpf(qf, 24 - qe);  // of q . c as the tensor core sums it
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
@@ -373,7 +406,7 @@ __global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kerne
             reinterpret_cast<uint2 *>(qfrag + (gr * kWords + j) * 32 + r * 4 + tt)[lane & 1] = w;
         }
         __syncwarp();
-        float qs[2][kNG];  // sums of q per group, by the same operands against ones (and 16s)
+        // sums of q per group, by the same operands against ones (and 16s)
 #pragma unroll
         for (int gr = 0; gr < kNG; ++gr) {
             float d[4] = {};
@@ -387,46 +420,38 @@ __global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kerne
             const float f = ldexpf(qf, -qe);
             qs[0][gr] = d[0] * f, qs[1][gr] = d[1] * f;
         }
-        int2 lm[2];  // tokens that rows 2 t and 2 t + 1 see
-        int lo_max = 0, hi_min = 0x7fffffff;
+        lo_max = 0, hi_min = 0x7fffffff;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             const int r = 2 * t + c, pos = sw.len - sw.n + (row0 + r) / heads;
             lm[c].y = p.a.causal ? max(0, min(sw.len, pos + 1)) : sw.len;
             lm[c].x = p.a.window ? max(0, pos - (int)p.a.window + 1) : 0;
             if (r < nrows) lo_max = max(lo_max, lm[c].x), hi_min = min(hi_min, lm[c].y);
+            mx[c] = over[c] = -INFINITY;
+            ref[c] = ls[c] = 0.0f;
+#pragma unroll
+            for (int gr = 0; gr < kNG; ++gr) om[c][gr] = ws[gr][c] = ws[gr][c + 2] = 0.0f;
         }
         lo_max = __reduce_max_sync(0xffffffffu, lo_max);
         hi_min = __reduce_min_sync(0xffffffffu, hi_min);
-
-        float om[2][kNG], ws[kNG][4];  // sum p (low' + 7.5 scale'); sum w (rows of the accumulator are alike)
 #pragma unroll
         for (int v = 0; v < kVB; ++v)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) acc[v][i][c] = 0.0f;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            mx[c] = -INFINITY;
-            ls[c] = 0.0f;
-#pragma unroll
-            for (int gr = 0; gr < kNG; ++gr) om[c][gr] = ws[gr][c] = ws[gr][c + 2] = 0.0f;
+        vexp = 119, vbound = vmul = 0.0f;
         }
-        int vexp = 126;  // 2^-vexp bounds the value scales met: operands are p scale' 2^(15 + vexp)
-        float vbound = 0.0f, vmul = 0.0f;
 
-        for (; tile < tile_end; ++tile) {
+        {
+            // ---- a tile: scores of two times 16 tokens x 8 rows ----
             const int tok0 = sw.first + tile * kAtTile;
             if (pending) {  // (0 only after a wait ran out: nothing more is fetched then)
                 alive = __all_sync(0xffffffffu, mbar_wait_bounded(bars + stage, phase, p.c.status)) && alive;
                 --pending;
             }
             const unsigned char *st = ring + stage * S::kStage;
-            const bool edge = tok0 + kAtTile > hi_min || tok0 < lo_max;
-            // ---- scores: two tiles of 16 tokens x 8 rows ----
             float s[2][4];
-            const int tg = g ^ ((g >> 1) & 1);  // the token of operand row g (and + 8): see below
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
@@ -455,84 +480,92 @@ __global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kerne
                     const float2 f1 = __half22float2(km[(mt * 16 + 8 + tg) * kNG + gr]);
                     const float r0 = f0.x * raw, r1 = f1.x * raw;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const float low = (c < 2 ? f0.y : f1.y) * qs[c & 1][gr];
-                        const float v = fmaf(c < 2 ? r0 : r1, d[c], low);
-                        s[mt][c] = gr ? s[mt][c] + v : v;
-                    }
+                    for (int c = 0; c < 4; ++c)
+                        s[mt][c] = fmaf(c < 2 ? r0 : r1, d[c], fmaf(c < 2 ? f0.y : f1.y, qs[c & 1][gr], gr ? s[mt][c] : -ref[c & 1]));
                 }
             }
-            uint32_t hidden = 0;  // bit 4 mt + c
-            if (edge) {
-#pragma unroll
-                for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const int tok = tok0 + mt * 16 + tg + (c >> 1) * 8;
-                        if (tok < lm[c & 1].x || tok >= lm[c & 1].y) {
-                            s[mt][c] = -INFINITY;
-                            hidden |= 1u << (mt * 4 + c);
-                        }
-                    }
-            }
-            // ---- running maximum ----
-            float al[2];
-            bool moved = false;
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                float m = fmaxf(fmaxf(s[0][c], s[0][c + 2]), fmaxf(s[1][c], s[1][c + 2]));
-                m = fmaxf(mx[c], max_over_g(m));
-                const float ref = m == -INFINITY ? 0.0f : m;
-                al[c] = ex2(mx[c] - ref);
-                moved |= m != mx[c];
-                mx[c] = m;
-#pragma unroll
-                for (int mt = 0; mt < 2; ++mt) {
-                    s[mt][c] = ex2(s[mt][c] - ref);
-                    s[mt][c + 2] = ex2(s[mt][c + 2] - ref);
-                }
-            }
-            // ---- value factors; the bound on their scales ----
-            const __half2 *vm = reinterpret_cast<const __half2 *>(st + 2 * S::kCodes + S::kMeta);
-            float2 vf[2][2][kNG];
-            float smax = 0.0f;
+            const uint32_t *vm = reinterpret_cast<const uint32_t *>(st + 2 * S::kCodes + S::kMeta);
+            uint32_t vf[2][2][kNG];  // the tokens' value factors
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
                 for (int r = 0; r < 2; ++r)
 #pragma unroll
-                    for (int gr = 0; gr < kNG; ++gr) {
-                        const int tok = mt * 16 + tg + r * 8;
-                        float2 f = __half22float2(vm[tok * kNG + gr]);
-                        if (edge && tok0 + tok >= sw.len) f = make_float2(0.0f, 0.0f);
-                        smax = fmaxf(smax, f.x < 65536.0f ? f.x : 0.0f);
-                        f.y = fmaf(7.5f, f.x, f.y);
-                        vf[mt][r][gr] = f;
+                    for (int gr = 0; gr < kNG; ++gr) vf[mt][r][gr] = vm[(mt * 16 + tg + r * 8) * kNG + gr];
+            if (tok0 + kAtTile > hi_min || tok0 < lo_max) {  // some row does not see some token
+#pragma unroll
+                for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const int tok = tok0 + mt * 16 + tg + r * 8;
+#pragma unroll
+                        for (int c = 0; c < 2; ++c)
+                            if (tok < lm[c].x || tok >= lm[c].y) s[mt][2 * r + c] = -INFINITY;
+                        if (tok >= sw.len) {  // nobody does: the bytes may be anything
+#pragma unroll
+                            for (int gr = 0; gr < kNG; ++gr) vf[mt][r][gr] = 0;
+                        }
                     }
-            float shrink = 1.0f;
-            if (__any_sync(0xffffffffu, smax > vbound)) {
-                smax = max_over_g(smax);
-                const int e = -(ilogbf(smax) + 1);  // smax < 2^-e
-                shrink = vbound > 0.0f ? ldexpf(1.0f, e - vexp) : 1.0f;
-                vexp = e;
-                vbound = ldexpf(1.0f, -e);
-                vmul = ldexpf(1.0f, 15 + e);
-                moved = true;
             }
-            if (__any_sync(0xffffffffu, moved)) {
+            // ---- maxima, bound of the value scales: the rare way out of the tile's course ----
+            __half2 most = __half2half2(__ushort_as_half(0));
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+#pragma unroll
+                    for (int gr = 0; gr < kNG; ++gr) most = __hmax2_nan(most, __habs2(*reinterpret_cast<__half2 *>(&vf[mt][r][gr])));
+            const float2 mf = __half22float2(most);
+            bool out_of_course = !(mf.x <= vbound) || !(mf.y <= 65504.0f);
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+                out_of_course |= fmaxf(fmaxf(s[0][c], s[0][c + 2]), fmaxf(s[1][c], s[1][c + 2])) > over[c];
+            if (__any_sync(0xffffffffu, out_of_course)) {
+                float smax = 0.0f;
+#pragma unroll
+                for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+#pragma unroll
+                        for (int gr = 0; gr < kNG; ++gr) {
+                            const float2 f = __half22float2(*reinterpret_cast<__half2 *>(&vf[mt][r][gr]));
+                            if (fabsf(f.x) <= 65504.0f && fabsf(f.y) <= 65504.0f) {
+                                smax = fmaxf(smax, fabsf(f.x));
+                                continue;
+                            }
+                            vf[mt][r][gr] = 0;
+#pragma unroll
+                            for (int c = 0; c < 2; ++c)
+                                if (s[mt][2 * r + c] != -INFINITY) ls[c] = __int_as_float(0x7fc00000);
+                        }
+                smax = max_over_g(smax);
+                float shrink = 1.0f;
+                if (smax > vbound) {
+                    const int e = -(ilogbf(smax) + 1);  // smax < 2^-e
+                    if (vbound > 0.0f) shrink = ldexpf(1.0f, e - vexp);
+                    vexp = e;
+                    vbound = ldexpf(1.0f, -e);
+                    vmul = ldexpf(1.0f, 7 + e);
+                }
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    ls[c] *= al[c];
-                    const float f = al[c] * shrink;
+                    float m = fmaxf(fmaxf(s[0][c], s[0][c + 2]), fmaxf(s[1][c], s[1][c + 2]));
+                    m = max_over_g(m) + ref[c];
+                    const bool grew = m > mx[c] + (mx[c] == -INFINITY ? 0.0f : 8.0f);
+                    const float k = grew ? ex2(mx[c] - m) : 1.0f, f = k * shrink;
+                    if (grew) {
+                        const float shift = ref[c] - m;
+                        mx[c] = ref[c] = m, over[c] = 8.0f;
 #pragma unroll
-                    for (int gr = 0; gr < kNG; ++gr) om[c][gr] *= al[c], ws[gr][c] *= f;
+                        for (int mt = 0; mt < 2; ++mt) s[mt][c] += shift, s[mt][c + 2] += shift;
+                    }
+                    ls[c] *= k;
+#pragma unroll
+                    for (int gr = 0; gr < kNG; ++gr) om[c][gr] *= k, ws[gr][c] *= f;
 #pragma unroll
                     for (int v = 0; v < kVB; ++v)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            acc[v][i][c] *= f;
-                            acc[v][i][c + 2] *= f;
-                        }
+                        for (int i = 0; i < 4; ++i) acc[v][i][c] *= f, acc[v][i][c + 2] *= f;
                 }
             }
             // ---- values: per 16 tokens, p scale' transposed into the 16-deep operand ----
@@ -540,17 +573,22 @@ __global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kerne
             for (int mt = 0; mt < 2; ++mt) {
                 uint32_t pb[kNG][2];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) ls[c & 1] += s[mt][c];
+                for (int c = 0; c < 4; ++c) {
+                    s[mt][c] = ex2(s[mt][c]);
+                    ls[c & 1] += s[mt][c];
+                }
 #pragma unroll
                 for (int gr = 0; gr < kNG; ++gr) {
                     float x[4];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const float2 f = vf[mt][c >> 1][gr];
-                        x[c] = s[mt][c] * (f.x * vmul);
-                        float y = s[mt][c] * f.y;
-                        if (edge && (hidden >> (mt * 4 + c) & 1)) x[c] = y = 0.0f;
-                        om[c & 1][gr] += y;
+                    for (int r = 0; r < 2; ++r) {
+                        const float2 f = __half22float2(*reinterpret_cast<__half2 *>(&vf[mt][r][gr]));
+                        const float fw = f.x * vmul, fm = fmaf(7.5f, f.x, f.y);
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            x[2 * r + c] = s[mt][2 * r + c] * fw;
+                            om[c][gr] = fmaf(s[mt][2 * r + c], fm, om[c][gr]);
+                        }
                     }
                     pb[gr][0] = transpose8x8(pack_half2(x[0], x[1]));
                     pb[gr][1] = transpose8x8(pack_half2(x[2], x[3]));
@@ -578,22 +616,18 @@ __global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kerne
                                          y[i] & 0x00f000f0u, pb[gr][0], pb[gr][1]);
                 }
             }
-            // ---- the stage is read: refill it ----
-            __syncwarp();
-            if (ahead < u1 && alive) {
-                fetch(fstage);
-                ++pending;
-            }
-            if (++fstage == kAtStages) fstage = 0;
+            __syncwarp();  // the stage is read
             if (++stage == kAtStages) {
                 stage = 0;
                 phase ^= 1;
             }
         }
+        if (++tile < tile_end) continue;
         u = seg_end;
+        fresh = true;
 
         // ---- the warp's result of this job: acc becomes sum p v, ls the sum over its tokens ----
-        const float opow = ldexpf(1.0f, 9 - vexp);  // 2^24 of the codes, 2^-(15 + vexp) of the operand
+        const float opow = ldexpf(1.0f, 17 - vexp);  // 2^24 of the codes, 2^-(7 + vexp) of the operand
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             ls[c] = sum_over_g(ls[c]);
@@ -636,7 +670,10 @@ __global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kerne
         // Not whole: it waits for the other warps. The last job's part goes to shared memory (the
         // ring has run dry), an earlier one's (the run's first job) to the workspace.
         const bool last = u >= u1;
-        if (lane == 0) keys[2 * warp + (last ? 1 : 0)] = job_u0;
+        if (lane == 0) {
+            keys[2 * warp + (last ? 1 : 0)] = job_u0;
+            info[2 * warp + (last ? 1 : 0)] = make_int4(sw.q0, head, row0 << 4 | nrows, (int)(job_u1 - job_u0));
+        }
         float *dst = last ? reinterpret_cast<float *>(ring) : part_warp;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -651,94 +688,91 @@ __global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kerne
         }
     }
 
-    // ---- jobs cut over this block's warps: entries 2 w, 2 w + 1 are warp w's parts ----
+    // ---- jobs cut over this block's warps: entries 2 w, 2 w + 1 are warp w's parts. Warp r joins
+    // row r of each: a lane weighs an entry, then each takes 4 dimensions ----
     __syncthreads();
-    float *const wt = reinterpret_cast<float *>(at_smem + S::qfrag);  // [row][16] weights of the entries
-    float2 *const fin = reinterpret_cast<float2 *>(wt + kAtRows * 16);  // [row] (maximum, sum or 1 / sum)
     const int64_t key = lane < 2 * kAtWarps ? keys[lane] : -1;
-    auto entry = [&](int e) -> const float * {
-        return e & 1 ? reinterpret_cast<const float *>(at_smem + S::ring + (e >> 1) * S::kRing)
-                     : p.part + (size_t)2 * gridDim.x * kAtPart<D> + (size_t)(blockIdx.x * kAtWarps + (e >> 1)) * kAtPart<D>;
+    const float *entry = lane & 1 ? reinterpret_cast<const float *>(at_smem + S::ring + (lane >> 1) % kAtWarps * S::kRing)
+                                  : p.part + (size_t)2 * gridDim.x * kAtPart<D> +
+                                        (size_t)(blockIdx.x * kAtWarps + (lane >> 1) % kAtWarps) * kAtPart<D>;
+    // A part that saw nothing has maximum -inf and sum 0; a sum that is not 0 there is NaN and
+    // must show.
+    auto weigh = [&](float2 f, float m) { return f.x == -INFINITY ? 0.0f : ex2(f.x - m); };
+    auto share = [&](float2 f, float k) { return f.y * (f.x == -INFINITY && f.y != 0.0f ? 1.0f : k); };
+    int4 in{};  // of the job at hand
+    auto row_at = [&](int r) {  // of out and lse
+        const int row = (in.z >> 4) + r, tk = row / heads;
+        return (int64_t)(in.x + tk) * p.a.q_heads + in.y * heads + row - tk * heads;
     };
+    auto lse_of = [&](float m, float l) { return l == 0.0f ? -INFINITY : (m + log2f(l)) / kLog2e; };
+    uint32_t cut_jobs = 0;  // entries that begin jobs cut over blocks: at most two
     for (uint32_t left = __ballot_sync(0xffffffffu, key >= 0); left;) {
-        const int64_t job_u0 = __shfl_sync(0xffffffffu, key, __ffs(left) - 1);
+        const int e0 = __ffs(left) - 1;
+        job_u0 = __shfl_sync(0xffffffffu, key, e0);
         const uint32_t mine = __ballot_sync(0xffffffffu, key == job_u0);
         left &= ~mine;
-        const int bb = find(job_u0);
-        const SeqWork s = seq(bb);
-        const uint32_t jn = s.tiles + 1, job = (uint32_t)(job_u0 - base[bb]) / jn;
-        const int head = (int)(job / s.row_tiles), row0 = (int)(job - head * s.row_tiles) * kAtRows;
-        const int nrows = min(kAtRows, s.n * heads - row0);
-        const int64_t job_u1 = job_u0 + jn;
-        const bool starts = b0 <= job_u0 + 1, whole = starts && b1 >= job_u1;
+        in = info[e0];
+        const bool starts = b0 <= job_u0 + 1, whole = starts && b1 >= job_u0 + in.w;
+        if (!whole) cut_jobs |= 1u << e0;
+        if (warp >= (in.z & 15)) continue;
+        const float2 f = mine >> lane & 1 ? *reinterpret_cast<const float2 *>(entry + kAtRows * D + 2 * warp)
+                                          : make_float2(-INFINITY, 0.0f);
+        float m = f.x;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float k = weigh(f, m);
+        float l = share(f, k);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         float *slot = p.part + (size_t)(2 * blockIdx.x + (starts ? 1 : 0)) * kAtPart<D>;
-        auto row_at = [&](int r) {  // of out and lse
-            const int row = row0 + r, tk = row / heads;
-            return (int64_t)(s.q0 + tk) * p.a.q_heads + head * heads + row - tk * heads;
-        };
-        auto write_lse = [&](int r, float m, float l) {
-            if (r < nrows && p.a.lse) p.a.lse[row_at(r)] = l == 0.0f ? -INFINITY : (m + log2f(l)) / kLog2e;
-        };
-        // Warp r weighs row r's parts, a lane each. A part that saw nothing has maximum -inf, sum
-        // 0; a sum that is not 0 there is NaN and must show.
-        auto weigh = [&](float2 f, float m) { return f.x == -INFINITY ? 0.0f : ex2(f.x - m); };
-        auto share = [&](float2 f, float k) { return f.y * (f.x == -INFINITY && f.y != 0.0f ? 1.0f : k); };
-        {
-            const bool on = mine >> lane & 1;
-            const float2 f = on ? *reinterpret_cast<const float2 *>(entry(lane) + kAtRows * D + 2 * warp) : make_float2(-INFINITY, 0.0f);
-            float m = f.x;
-#pragma unroll
-            for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            const float k = weigh(f, m);
-            float l = share(f, k);
-#pragma unroll
-            for (int o = 8; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-            if (lane < 16) wt[warp * 16 + lane] = k;
-            if (lane == 0) {
-                fin[warp] = make_float2(m, whole ? (l == 0.0f ? 0.0f : 1.0f / l) : l);
-                if (whole) write_lse(warp, m, l);
-            }
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < nrows * (D / 4); i += kAtThreads) {
-            const int r = i / (D / 4), d = i % (D / 4) * 4;
+        const int64_t at = row_at(warp);
+#pragma unroll 1
+        for (int d = lane * 4; d < D + 127 - (D + 127) % 128; d += 128) {
             float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-            for (int e = 0; e < 2 * kAtWarps; ++e) {
-                if (!(mine >> e & 1)) continue;
-                const float4 x = *reinterpret_cast<const float4 *>(entry(e) + r * D + d);
-                const float k = wt[r * 16 + e];
-                sum.x += k != 0.0f ? k * x.x : 0.0f, sum.y += k != 0.0f ? k * x.y : 0.0f;
-                sum.z += k != 0.0f ? k * x.z : 0.0f, sum.w += k != 0.0f ? k * x.w : 0.0f;
+#pragma unroll 1
+            for (uint32_t rest = mine; rest; rest &= rest - 1) {
+                const int e = __ffs(rest) - 1;
+                const float *en = reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(entry), e));
+                const float w = __shfl_sync(0xffffffffu, k, e);
+                if (w != 0.0f && d < D) {
+                    const float4 x = *reinterpret_cast<const float4 *>(en + warp * D + d);
+                    sum.x = fmaf(w, x.x, sum.x), sum.y = fmaf(w, x.y, sum.y);
+                    sum.z = fmaf(w, x.z, sum.z), sum.w = fmaf(w, x.w, sum.w);
+                }
             }
-            if (whole) {
-                const float inv = fin[r].y;
-                store4(out + row_at(r) * D + d, sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
-            } else {
-                __stcg(reinterpret_cast<float4 *>(slot + r * D + d), sum);
-                if (d == 0) __stcg(reinterpret_cast<float2 *>(slot + kAtRows * D + 2 * r), fin[r]);
-            }
+            if (d >= D) continue;
+            if (whole) store4(out + at * D + d, sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+            else __stcg(reinterpret_cast<float4 *>(slot + warp * D + d), sum);
         }
-        if (whole) {
-            __syncthreads();
-            continue;
+        if (lane == 0) {
+            if (!whole) __stcg(reinterpret_cast<float2 *>(slot + kAtRows * D + 2 * warp), make_float2(m, l));
+            else if (p.a.lse) p.a.lse[at] = lse_of(m, l);
         }
-
+    }
+    if (!cut_jobs) return;
+    __threadfence();
+    __syncthreads();
+    float2 *const fin = reinterpret_cast<float2 *>(at_smem + S::qfrag);  // [row] (maximum, 1 / sum)
+    for (; cut_jobs; cut_jobs &= cut_jobs - 1) {
+        const int e0 = __ffs(cut_jobs) - 1;
+        job_u0 = keys[e0], in = info[e0];
+        const int nrows = in.z & 15;
         // ---- cut over blocks: the last to arrive joins. Unit x is the run of worker i, the last
         // with cut(i) <= x, that is i U < (x + 1) W ----
         auto owner = [&](int64_t x) { return (int)(((x + 1) * workers - 1) / units) / kAtWarps; };
-        const int first = owner(job_u0 + 1), last = owner(job_u1 - 1), parts = last - first + 1;
-        __threadfence();
-        __syncthreads();
+        const int first = owner(job_u0 + 1), last = owner(job_u0 + in.w - 1), parts = last - first + 1;
         if (threadIdx.x == 0) misc[1] = (int)atomicAdd(p.arrived + first, 1u) == last - first;
         __syncthreads();
-        if (!misc[1]) continue;
+        const bool joins = misc[1];
+        __syncthreads();  // (misc is free again)
+        if (!joins) continue;
         __threadfence();
         if (threadIdx.x == 0) p.arrived[first] = 0;
         // the first block's part is in its slot 1, the others' in their slot 0
         auto slot_of = [&](int i) { return p.part + (size_t)(2 * (first + i) + (i == 0 ? 1 : 0)) * kAtPart<D>; };
-        {
-            constexpr int kOf = (2 * 148 + 31) / 32;  // parts of a lane, read at once
+        if (warp < kAtRows) {
+            constexpr int kOf = (148 + 31) / 32;  // parts of a lane, read at once
             float2 f[kOf];
             float m = -INFINITY, l = 0.0f;
 #pragma unroll
@@ -761,7 +795,7 @@ __global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kerne
             for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
             if (lane == 0) {
                 fin[warp] = make_float2(m, l == 0.0f ? 0.0f : 1.0f / l);
-                write_lse(warp, m, l);
+                if (warp < nrows && p.a.lse) p.a.lse[row_at(warp)] = lse_of(m, l);
             }
         }
         __syncthreads();
@@ -775,7 +809,7 @@ __global__ void __launch_bounds__(kAtThreads, D <= 128 ? 2 : 1) kv4_attend_kerne
             const int r = i / (D / 4), d = i % (D / 4) * 4;
             if (on) {
                 const float m = fin[r].x;
-#pragma unroll 8
+#pragma unroll 4
                 for (int k = groups > 1 ? gi : 0; k < parts; k += groups) {
                     const float4 x = __ldcg(reinterpret_cast<const float4 *>(slot_of(k) + r * D + d));
                     const float pm = __ldcg(slot_of(k) + kAtRows * D + 2 * r);

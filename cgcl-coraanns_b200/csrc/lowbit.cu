@@ -118,8 +118,8 @@ uint64_t attend_counters() { return ((uint64_t)sm_count() * 2 * 4 + 255) / 256 *
 // partial results per block.
 uint64_t attend_workspace(const cora_kv4_cache &c, uint64_t rows) {
     const uint64_t blocks = sm_count();
-    // few rows: two parts of 8 rows per block and one per warp, two blocks per SM
-    const uint64_t parts = rows <= kFewRows ? (2 * blocks) * (2 + kAtWarps) * kAtRows
+    // few rows: two parts of 8 rows per block and one per warp
+    const uint64_t parts = rows <= kFewRows ? blocks * (2 + at_warps(c.head_dim)) * kAtRows
                                             : 2 * blocks * (rows <= 128 || c.head_dim == 256 ? 128 : 256);
     return attend_counters() + parts * (c.head_dim + 2) * 4;
 }
@@ -128,14 +128,14 @@ template <typename T, int D, int kNG>
 void launch_attend(AttendParams p, cudaStream_t st) {
     auto *kern = kv4_attend_kernel<T, D, kNG>;
     using S = AttendSmem<D, kNG>;
-    static_assert(S::bytes(kAtMaxSeqs) <= (D <= 128 ? 115 : 227) * 1024, "");
+    static_assert(S::bytes(kAtMaxSeqs) <= 232448, "");
     static int seen[64] = {};
     allow_smem(kern, S::bytes(kAtMaxSeqs), seen);
     const uint32_t seqs = p.a.seqs;
     for (uint32_t s0 = 0; s0 < seqs; s0 += kAtMaxSeqs) {
         p.seq0 = s0;
         p.seqs = std::min<uint32_t>(kAtMaxSeqs, seqs - s0);
-        kern<<<sm_count() * (D <= 128 ? 2 : 1), kAtThreads, S::bytes(p.seqs), st>>>(p);
+        kern<<<sm_count(), at_warps(D) * 32, S::bytes(p.seqs), st>>>(p);
         CUDA_TRY(cudaGetLastError());
     }
 }
