@@ -89,6 +89,22 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t *bar, uint32_t parity
         __nanosleep(64);
     }
 }
+// The same for waits that are short and often: no sleep between tries (try_wait itself suspends
+// the thread for a while), the clock read once in 64 tries.
+__device__ __forceinline__ bool mbar_wait_short(uint64_t *bar, uint32_t parity, int *err,
+                                                uint64_t limit_ns = 2000000000ull) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = global_ns();
+    while (true) {
+#pragma unroll 1
+        for (int i = 0; i < 64; ++i)
+            if (mbar_try_wait(bar, parity)) return true;
+        if (global_ns() - t0 > limit_ns) {
+            atomicOr(err, kDevWaitTimeout);
+            return false;
+        }
+    }
+}
 // 1-D bulk copy global -> shared; both addresses 16-byte aligned, bytes % 16 == 0.
 __device__ __forceinline__ void bulk_g2s(void *smem_dst, const void *gmem_src, uint32_t bytes,
                                          uint64_t *bar) {

@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const A
             // ---- a tile: scores of two times 16 tokens x 8 rows ----
             const int tok0 = sw.first + tile * kAtTile;
             if (pending) {  // (0 only after a wait ran out: nothing more is fetched then)
-                alive = __all_sync(0xffffffffu, mbar_wait_bounded(bars + stage, phase, p.c.status)) && alive;
+                alive = __all_sync(0xffffffffu, mbar_wait_short(bars + stage, phase, p.c.status)) && alive;
                 --pending;
             }
             const unsigned char *st = ring + stage * S::kStage;

@@ -5,9 +5,12 @@
 // memory. Rows (query token, head of the group) fill tiles of 128; one block takes kNQ = 2 tiles
 // (1 for few rows or head size 256) against the same keys, so each unpacked key tile serves 256
 // rows. Warp roles:
-//   0-3, 4-7  softmax of row tile 0 / 1: one thread per row; sums of q . c from TMEM, the
-//             token's factors from shared memory, running maximum and sum in fp32,
-//             probabilities back to TMEM as the fp16 operand of the second product. One pass:
+//   0-3, 4-7  softmax of row tile 0 / 1, 32 rows per warp: sums of q . c from TMEM, the token's
+//             factors from shared memory, running maximum and sum in fp32, probabilities back to
+//             TMEM as the fp16 operand of the second product. A thread holds 8 columns of 4 rows
+//             at a time (accumulator fragments), so that a factor it reads serves 4 rows: with a
+//             thread per row the factors alone took 2048 of 7200 cycles of shared memory a tile.
+//             One pass:
 //             probabilities refer to the maximum met before; only where it grows by more than
 //             2^8 are the sums (and the tile's earlier probabilities) rescaled, so that they
 //             stay below 2^8, which fp16 holds.
@@ -16,7 +19,7 @@
 //             one rounding each (2^-12 of the value, as of the probability; values past 65504
 //             do not fit).
 //   16        copies code tiles from the cache's pages (bulk copies into a ring).
-//   17        issues the tcgen05 products: S_g = Q_g C_g^T per factor group (keys K-major) and
+//   17        (18, 19 idle) issues the tcgen05 products: S_g = Q_g C_g^T per factor group (keys K-major) and
 //             O += P V (P in TMEM, values as stored, token-major: the N-major operand).
 // Units (sequence, key head, row tile, token tile) are cut into equal runs, one per block; a job
 // cut over blocks is joined by the last to arrive. Every wait is bounded.
@@ -29,7 +32,20 @@
 
 namespace cora {
 
-constexpr int kCkThreads = 576, kCkMinRun = 2;
+// Registers per thread: 640 x 96 at launch; then softmax 136, unpack 72, the last group 64
+// (256 x 136 + 256 x 72 + 128 x 64 = 61440). Spilled variables would go to L2: shared
+// memory leaves almost no L1.
+constexpr int kCkThreads = 640, kCkMinRun = 2;
+constexpr int kCkRegsSoftmax = 136, kCkRegsUnpack = 72, kCkRegsRest = 64;
+static_assert(256 * kCkRegsSoftmax + 256 * kCkRegsUnpack + 128 * kCkRegsRest <= kCkThreads * 96, "");
+template <int kRegs>
+__device__ __forceinline__ void more_registers() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+template <int kRegs>
+__device__ __forceinline__ void fewer_registers() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
 
 template <int D, int kNG, int kNQ>
 struct ChunkSmem {
@@ -42,11 +58,12 @@ struct ChunkSmem {
     static constexpr uint32_t q = 0;
     static constexpr uint32_t slot = q + kNQ * kQ;
     static constexpr uint32_t raw = slot + kSlots * kSlot;
-    static constexpr uint32_t fac = raw + kRaw * kRawBytes;         // [4][scale | low][kNG][kTN] of the keys
+    static constexpr uint32_t fac = raw + kRaw * kRawBytes;         // [4][kNG][kTN / 2] (two scales, two lows) of the keys
     static constexpr uint32_t poison = fac + 4 * 2 * kNG * kTN * 4; // [4][4] bits: token's value is not finite
     static constexpr uint32_t misc = poison + 64;                   // tmem slot, last-to-arrive flags
     static constexpr uint32_t bars = misc + 32;
-    static constexpr uint32_t base = bars + 256;                    // int64[seqs + 1]
+    static constexpr uint32_t walk = bars + 256;                    // [warp] WarpWalk
+    static constexpr uint32_t base = walk + 18 * 160;               // int64[seqs + 1]
     static constexpr size_t bytes(uint32_t seqs) { return 1024 + base + 8 * (size_t)(seqs + 1); }
 };
 
@@ -59,14 +76,15 @@ struct Segment {
     bool first, last;                // holds the job's first / last tile
 };
 
-// Walks the stretches of units [u, end); every role of a block sees the same ones.
+// Walks the stretches of units [u, end); every role of a block sees the same ones. One per warp,
+// in shared memory, moved by lane 0: its state would crowd out the registers of the tile loops.
 template <int kTN, int kRows>
 struct Walker {
-    const AttendParams &p;
-    const int64_t *base;
     int64_t u, end;
-    int b = -1;
-    SeqWork s{};
+    SeqWork s;
+    int b;
+    int more;   // whether g holds a stretch
+    Segment g;
     // tokens that row tile rt's queries see: [lo, hi)
     __device__ static int2 sees(const AttendParams &p, const SeqWork &s, int rt) {
         const int heads = p.a.q_heads / p.c.kv_heads;
@@ -82,7 +100,7 @@ struct Walker {
         for (int rt = 0; rt < s.row_tiles; ++rt) n += tiles(sees(p, s, rt));
         return n;
     }
-    __device__ bool next(Segment &g) {
+    __device__ bool next(const AttendParams &p, const int64_t *base) {
         if (u >= end) return false;
         if (b < 0 || u >= base[b + 1]) {
             int lo = 0, hi = (int)p.seqs - 1;
@@ -200,13 +218,24 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
     tc_fence_after();
     const uint32_t tmem = misc[0];
     const int64_t units = base[p.seqs], blocks = max((int64_t)1, min((int64_t)gridDim.x, units / kCkMinRun));
-    const int64_t u0 = blockIdx.x < blocks ? blockIdx.x * units / blocks : 0;
-    const int64_t u1 = blockIdx.x < blocks ? (blockIdx.x + 1) * units / blocks : 0;
-    Walk walk{p, base, u0, u1};
-    Segment g;
+    static_assert(sizeof(Walk) <= 160, "");
+    Walk &walk = *reinterpret_cast<Walk *>(sm + S::walk + (warp < 18 ? warp : 0) * 160);
+    const Segment &g = walk.g;
+    if (lane == 0 && warp < 18) {
+        walk.u = blockIdx.x < blocks ? blockIdx.x * units / blocks : 0;
+        walk.end = blockIdx.x < blocks ? (blockIdx.x + 1) * units / blocks : 0;
+        walk.b = -1;
+    }
+    auto next = [&]() {  // by a whole warp
+        __syncwarp();
+        if (lane == 0) walk.more = walk.next(p, base);
+        __syncwarp();
+        return walk.more != 0;
+    };
 
     if (warp < 4 * kNQ) {
         // ---------------- softmax: thread = row of tile q ----------------
+        more_registers<kCkRegsSoftmax>();
         const int q = warp / 4, row = (warp % 4) * 32 + lane;
         const uint32_t lanes = tmem + (uint32_t((warp % 4) * 32) << 16);
         const uint32_t t_o = lanes + kOCol + q * D;
@@ -217,170 +246,215 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
         T *out = static_cast<T *>(p.a.out);
         uint32_t tile_no = 0;  // tiles this thread has done (phases of the barriers)
         bool ok = true;
-        while (ok && walk.next(g)) {
+        while (ok && next()) {
             const int r = q * 128 + row, grow = g.row0 + r;
             const bool in = r < g.rows;
             const int i = in ? grow / heads : 0, hh = g.head * heads + (in ? grow % heads : 0);
             const T *src = static_cast<const T *>(p.a.q) + (int64_t)(g.s.q0 + i) * p.a.q_token + (int64_t)hh * p.a.q_head;
-            // the row under its own power of two, largest |q| in [2^13, 2^14)
-            float big = 0.0f;
-#pragma unroll 8
-            for (int d = 0; d < D; d += 8) {
-                float x[8] = {};
-                if (in) {
-                    if (vec) load8<T, true>(src + d, x);
-                    else load8<T, false>(src + d, x);
-                }
+            // the row under its own power of two, largest |q| in [2^13, 2^14); kBatch loads at once
+            constexpr int kBatch = 8;
+            auto load = [&](int d, uint4 (&w)[kBatch]) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) big = fabsf(x[e]) < 3.4e38f ? fmaxf(big, fabsf(x[e])) : big;
+                for (int e = 0; e < kBatch; ++e) {
+                    if (vec) {
+                        w[e] = __ldg(reinterpret_cast<const uint4 *>(src + d + e * 8));
+                    } else {
+                        const uint16_t *h = reinterpret_cast<const uint16_t *>(src + d + e * 8);
+                        w[e] = make_uint4(h[0] | uint32_t(h[1]) << 16, h[2] | uint32_t(h[3]) << 16, h[4] | uint32_t(h[5]) << 16,
+                                          h[6] | uint32_t(h[7]) << 16);
+                    }
+                }
+            };
+            float big = 0.0f;
+#pragma unroll 1
+            for (int d = 0; d < (in ? D : 0); d += kBatch * 8) {
+                uint4 w[kBatch];
+                load(d, w);
+#pragma unroll
+                for (int e = 0; e < kBatch * 8; ++e) {
+                    const float x = fabsf(to_f32(reinterpret_cast<const T *>(w)[e]));
+                    big = x < 3.4e38f ? fmaxf(big, x) : big;
+                }
             }
             const int qe = big > 0.0f ? max(-100, min(126, 13 - ilogbf(big))) : 0;
-            const float qpow = in ? ldexpf(sign, qe) : 0.0f;
+            const float qpow = in && f0 != 0.0f ? ldexpf(sign, qe) : 0.0f;
             float qs[kNG];  // sums of q per group, in the units of the products
 #pragma unroll
             for (int gr = 0; gr < kNG; ++gr) {
                 float sum = 0.0f;
-#pragma unroll 8
-                for (int d = gr * kG; d < (gr + 1) * kG; d += 8) {
-                    float x[8] = {};
-                    if (in) {
-                        if (vec) load8<T, true>(src + d, x);
-                        else load8<T, false>(src + d, x);
-                    }
+#pragma unroll 1
+                for (int d = gr * kG; d < (gr + 1) * kG; d += kBatch * 8) {
+                    uint4 w[kBatch];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        x[e] *= qpow;
-                        sum += x[e];
+                    for (int e = 0; e < kBatch; ++e) w[e] = make_uint4(0, 0, 0, 0);
+                    if (in) load(d, w);
+#pragma unroll
+                    for (int e = 0; e < kBatch; ++e) {
+                        float x[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            x[k] = to_f32(reinterpret_cast<const T *>(&w[e])[k]) * qpow;
+                            sum += x[k];
+                        }
+                        const float odd = 0.0625f;  // against the odd nibbles' 2^-20
+                        uint4 o;
+                        o.x = pack_half2(x[0], x[4]), o.y = pack_half2(x[1] * odd, x[5] * odd);
+                        o.z = pack_half2(x[2], x[6]), o.w = pack_half2(x[3] * odd, x[7] * odd);
+                        *reinterpret_cast<uint4 *>(sq + (d / 64) * kQBlock + row * 128 + ((e ^ (row & 7)) << 4)) = o;
                     }
-                    const float odd = 0.0625f;  // against the odd nibbles' 2^-20
-                    uint4 w;
-                    w.x = pack_half2(x[0], x[4]), w.y = pack_half2(x[1] * odd, x[5] * odd);
-                    w.z = pack_half2(x[2], x[6]), w.w = pack_half2(x[3] * odd, x[7] * odd);
-                    const int c = (d / 8) & 7;
-                    *reinterpret_cast<uint4 *>(sq + (d / 64) * kQBlock + row * 128 + ((c ^ (row & 7)) << 4)) = w;
                 }
                 qs[gr] = sum * 5.9604644775390625e-8f;  // 2^-24
             }
             fence_proxy_async_smem();
             mbar_arrive(q_full + q);
-            const float f = ldexpf(f0, 24 - qe);
-            const int pos = g.s.len - g.s.n + i;
-            const int hi = !in ? 0x7fffffff : p.a.causal ? max(0, min(g.s.len, pos + 1)) : g.s.len;
-            const int lo = in && p.a.window ? max(0, pos - (int)p.a.window + 1) : 0;
-            const int hi_min = __reduce_min_sync(0xffffffffu, hi), lo_max = __reduce_max_sync(0xffffffffu, lo);
-            float m = -INFINITY, l = 0.0f;
+            // From here a thread holds rows 8 k + lane / 4 of its warp, k = 0..3.
+            float fr[4], qr[4][kNG], m[4], over[4];  // unit of the scores; sums of q; maximum, room above it
+            int lo[4], hi[4];                        // tokens that the row sees
+            float2 l2[4];                            // sum of p, over even and odd columns
+            int hi_min = 0x7fffffff, lo_max = 0;
+            {
+                // scale 0: scores 0, whatever the products are
+                const float f = f0 == 0.0f ? 1.0f : ldexpf(f0, 24 - qe);
+                const int pos = g.s.len - g.s.n + i;
+                const int h1 = !in ? 0x7fffffff : p.a.causal ? max(0, min(g.s.len, pos + 1)) : g.s.len;
+                const int l1 = in && p.a.window ? max(0, pos - (int)p.a.window + 1) : 0;
+                hi_min = __reduce_min_sync(0xffffffffu, h1), lo_max = __reduce_max_sync(0xffffffffu, l1);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int from = 8 * k + lane / 4;
+                    fr[k] = __shfl_sync(0xffffffffu, f, from);
+                    lo[k] = __shfl_sync(0xffffffffu, l1, from);
+                    hi[k] = __shfl_sync(0xffffffffu, h1, from);
+#pragma unroll
+                    for (int gr = 0; gr < kNG; ++gr) qr[k][gr] = __shfl_sync(0xffffffffu, qs[gr], from);
+                    m[k] = over[k] = -INFINITY;
+                    l2[k] = make_float2(0.0f, 0.0f);
+                }
+            }
             for (int j = 0; j < g.tiles && ok; ++j, ++tile_no) {
                 const int buf = kNQ == 2 ? q : (int)(tile_no & 1);
                 const uint32_t sph = kNQ == 2 ? tile_no & 1 : (tile_no >> 1) & 1;
                 const uint32_t t_s = lanes + kSCol + buf * kSCols;
                 const int tok0 = g.tok0 + j * kTN;
                 const bool edge = tok0 + kTN > hi_min || tok0 < lo_max;
-                ok = __all_sync(0xffffffffu, mbar_wait_bounded(s_full + buf, sph, err));
+                ok = __all_sync(0xffffffffu, mbar_wait_short(s_full + buf, sph, err));
                 if (!ok) break;
                 tc_fence_after();
-                const float *tf = fac + (tile_no & 3) * 2 * kNG * kTN;
-                float2 ls = make_float2(0.0f, 0.0f);
+                const float4 *tf = reinterpret_cast<const float4 *>(fac + (tile_no & 3) * 2 * kNG * kTN) + lane % 4;
 #pragma unroll 1
                 for (int c = 0; c < kTN / 32; ++c) {
-                    // scores of 32 tokens, in units of 1 / f
-                    uint32_t x[32];
-                    float2 u[16];
-                    tmem_ld32_async(t_s + c * 32, x);
-                    tmem_wait_ld(x);
+                    // scores of 32 tokens x 32 rows: u[k][j] columns 8 j + 2 t, + 1 of row 8 k + g
+                    float2 u[4][4];
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) {
-                        const float4 s4 = *reinterpret_cast<const float4 *>(tf + c * 32 + e);
-                        const float4 l4 = *reinterpret_cast<const float4 *>(tf + kNG * kTN + c * 32 + e);
-                        const float2 qq = make_float2(qs[0], qs[0]);
-                        u[e / 2] = fma2(make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), make_float2(s4.x, s4.y),
-                                        mul2(make_float2(l4.x, l4.y), qq));
-                        u[e / 2 + 1] = fma2(make_float2(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])),
-                                            make_float2(s4.z, s4.w), mul2(make_float2(l4.z, l4.w), qq));
+                    for (int gr = 0; gr < kNG; ++gr) {
+                        uint32_t x[16], y[16];
+                        tmem_ld_frag(t_s + gr * kTN + c * 32, x);
+                        tmem_ld_frag(t_s + gr * kTN + c * 32 + (16u << 16), y);
+                        float4 ft[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) ft[j] = tf[gr * (kTN / 2) + c * 16 + j * 4];
+                        tmem_wait_frag(x, y);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const uint32_t *v = k < 2 ? x : y;
+                                const float2 d = make_float2(__uint_as_float(v[4 * j + (k & 1) * 2]), __uint_as_float(v[4 * j + (k & 1) * 2 + 1]));
+                                const float2 q2 = make_float2(qr[k][gr], qr[k][gr]), low = make_float2(ft[j].z, ft[j].w);
+                                u[k][j] = fma2(d, make_float2(ft[j].x, ft[j].y), gr ? fma2(low, q2, u[k][j]) : mul2(low, q2));
+                            }
                     }
-#pragma unroll
-                    for (int gr = 1; gr < kNG; ++gr) {
-                        tmem_ld32_async(t_s + gr * kTN + c * 32, x);
-                        tmem_wait_ld(x);
-#pragma unroll
-                        for (int e = 0; e < 32; e += 4) {
-                            const float4 s4 = *reinterpret_cast<const float4 *>(tf + gr * kTN + c * 32 + e);
-                            const float4 l4 = *reinterpret_cast<const float4 *>(tf + (kNG + gr) * kTN + c * 32 + e);
-                            const float2 qq = make_float2(qs[gr], qs[gr]);
-                            u[e / 2] = fma2(make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), make_float2(s4.x, s4.y),
-                                            fma2(make_float2(l4.x, l4.y), qq, u[e / 2]));
-                            u[e / 2 + 1] = fma2(make_float2(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])),
-                                                make_float2(s4.z, s4.w), fma2(make_float2(l4.z, l4.w), qq, u[e / 2 + 1]));
-                        }
-                    }
-                    uint32_t hidden = 0;
                     if (edge) {
+                        const int t0 = tok0 + c * 32 + 2 * (lane % 4);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            const int t0 = tok0 + c * 32 + e;
-                            if (t0 < lo || t0 >= hi) {
-                                (e & 1 ? u[e / 2].y : u[e / 2].x) = -INFINITY;
-                                hidden |= 1u << e;
+                        for (int k = 0; k < 4; ++k)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const int tk = t0 + 8 * j;
+                                if (tk < lo[k] || tk >= hi[k]) u[k][j].x = -INFINITY;
+                                if (tk + 1 < lo[k] || tk + 1 >= hi[k]) u[k][j].y = -INFINITY;
+                            }
+                    }
+                    float tm[4];
+                    bool grew = false;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        tm[k] = fmaxf(fmaxf(fmaxf(u[k][0].x, u[k][0].y), fmaxf(u[k][1].x, u[k][1].y)),
+                                      fmaxf(fmaxf(u[k][2].x, u[k][2].y), fmaxf(u[k][3].x, u[k][3].y)));
+                        grew |= tm[k] > over[k];
+                    }
+                    if (__any_sync(0xffffffffu, grew)) {
+                        // rescale the rows' sums, this tile's earlier probabilities among them
+                        float kf[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            tm[k] = fmaxf(tm[k], __shfl_xor_sync(0xffffffffu, tm[k], 1));
+                            tm[k] = fmaxf(tm[k], __shfl_xor_sync(0xffffffffu, tm[k], 2));
+                            kf[k] = 1.0f;
+                            if (tm[k] > over[k]) {
+                                const float to = tm[k] * fr[k];
+                                kf[k] = ex2(m[k] - to);
+                                m[k] = to;
+                                over[k] = tm[k] + 8.0f / fr[k];
+                                l2[k].x *= kf[k], l2[k].y *= kf[k];
                             }
                         }
-                    }
-                    float tm = -INFINITY, t2 = -INFINITY;
-#pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        tm = fmaxf(fmaxf(tm, u[e].x), u[e].y);
-                        t2 = fmaxf(fmaxf(t2, u[e + 1].x), u[e + 1].y);
-                    }
-                    tm = fmaxf(tm, t2);
-                    tm = tm == -INFINITY ? tm : tm * f;
-                    const bool grew = tm > m + 8.0f || (m == -INFINITY && tm > m);
-                    if (__any_sync(0xffffffffu, grew)) {
-                        // rescale the row's sums, this tile's earlier probabilities among them
-                        const float k = grew ? ex2(m - tm) : 1.0f;
-                        if (grew) m = tm;
-                        l *= k, ls.x *= k, ls.y *= k;
                         tmem_wait_st();
 #pragma unroll 1
                         for (int cc = 0; cc < c; ++cc) {
-                            uint32_t w[16];
-                            tmem_ld16(t_s + cc * 16, w);
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) {
-                                const float2 h = __half22float2(*reinterpret_cast<__half2 *>(&w[e]));
-                                w[e] = pack_half2(h.x * k, h.y * k);
+                            for (int h = 0; h < 2; ++h) {
+                                uint32_t w[8];
+                                const uint32_t at = t_s + cc * 16 + (uint32_t(16 * h) << 16);
+                                tmem_ld_frag16(at, w);
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) {
+                                    const float2 v = __half22float2(*reinterpret_cast<__half2 *>(&w[e]));
+                                    w[e] = pack_half2(v.x * kf[2 * h + (e & 1)], v.y * kf[2 * h + (e & 1)]);
+                                }
+                                tmem_st_frag16(at, w);
                             }
-                            tmem_st16(t_s + cc * 16, w);
                         }
                         if (j > 0) {
-                            ok = __all_sync(0xffffffffu, mbar_wait_bounded(pv_done + q, (tile_no - 1) & 1, err));
+                            ok = __all_sync(0xffffffffu, mbar_wait_short(pv_done + q, (tile_no - 1) & 1, err));
                             if (!ok) break;
                             tc_fence_after();
 #pragma unroll 1
-                            for (int d = 0; d < D; d += 16) {
-                                uint32_t w[16];
-                                tmem_ld16(t_o + d, w);
+                            for (int d = 0; d < D; d += 32) {
+                                uint32_t x[16], y[16];
+                                tmem_ld_frag(t_o + d, x);
+                                tmem_ld_frag(t_o + d + (16u << 16), y);
+                                tmem_wait_frag(x, y);
 #pragma unroll
-                                for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) * k);
-                                tmem_st16(t_o + d, w);
+                                for (int e = 0; e < 16; ++e) {
+                                    x[e] = __float_as_uint(__uint_as_float(x[e]) * kf[e >> 1 & 1]);
+                                    y[e] = __float_as_uint(__uint_as_float(y[e]) * kf[2 + (e >> 1 & 1)]);
+                                }
+                                tmem_st_frag(t_o + d, x);
+                                tmem_st_frag(t_o + d + (16u << 16), y);
                             }
                         }
                         tmem_wait_st();
                     }
-                    const float mr = m == -INFINITY ? 0.0f : -m;
-                    uint32_t w[16];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        float2 pr = fma2(u[e], make_float2(f, f), make_float2(mr, mr));
-                        pr.x = ex2(pr.x), pr.y = ex2(pr.y);
-                        if (edge) {
-                            if (hidden >> (2 * e) & 1) pr.x = 0.0f;
-                            if (hidden >> (2 * e + 1) & 1) pr.y = 0.0f;
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t w[8];
+#pragma unroll
+                        for (int kk = 0; kk < 2; ++kk) {
+                            const int k = 2 * h + kk;
+                            const float mr = m[k] == -INFINITY ? 0.0f : -m[k];
+#pragma unroll
+                            for (int jj = 0; jj < 4; ++jj) {
+                                float2 pr = fma2(u[k][jj], make_float2(fr[k], fr[k]), make_float2(mr, mr));
+                                pr.x = ex2(pr.x), pr.y = ex2(pr.y);
+                                l2[k] = add2(l2[k], pr);
+                                w[2 * jj + kk] = pack_half2(pr.x, pr.y);
+                            }
                         }
-                        ls = add2(ls, pr);
-                        w[e] = pack_half2(pr.x, pr.y);
+                        tmem_st_frag16(t_s + c * 16 + (uint32_t(16 * h) << 16), w);
                     }
-                    tmem_st16(t_s + c * 16, w);
                 }
                 if (!ok) break;
-                l += ls.x + ls.y;
                 // values that are not finite are kept out of the product: rows that see one say so here
                 {
                     const volatile uint32_t *bits = poison + 4 * (tile_no & 3);
@@ -389,7 +463,11 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
                     for (int c = 0; c < kTN / 32; ++c) any |= bits[c];
                     if (any) {
                         for (int e = 0; e < kTN; ++e)
-                            if ((bits[e / 32] >> (e % 32) & 1) && tok0 + e >= lo && tok0 + e < hi) l = __int_as_float(0x7fc00000);
+                            if (bits[e / 32] >> (e % 32) & 1) {
+#pragma unroll
+                                for (int k = 0; k < 4; ++k)
+                                    if (tok0 + e >= lo[k] && tok0 + e < hi[k]) l2[k].x = __int_as_float(0x7fc00000);
+                            }
                     }
                 }
                 tmem_wait_st();
@@ -398,9 +476,18 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
             }
             if (!ok) break;
             // ---- the stretch is done: result, or this block's part of it ----
-            ok = __all_sync(0xffffffffu, mbar_wait_bounded(pv_done + q, (tile_no - 1) & 1, err));
+            ok = __all_sync(0xffffffffu, mbar_wait_short(pv_done + q, (tile_no - 1) & 1, err));
             if (!ok) break;
             tc_fence_after();
+            float mrow = 0.0f, l = 0.0f;  // a thread per row again
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float sum = l2[k].x + l2[k].y;
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                const float a = __shfl_sync(0xffffffffu, m[k], (lane & 7) * 4), b = __shfl_sync(0xffffffffu, sum, (lane & 7) * 4);
+                if (lane / 8 == k) mrow = a, l = b;
+            }
             const bool whole = g.first && g.last;
             T *dst = out + ((int64_t)(g.s.q0 + i) * p.a.q_heads + hh) * D;
             const size_t slots = (size_t)2 * gridDim.x * kNQ;
@@ -430,10 +517,10 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
             mbar_arrive(o_free + q);
             if (whole) {
                 if (in && p.a.lse)
-                    p.a.lse[(int64_t)(g.s.q0 + i) * p.a.q_heads + hh] = l == 0.0f ? -INFINITY : (m + log2f(l)) / kLog2e;
+                    p.a.lse[(int64_t)(g.s.q0 + i) * p.a.q_heads + hh] = l == 0.0f ? -INFINITY : (mrow + log2f(l)) / kLog2e;
                 continue;
             }
-            __stcg(ps, make_float2(m, l));
+            __stcg(ps, make_float2(mrow, l));
             __threadfence();
             named_barrier_sync(1 + q, 128);
             const int first = (int)(((g.job_u0 + 1) * blocks - 1) / units), last = (int)((g.job_u1 * blocks - 1) / units);
@@ -473,12 +560,13 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
         }
     } else if (warp >= 8 && warp < 16) {
         // ---------------- unpack ----------------
+        fewer_registers<kCkRegsUnpack>();
         const int tid = threadIdx.x - 256, t3 = lane & 7, quarter0 = lane >> 3;
         const int rot = D == 128 ? t3 >> 1 : D == 256 ? t3 : 0;  // 16-byte reads and writes of 8 lanes hit all banks
         constexpr int kQuads = D / 32;                            // 16-byte pieces of a token's codes
         uint32_t raw_no = 0, item = 0;
         bool ok = true;
-        while (ok && walk.next(g)) {
+        while (ok && next()) {
             int see_lo = 0x7fffffff, see_hi = 0;  // tokens that any row of this job sees
             {
                 const int2 see = Walk::sees(p, g.s, g.row0 / kRows);
@@ -487,13 +575,13 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
             for (int j = 0; j < g.tiles && ok; ++j, ++raw_no) {
                 const int rs = raw_no % S::kRaw, tok0 = g.tok0 + j * kTN;
                 const unsigned char *rw = sm + S::raw + rs * S::kRawBytes;
-                ok = mbar_wait_bounded(raw_full + rs, (raw_no / S::kRaw) & 1, err);
+                ok = mbar_wait_short(raw_full + rs, (raw_no / S::kRaw) & 1, err);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
 #pragma unroll
                 for (int kv = 0; kv < 2; ++kv, ++item) {
                     const int sl = item % S::kSlots;
-                    ok = mbar_wait_bounded(deq_empty + sl, ((item / S::kSlots) & 1) ^ 1, err);
+                    ok = mbar_wait_short(deq_empty + sl, ((item / S::kSlots) & 1) ^ 1, err);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     unsigned char *dst = sm + S::slot + sl * S::kSlot;
@@ -508,8 +596,9 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
 #pragma unroll
                         for (int gr = 0; gr < kNG; ++gr) {
                             const float2 kf = __half22float2(meta[tid * kNG + gr]);
-                            tf[gr * kTN + tid] = seen ? kf.x : 0.0f;
-                            tf[(kNG + gr) * kTN + tid] = seen ? kf.y : 0.0f;
+                            float *at = tf + (gr * (kTN / 2) + tid / 2) * 4 + (tid & 1);
+                            at[0] = seen ? kf.x : 0.0f;
+                            at[2] = seen ? kf.y : 0.0f;
                             const uint32_t u = *reinterpret_cast<const uint32_t *>(vm + tid * kNG + gr);
                             bad |= (u & 0x7c00u) == 0x7c00u || (u & 0x7c000000u) == 0x7c000000u;
                         }
@@ -572,7 +661,11 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
                 }
             }
         }
-    } else if (warp == 16) {
+    } else if (warp < 16) {
+        fewer_registers<kCkRegsRest>();  // (no second row tile)
+    } else {
+        fewer_registers<kCkRegsRest>();
+        if (warp == 16) {
         // ---------------- copies from the pages ----------------
         const Kv4Block blk(P, D, kG);
         const int per = min(P, kTN), piece = lane >> 2, kind = lane & 3;
@@ -581,10 +674,10 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
         const uint32_t dst_at = (kind & 1 ? (kind < 2 ? S::kCodes : S::kMeta) : 0) + (kind < 2 ? 0 : 2 * S::kCodes);
         uint32_t raw_no = 0;
         bool ok = true;
-        while (ok && walk.next(g)) {
+        while (ok && next()) {
             for (int j = 0; j < g.tiles; ++j, ++raw_no) {
                 const int rs = raw_no % S::kRaw, tok0 = g.tok0 + j * kTN;
-                ok = __all_sync(0xffffffffu, mbar_wait_bounded(raw_empty + rs, ((raw_no / S::kRaw) & 1) ^ 1, err));
+                ok = __all_sync(0xffffffffu, mbar_wait_short(raw_empty + rs, ((raw_no / S::kRaw) & 1) ^ 1, err));
                 if (!ok) break;
                 const int pieces = max(0, min(kTN / per, (g.s.len - tok0 + per - 1) / per));
                 uint32_t bytes = 0;
@@ -607,14 +700,14 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
         }
         // the last copy into each stage has landed before the block exits
         for (uint32_t k = raw_no > S::kRaw ? raw_no - S::kRaw : 0; k < raw_no; ++k)
-            mbar_wait_bounded(raw_full + k % S::kRaw, (k / S::kRaw) & 1, err);
-    } else if (warp == 17 && lane == 0) {
+            mbar_wait_short(raw_full + k % S::kRaw, (k / S::kRaw) & 1, err);
+        } else if (warp == 17 && lane == 0) {
         // ---------------- products ----------------
         constexpr uint32_t id_qk = idesc_f16(128, kTN, false), id_pv = idesc_f16(128, D, true);
         uint32_t seg_no = 0, done = 0;  // stretches and tiles before this one
         bool ok = true;
         auto slot_wait = [&](uint32_t item) {
-            const bool w = mbar_wait_bounded(deq_full + item % S::kSlots, (item / S::kSlots) & 1, err);
+            const bool w = mbar_wait_short(deq_full + item % S::kSlots, (item / S::kSlots) & 1, err);
             tc_fence_after();
             return w;
         };
@@ -641,8 +734,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
             mma_commit(pv_done + q);
             if (q == kNQ - 1) mma_commit(deq_empty + (2 * tile + 1) % S::kSlots);
         };
-        while (ok && walk.next(g)) {
-            for (int q = 0; q < kNQ && ok; ++q) ok = mbar_wait_bounded(q_full + q, seg_no & 1, err);
+        while (ok && walk.next(p, base)) {
+            for (int q = 0; q < kNQ && ok; ++q) ok = mbar_wait_short(q_full + q, seg_no & 1, err);
             tc_fence_after();
             constexpr int kAhead = kNQ == 2 ? 1 : 2;  // score tiles issued ahead of the second product
             for (int a = 0; a < min(kAhead, g.tiles) && ok; ++a) {
@@ -653,8 +746,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
                 const uint32_t tile = done + j;
                 for (int q = 0; q < kNQ && ok; ++q) {
                     if (q == 0) ok = slot_wait(2 * tile + 1);
-                    if (j == 0 && ok) ok = mbar_wait_bounded(o_free + q, (seg_no & 1) ^ 1, err);
-                    if (ok) ok = mbar_wait_bounded(p_full + buffer(q, tile), kNQ == 2 ? tile & 1 : tile >> 1 & 1, err);
+                    if (j == 0 && ok) ok = mbar_wait_short(o_free + q, (seg_no & 1) ^ 1, err);
+                    if (ok) ok = mbar_wait_short(p_full + buffer(q, tile), kNQ == 2 ? tile & 1 : tile >> 1 & 1, err);
                     if (!ok) break;
                     tc_fence_after();
                     pv(q, tile, j > 0);
@@ -668,7 +761,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
             ++seg_no;
         }
         mma_commit(mma_done);  // every product has finished before TMEM is freed
-        mbar_wait_bounded(mma_done, 0, err);
+        mbar_wait_short(mma_done, 0, err);
+        }
     }
     tc_fence_before();
     __syncthreads();
