@@ -49,20 +49,28 @@ __device__ __forceinline__ void fewer_registers() {
 
 template <int D, int kNG, int kNQ>
 struct ChunkSmem {
-    static constexpr int kTN = 128 / kNG;                           // tokens of a tile: 128 columns of scores
+    // Score buffers per row tile: two where TMEM holds them beside the outputs (kNQ x (D + kBufs x
+    // kNG x kTN) <= 512 columns), so that the next scores are formed while softmax runs.
+    static constexpr int kBufs = kNQ == 1 || kNG == 1 ? 2 : 1;
+    static constexpr int kTN = kNQ == 2 && kNG == 1 ? 64 : 128 / kNG;  // tokens of a tile
     static constexpr uint32_t kQ = 128 * D * 2, kSlot = kTN * D * 2;
-    static constexpr int kSlots = (kNQ * kQ + 4 * kSlot <= 160 * 1024) ? 4 : 3;
+    static constexpr int kFit = (160 * 1024 - kNQ * kQ) / kSlot;
+    static constexpr int kSlots = kFit < 3 ? 3 : kFit < 6 ? kFit : 6;  // unpacked tiles, keys and values in turn
     static constexpr int kRaw = 3;
+    // Tables of key factors (and marks of bad values) in use at once: keys of tile t + m are
+    // unpacked once the slot's last tile is free: with 6 slots keys of t + m - 3, multiplied after
+    // the softmax of t + m - 5; with 4, t + m - 2 and t + m - 4; with 3, values of t + m - 2.
+    static constexpr int kTables = kSlots > 4 ? 8 : 4;
     static constexpr uint32_t kCodes = kTN * D / 2, kMeta = kTN * kNG * 4;
     static constexpr uint32_t kRawBytes = 2 * kCodes + 2 * kMeta;
     static constexpr uint32_t q = 0;
     static constexpr uint32_t slot = q + kNQ * kQ;
     static constexpr uint32_t raw = slot + kSlots * kSlot;
-    static constexpr uint32_t fac = raw + kRaw * kRawBytes;         // [4][kNG][kTN / 2] (two scales, two lows) of the keys
-    static constexpr uint32_t poison = fac + 4 * 2 * kNG * kTN * 4; // [4][4] bits: token's value is not finite
-    static constexpr uint32_t misc = poison + 64;                   // tmem slot, last-to-arrive flags
+    static constexpr uint32_t fac = raw + kRaw * kRawBytes;         // [kTables][kNG][kTN / 2] (two scales, two lows)
+    static constexpr uint32_t poison = fac + kTables * 2 * kNG * kTN * 4;  // [kTables][4] bits: value is not finite
+    static constexpr uint32_t misc = poison + kTables * 16;                   // tmem slot, last-to-arrive flags
     static constexpr uint32_t bars = misc + 32;
-    static constexpr uint32_t walk = bars + 256;                    // [warp] WarpWalk
+    static constexpr uint32_t walk = bars + 288;                    // [warp] Walker
     static constexpr uint32_t base = walk + 18 * 160;               // int64[seqs + 1]
     static constexpr size_t bytes(uint32_t seqs) { return 1024 + base + 8 * (size_t)(seqs + 1); }
 };
@@ -168,7 +176,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
     constexpr uint32_t kQBlock = 128 * 128, kTBlock = kTN * 128;  // bytes of 64 dimensions of a tile
     constexpr uint32_t kOCol = 0, kSCol = kNQ * D;                // TMEM columns: O tiles, then S buffers
     constexpr uint32_t kSCols = kNG * kTN;                        // of one buffer: a block per group
-    static_assert(kNQ * D + 2 * kSCols <= 512, "");
+    constexpr int kBufs = S::kBufs;
+    static_assert(kNQ * (D + kBufs * kSCols) <= 512, "");
     extern __shared__ unsigned char ck_raw[];
     unsigned char *sm = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(ck_raw) + 1023) & ~uintptr_t(1023));
     float *fac = reinterpret_cast<float *>(sm + S::fac);
@@ -178,8 +187,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
     uint64_t *raw_full = bars, *raw_empty = raw_full + S::kRaw;
     uint64_t *deq_full = raw_empty + S::kRaw, *deq_empty = deq_full + S::kSlots;
     uint64_t *q_full = deq_empty + S::kSlots, *o_free = q_full + 2;
-    uint64_t *s_full = o_free + 2, *p_full = s_full + 2, *pv_done = p_full + 2, *mma_done = pv_done + 2;
-    static_assert((2 * S::kRaw + 2 * S::kSlots + 11) * 8 <= 256, "");
+    uint64_t *s_full = o_free + 2, *p_full = s_full + 4, *pv_done = p_full + 4, *mma_done = pv_done + 2;
+    static_assert((2 * S::kRaw + 2 * S::kSlots + 15) * 8 <= 288, "");
     int64_t *base = reinterpret_cast<int64_t *>(sm + S::base);
     int *err = p.c.status;
 
@@ -191,9 +200,9 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
         for (int i = 0; i < S::kRaw; ++i) mbar_init(raw_full + i, 1), mbar_init(raw_empty + i, 8);
         for (int i = 0; i < S::kSlots; ++i) mbar_init(deq_full + i, 8), mbar_init(deq_empty + i, 1);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(q_full + i, 128), mbar_init(o_free + i, 128), mbar_init(s_full + i, 1);
-            mbar_init(p_full + i, 128), mbar_init(pv_done + i, 1);
+            mbar_init(q_full + i, 128), mbar_init(o_free + i, 128), mbar_init(pv_done + i, 1);
         }
+        for (int i = 0; i < 4; ++i) mbar_init(s_full + i, 1), mbar_init(p_full + i, 128);
         mbar_init(mma_done, 1);
         fence_barrier_init();
     }
@@ -332,15 +341,15 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
                 }
             }
             for (int j = 0; j < g.tiles && ok; ++j, ++tile_no) {
-                const int buf = kNQ == 2 ? q : (int)(tile_no & 1);
-                const uint32_t sph = kNQ == 2 ? tile_no & 1 : (tile_no >> 1) & 1;
+                const int buf = q * kBufs + (int)(tile_no % kBufs);
+                const uint32_t sph = tile_no / kBufs & 1;
                 const uint32_t t_s = lanes + kSCol + buf * kSCols;
                 const int tok0 = g.tok0 + j * kTN;
                 const bool edge = tok0 + kTN > hi_min || tok0 < lo_max;
                 ok = __all_sync(0xffffffffu, mbar_wait_short(s_full + buf, sph, err));
                 if (!ok) break;
                 tc_fence_after();
-                const float4 *tf = reinterpret_cast<const float4 *>(fac + (tile_no & 3) * 2 * kNG * kTN) + lane % 4;
+                const float4 *tf = reinterpret_cast<const float4 *>(fac + (tile_no % S::kTables) * 2 * kNG * kTN) + lane % 4;
 #pragma unroll 1
                 for (int c = 0; c < kTN / 32; ++c) {
                     // scores of 32 tokens x 32 rows: u[k][j] columns 8 j + 2 t, + 1 of row 8 k + g
@@ -457,7 +466,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
                 if (!ok) break;
                 // values that are not finite are kept out of the product: rows that see one say so here
                 {
-                    const volatile uint32_t *bits = poison + 4 * (tile_no & 3);
+                    const volatile uint32_t *bits = poison + 4 * (tile_no % S::kTables);
                     uint32_t any = 0;
 #pragma unroll
                     for (int c = 0; c < kTN / 32; ++c) any |= bits[c];
@@ -589,7 +598,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
                     const __half2 *meta = reinterpret_cast<const __half2 *>(rw + 2 * S::kCodes + kv * S::kMeta);
                     if (kv == 0 && tid < kTN) {  // the keys' factors; which values are not finite
                         const __half2 *vm = reinterpret_cast<const __half2 *>(rw + 2 * S::kCodes + S::kMeta);
-                        float *tf = fac + (raw_no & 3) * 2 * kNG * kTN;
+                        float *tf = fac + (raw_no % S::kTables) * 2 * kNG * kTN;
                         const int tok = tok0 + tid;
                         const bool seen = tok >= see_lo && tok < see_hi;
                         bool bad = false;
@@ -603,12 +612,13 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
                             bad |= (u & 0x7c00u) == 0x7c00u || (u & 0x7c000000u) == 0x7c000000u;
                         }
                         const uint32_t bits = __ballot_sync(0xffffffffu, bad && seen);
-                        if (lane == 0) poison[4 * (raw_no & 3) + tid / 32] = bits;
+                        if (lane == 0) poison[4 * (raw_no % S::kTables) + tid / 32] = bits;
                     }
 #pragma unroll
-                    for (int it = 0; it < kTN * kQuads / 256; ++it) {
+                    for (int it = 0; it < (kTN * kQuads + 255) / 256; ++it) {
                         // 8 tokens x 4 pieces per warp and step
                         const int step = it * 8 + (warp - 8);
+                        if (kTN * kQuads % 256 && step >= kTN * kQuads / 32) break;
                         constexpr int kParts = kQuads > 4 ? kQuads / 4 : 1;
                         const int tg8 = step / kParts, part = step % kParts;
                         int tk, quad;
@@ -711,7 +721,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
             tc_fence_after();
             return w;
         };
-        auto buffer = [&](int q, uint32_t tile) { return kNQ == 2 ? q : (int)(tile & 1); };
+        auto buffer = [&](int q, uint32_t tile) { return q * kBufs + (int)(tile % kBufs); };
         auto qk = [&](int q, uint32_t tile) {  // scores of row tile q against key tile `tile`
             const unsigned char *kt = sm + S::slot + (2 * tile) % S::kSlots * S::kSlot;
             const uint64_t a0 = smem_desc_sw128(sm + S::q + q * S::kQ), b0 = smem_desc_sw128(kt);
@@ -737,7 +747,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
         while (ok && walk.next(p, base)) {
             for (int q = 0; q < kNQ && ok; ++q) ok = mbar_wait_short(q_full + q, seg_no & 1, err);
             tc_fence_after();
-            constexpr int kAhead = kNQ == 2 ? 1 : 2;  // score tiles issued ahead of the second product
+            constexpr int kAhead = kBufs;  // score tiles issued ahead of the second product
             for (int a = 0; a < min(kAhead, g.tiles) && ok; ++a) {
                 ok = slot_wait(2 * (done + a));
                 for (int q = 0; q < kNQ && ok; ++q) qk(q, done + a);
@@ -747,7 +757,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
                 for (int q = 0; q < kNQ && ok; ++q) {
                     if (q == 0) ok = slot_wait(2 * tile + 1);
                     if (j == 0 && ok) ok = mbar_wait_short(o_free + q, (seg_no & 1) ^ 1, err);
-                    if (ok) ok = mbar_wait_short(p_full + buffer(q, tile), kNQ == 2 ? tile & 1 : tile >> 1 & 1, err);
+                    if (ok) ok = mbar_wait_short(p_full + buffer(q, tile), tile / kBufs & 1, err);
                     if (!ok) break;
                     tc_fence_after();
                     pv(q, tile, j > 0);
