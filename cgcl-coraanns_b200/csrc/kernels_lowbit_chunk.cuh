@@ -479,6 +479,12 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
                             }
                     }
                 }
+                // The product before this one has finished: so the waits on pv_done, which know a
+                // phase by its parity alone, are never two phases apart.
+                if (j > 0) {
+                    ok = __all_sync(0xffffffffu, mbar_wait_short(pv_done + q, (tile_no - 1) & 1, err));
+                    if (!ok) break;
+                }
                 tmem_wait_st();
                 tc_fence_before();
                 mbar_arrive(p_full + buf);

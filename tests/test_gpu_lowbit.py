@@ -311,6 +311,23 @@ def test_attend_long_split_over_blocks(lb):
     assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("D,G,H,per,n,lens", [
+    (128, 128, 8, 4, [1024], [4096]), (64, 64, 4, 8, [600, 70], [2000, 7000]), (128, 64, 8, 4, [500, 100, 7], [4096, 100, 3000]),
+    (256, 128, 4, 3, [300, 17, 200], [3000, 40, 900]), (128, 128, 2, 16, [1], [30000]), (128, 64, 2, 2, [1, 2, 3], [9000, 20, 700])])
+def test_attend_repeats_bit_for_bit(lb, D, G, H, per, n, lens):
+    """A hand-over that came too early anywhere in the pipelines would show as a changing result."""
+    pages = sum(-(-x // 32) for x in lens)
+    cache = random_cache(lb, pages, H, D, 32, G, seed=8)
+    _, table = page_tables(lens, 32, pages, 9)
+    dl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    qs = torch.tensor(np.concatenate(([0], np.cumsum(n))), dtype=torch.int32, device="cuda")
+    q = torch.randn(sum(n), H * per, D, device="cuda").to(torch.bfloat16)
+    want = cache.attend(q, table, dl, q_start=qs, max_queries=max(n))
+    for _ in range(60):
+        assert torch.equal(cache.attend(q, table, dl, q_start=qs, max_queries=max(n)), want)
+    cache.check()
+
+
 def test_attend_many_sequences(lb):
     """More sequences than one launch takes (their offsets live in shared memory)."""
     rng = np.random.default_rng(0)
