@@ -89,21 +89,30 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t *bar, uint32_t parity
         __nanosleep(64);
     }
 }
-// The same for waits that are short and often: no sleep between tries (try_wait itself suspends
-// the thread for a while), the clock read once in 64 tries.
+// The same for kernels whose warps wait often: no sleep between tries, but each try may suspend
+// the thread for up to a millisecond (spinning warps would take issue slots from working ones).
+__device__ __forceinline__ bool mbar_try_wait_long(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
+        : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ bool mbar_wait_short(uint64_t *bar, uint32_t parity, int *err,
                                                 uint64_t limit_ns = 2000000000ull) {
-    if (mbar_try_wait(bar, parity)) return true;
+    if (mbar_try_wait_long(bar, parity)) return true;
     const uint64_t t0 = global_ns();
-    while (true) {
 #pragma unroll 1
-        for (int i = 0; i < 64; ++i)
-            if (mbar_try_wait(bar, parity)) return true;
+    while (!mbar_try_wait_long(bar, parity)) {
         if (global_ns() - t0 > limit_ns) {
             atomicOr(err, kDevWaitTimeout);
             return false;
         }
     }
+    return true;
 }
 // 1-D bulk copy global -> shared; both addresses 16-byte aligned, bytes % 16 == 0.
 __device__ __forceinline__ void bulk_g2s(void *smem_dst, const void *gmem_src, uint32_t bytes,

@@ -32,11 +32,11 @@
 
 namespace cora {
 
-// Registers per thread: 640 x 96 at launch; then softmax 136, unpack 72, the last group 64
-// (256 x 136 + 256 x 72 + 128 x 64 = 61440). Spilled variables would go to L2: shared
+// Registers per thread: 640 x 96 at launch; then softmax 144, unpack 72, the last group 48
+// (256 x 144 + 256 x 72 + 128 x 48 = 61440). Spilled variables would go to L2: shared
 // memory leaves almost no L1.
 constexpr int kCkThreads = 640, kCkMinRun = 2;
-constexpr int kCkRegsSoftmax = 136, kCkRegsUnpack = 72, kCkRegsRest = 64;
+constexpr int kCkRegsSoftmax = 144, kCkRegsUnpack = 72, kCkRegsRest = 48;
 static_assert(256 * kCkRegsSoftmax + 256 * kCkRegsUnpack + 128 * kCkRegsRest <= kCkThreads * 96, "");
 template <int kRegs>
 __device__ __forceinline__ void more_registers() {
@@ -49,10 +49,11 @@ __device__ __forceinline__ void fewer_registers() {
 
 template <int D, int kNG, int kNQ>
 struct ChunkSmem {
-    // Score buffers per row tile: two where TMEM holds them beside the outputs (kNQ x (D + kBufs x
-    // kNG x kTN) <= 512 columns), so that the next scores are formed while softmax runs.
-    static constexpr int kBufs = kNQ == 1 || kNG == 1 ? 2 : 1;
-    static constexpr int kTN = kNQ == 2 && kNG == 1 ? 64 : 128 / kNG;  // tokens of a tile
+    static constexpr int kTN = 128 / kNG;             // tokens of a tile: 128 columns of scores
+    // Score buffers per row tile. One row tile alone needs two (the next scores are formed while
+    // softmax runs); two row tiles take turns with one each (64-token tiles with two buffers
+    // each measured 788 against 730 us at 2048 queries, 16384 tokens: more issue per token).
+    static constexpr int kBufs = kNQ == 1 ? 2 : 1;
     static constexpr uint32_t kQ = 128 * D * 2, kSlot = kTN * D * 2;
     static constexpr int kFit = (160 * 1024 - kNQ * kQ) / kSlot;
     static constexpr int kSlots = kFit < 3 ? 3 : kFit < 6 ? kFit : 6;  // unpacked tiles, keys and values in turn
@@ -187,8 +188,10 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
     uint64_t *raw_full = bars, *raw_empty = raw_full + S::kRaw;
     uint64_t *deq_full = raw_empty + S::kRaw, *deq_empty = deq_full + S::kSlots;
     uint64_t *q_full = deq_empty + S::kSlots, *o_free = q_full + 2;
-    uint64_t *s_full = o_free + 2, *p_full = s_full + 4, *pv_done = p_full + 4, *mma_done = pv_done + 2;
-    static_assert((2 * S::kRaw + 2 * S::kSlots + 15) * 8 <= 288, "");
+    // (pv_done has a barrier per tile parity: a wait on one knows a phase by its parity alone, and
+    // the softmax may be two second products ahead)
+    uint64_t *s_full = o_free + 2, *p_full = s_full + 4, *pv_done = p_full + 4, *mma_done = pv_done + 4;
+    static_assert((2 * S::kRaw + 2 * S::kSlots + 17) * 8 <= 288, "");
     int64_t *base = reinterpret_cast<int64_t *>(sm + S::base);
     int *err = p.c.status;
 
@@ -200,9 +203,9 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
         for (int i = 0; i < S::kRaw; ++i) mbar_init(raw_full + i, 1), mbar_init(raw_empty + i, 8);
         for (int i = 0; i < S::kSlots; ++i) mbar_init(deq_full + i, 8), mbar_init(deq_empty + i, 1);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(q_full + i, 128), mbar_init(o_free + i, 128), mbar_init(pv_done + i, 1);
+            mbar_init(q_full + i, 4), mbar_init(o_free + i, 4);  // (an arrival per warp)
         }
-        for (int i = 0; i < 4; ++i) mbar_init(s_full + i, 1), mbar_init(p_full + i, 128);
+        for (int i = 0; i < 4; ++i) mbar_init(s_full + i, 1), mbar_init(p_full + i, 4), mbar_init(pv_done + i, 1);
         mbar_init(mma_done, 1);
         fence_barrier_init();
     }
@@ -315,7 +318,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
                 qs[gr] = sum * 5.9604644775390625e-8f;  // 2^-24
             }
             fence_proxy_async_smem();
-            mbar_arrive(q_full + q);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full + q);
             // From here a thread holds rows 8 k + lane / 4 of its warp, k = 0..3.
             float fr[4], qr[4][kNG], m[4], over[4];  // unit of the scores; sums of q; maximum, room above it
             int lo[4], hi[4];                        // tokens that the row sees
@@ -425,7 +429,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
                             }
                         }
                         if (j > 0) {
-                            ok = __all_sync(0xffffffffu, mbar_wait_short(pv_done + q, (tile_no - 1) & 1, err));
+                            ok = __all_sync(0xffffffffu, mbar_wait_short(pv_done + 2 * q + ((tile_no - 1) & 1), (tile_no - 1) >> 1 & 1, err));
                             if (!ok) break;
                             tc_fence_after();
 #pragma unroll 1
@@ -479,19 +483,14 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
                             }
                     }
                 }
-                // The product before this one has finished: so the waits on pv_done, which know a
-                // phase by its parity alone, are never two phases apart.
-                if (j > 0) {
-                    ok = __all_sync(0xffffffffu, mbar_wait_short(pv_done + q, (tile_no - 1) & 1, err));
-                    if (!ok) break;
-                }
                 tmem_wait_st();
                 tc_fence_before();
-                mbar_arrive(p_full + buf);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full + buf);
             }
             if (!ok) break;
             // ---- the stretch is done: result, or this block's part of it ----
-            ok = __all_sync(0xffffffffu, mbar_wait_short(pv_done + q, (tile_no - 1) & 1, err));
+            ok = __all_sync(0xffffffffu, mbar_wait_short(pv_done + 2 * q + ((tile_no - 1) & 1), (tile_no - 1) >> 1 & 1, err));
             if (!ok) break;
             tc_fence_after();
             float mrow = 0.0f, l = 0.0f;  // a thread per row again
@@ -529,7 +528,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
                 }
             }
             tc_fence_before();
-            mbar_arrive(o_free + q);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(o_free + q);
             if (whole) {
                 if (in && p.a.lse)
                     p.a.lse[(int64_t)(g.s.q0 + i) * p.a.q_heads + hh] = l == 0.0f ? -INFINITY : (mrow + log2f(l)) / kLog2e;
@@ -717,11 +717,13 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
         // the last copy into each stage has landed before the block exits
         for (uint32_t k = raw_no > S::kRaw ? raw_no - S::kRaw : 0; k < raw_no; ++k)
             mbar_wait_short(raw_full + k % S::kRaw, (k / S::kRaw) & 1, err);
-        } else if (warp == 17 && lane == 0) {
+        } else if (warp == 17) {
         // ---------------- products ----------------
         constexpr uint32_t id_qk = idesc_f16(128, kTN, false), id_pv = idesc_f16(128, D, true);
         uint32_t seg_no = 0, done = 0;  // stretches and tiles before this one
         bool ok = true;
+        const uint32_t leader = elect_one();
+        const uint32_t sm0 = __shfl_sync(0xffffffffu, smem_u32(sm), 0), tm0 = __shfl_sync(0xffffffffu, tmem, 0);
         auto slot_wait = [&](uint32_t item) {
             const bool w = mbar_wait_short(deq_full + item % S::kSlots, (item / S::kSlots) & 1, err);
             tc_fence_after();
@@ -729,36 +731,37 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
         };
         auto buffer = [&](int q, uint32_t tile) { return q * kBufs + (int)(tile % kBufs); };
         auto qk = [&](int q, uint32_t tile) {  // scores of row tile q against key tile `tile`
-            const unsigned char *kt = sm + S::slot + (2 * tile) % S::kSlots * S::kSlot;
-            const uint64_t a0 = smem_desc_sw128(sm + S::q + q * S::kQ), b0 = smem_desc_sw128(kt);
-            const uint32_t d = tmem + kSCol + buffer(q, tile) * kSCols;
+            const uint32_t kt = sm0 + S::slot + (2 * tile) % S::kSlots * S::kSlot;
+            const uint32_t a0 = desc_low(sm0 + S::q + q * S::kQ), b0 = desc_low(kt);
+            const uint32_t d = tm0 + kSCol + buffer(q, tile) * kSCols;
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
                 const int gr = k / (kG / 16);
-                mma_f16(d + gr * kTN, a0 + (k / 4) * (kQBlock >> 4) + (k % 4) * 2, b0 + (k / 4) * (kTBlock >> 4) + (k % 4) * 2,
+                mma_f16(leader, d + gr * kTN, a0 + (k / 4) * (kQBlock >> 4) + (k % 4) * 2, b0 + (k / 4) * (kTBlock >> 4) + (k % 4) * 2,
                         id_qk, k % (kG / 16) != 0);
             }
-            mma_commit(s_full + buffer(q, tile));
-            if (q == kNQ - 1) mma_commit(deq_empty + (2 * tile) % S::kSlots);
+            mma_commit_by(leader, s_full + buffer(q, tile));
+            if (q == kNQ - 1) mma_commit_by(leader, deq_empty + (2 * tile) % S::kSlots);
         };
         auto pv = [&](int q, uint32_t tile, bool add) {
-            const unsigned char *vt = sm + S::slot + (2 * tile + 1) % S::kSlots * S::kSlot;
-            const uint64_t b0 = smem_desc_sw128_mn(vt, kTBlock);
-            const uint32_t a = tmem + kSCol + buffer(q, tile) * kSCols;
+            const uint32_t vt = sm0 + S::slot + (2 * tile + 1) % S::kSlots * S::kSlot;
+            const uint32_t b0 = desc_low(vt, kTBlock);
+            const uint32_t a = tm0 + kSCol + buffer(q, tile) * kSCols;
 #pragma unroll
-            for (int k = 0; k < kTN / 16; ++k) mma_f16_ta(tmem + kOCol + q * D, a + k * 8, b0 + k * (2048 >> 4), id_pv, add || k != 0);
-            mma_commit(pv_done + q);
-            if (q == kNQ - 1) mma_commit(deq_empty + (2 * tile + 1) % S::kSlots);
+            for (int k = 0; k < kTN / 16; ++k) mma_f16_ta(leader, tm0 + kOCol + q * D, a + k * 8, b0 + k * (2048 >> 4), id_pv, add || k != 0);
+            mma_commit_by(leader, pv_done + 2 * q + (tile & 1));
+            if (q == kNQ - 1) mma_commit_by(leader, deq_empty + (2 * tile + 1) % S::kSlots);
         };
-        while (ok && walk.next(p, base)) {
+        while (ok && next()) {
+            const int tiles = __shfl_sync(0xffffffffu, g.tiles, 0);
             for (int q = 0; q < kNQ && ok; ++q) ok = mbar_wait_short(q_full + q, seg_no & 1, err);
             tc_fence_after();
             constexpr int kAhead = kBufs;  // score tiles issued ahead of the second product
-            for (int a = 0; a < min(kAhead, g.tiles) && ok; ++a) {
+            for (int a = 0; a < min(kAhead, tiles) && ok; ++a) {
                 ok = slot_wait(2 * (done + a));
                 for (int q = 0; q < kNQ && ok; ++q) qk(q, done + a);
             }
-            for (int j = 0; j < g.tiles && ok; ++j) {
+            for (int j = 0; j < tiles && ok; ++j) {
                 const uint32_t tile = done + j;
                 for (int q = 0; q < kNQ && ok; ++q) {
                     if (q == 0) ok = slot_wait(2 * tile + 1);
@@ -767,16 +770,16 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
                     if (!ok) break;
                     tc_fence_after();
                     pv(q, tile, j > 0);
-                    if (j + kAhead < g.tiles) {
+                    if (j + kAhead < tiles) {
                         if (q == 0) ok = slot_wait(2 * (tile + kAhead));
                         if (ok) qk(q, tile + kAhead);
                     }
                 }
             }
-            done += g.tiles;
+            done += tiles;
             ++seg_no;
         }
-        mma_commit(mma_done);  // every product has finished before TMEM is freed
+        mma_commit_by(leader, mma_done);  // every product has finished before TMEM is freed
         mbar_wait_short(mma_done, 0, err);
         }
     }

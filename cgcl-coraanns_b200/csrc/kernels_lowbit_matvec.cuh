@@ -33,6 +33,25 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
 
 constexpr int kMvWarps = 8;
 
+// 16 bytes that are read once: they do not displace the activations from L1.
+__device__ __forceinline__ uint4 ld_stream(const void *p) {
+    uint4 v;
+    asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+        : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+        : "l"(p));
+    return v;
+}
+template <int kWords>
+__device__ __forceinline__ void ld_factors(const uint32_t *p, uint32_t (&f)[kWords]) {
+    if constexpr (kWords == 1) {
+        asm("ld.global.nc.u32 %0, [%1];" : "=r"(f[0]) : "l"(p));
+    } else if constexpr (kWords == 2) {
+        asm("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(f[0]), "=r"(f[1]) : "l"(p));
+    } else {
+        asm("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(f[0]), "=r"(f[1]), "=r"(f[2]), "=r"(f[3]) : "l"(p));
+    }
+}
+
 // One warp: kMT tiles of 16 weight rows, segments of 128 columns warp, warp + 8, ...; the
 // block's warps split the columns and add up in shared memory. grid: x over 16 kMT weight rows,
 // y over 8 kNT activation rows. kVec: x rows may be read 16 bytes at a time.
@@ -46,11 +65,15 @@ constexpr int kMvWarps = 8;
 //   bf16 x: 0x4300 | c is 128 + c; the 128 sum(x) is taken off with the low term. The sums hold
 //           24 bits, of which the offset costs about five, and the result keeps eight.
 // sum(x) of a group comes from one more product with a matrix of ones.
+//
+// What bounds it: reading the weights. Codes and factors of the next kMvDepth segments are in
+// flight in registers (a warp and segment: 1 or 2 KB).
 template <typename T, int kGroup, int kMT, int kNT, bool kVec>
-__global__ void __launch_bounds__(kMvWarps * 32) w4_matvec_kernel(const cora_w4_weight w,
-                                                                  const cora_w4_matvec_args p) {
+__global__ void __launch_bounds__(kMvWarps * 32, kNT >= 4 ? 1 : 2) w4_matvec_kernel(const cora_w4_weight w,
+                                                                                    const cora_w4_matvec_args p) {
     constexpr bool kHalf = std::is_same<T, __half>::value;
     constexpr int kGroups = 128 / kGroup, kSteps = kGroup / 32;
+    constexpr int kMvDepth = kNT >= 4 ? 2 : kMT == 2 ? 3 : 4;
     extern __shared__ float mv_red[];  // [warp][row of x][weight row]
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
     const int n0 = blockIdx.x * 16 * kMT, m0 = blockIdx.y * 8 * kNT;
@@ -58,19 +81,19 @@ __global__ void __launch_bounds__(kMvWarps * 32) w4_matvec_kernel(const cora_w4_
     const uint64_t row_bytes = (uint64_t)segs * 64, row_groups = (uint64_t)segs * kGroups;
     const int rows = (int)w.rows;
     const uint8_t *cp[2 * kMT];
-    const __half2 *mp[2 * kMT];
+    const uint32_t *mp[2 * kMT];
 #pragma unroll
     for (int i = 0; i < 2 * kMT; ++i) {
         const int r = min(n0 + i * 8 + g, rows - 1);
         cp[i] = w.codes + r * row_bytes + t * 16;
-        mp[i] = static_cast<const __half2 *>(w.meta) + r * row_groups;
+        mp[i] = static_cast<const uint32_t *>(w.meta) + r * row_groups;
     }
     const T *xp[kNT];
     bool xin[kNT];
 #pragma unroll
     for (int n = 0; n < kNT; ++n) {
         xin[n] = m0 + n * 8 + g < (int)p.rows;
-        xp[n] = static_cast<const T *>(p.x) + (uint64_t)(xin[n] ? m0 + n * 8 + g : 0) * p.x_stride;
+        xp[n] = static_cast<const T *>(p.x) + (uint64_t)(xin[n] ? m0 + n * 8 + g : 0) * p.x_stride + t * 8;
     }
     float y[kMT][kNT][4];
 #pragma unroll
@@ -80,94 +103,105 @@ __global__ void __launch_bounds__(kMvWarps * 32) w4_matvec_kernel(const cora_w4_
 #pragma unroll
             for (int c = 0; c < 4; ++c) y[i][n][c] = 0.0f;
 
-    uint4 code[2 * kMT];
-    if (warp < segs) {
+    uint4 code[kMvDepth][2 * kMT];
+    uint32_t fac[kMvDepth][2 * kMT][kGroups];
+    auto fetch = [&](int s, uint4 (&c)[2 * kMT], uint32_t (&f)[2 * kMT][kGroups]) {
+        if (s >= segs) return;
 #pragma unroll
-        for (int i = 0; i < 2 * kMT; ++i) code[i] = __ldg(reinterpret_cast<const uint4 *>(cp[i] + (uint64_t)warp * 64));
-    }
-    for (int s = warp; s < segs; s += kMvWarps) {
-        uint4 next[2 * kMT];
-        const int s2 = s + kMvWarps < segs ? s + kMvWarps : s;
+        for (int i = 0; i < 2 * kMT; ++i) {
+            c[i] = ld_stream(cp[i] + (uint32_t)s * 64);
+            ld_factors<kGroups>(mp[i] + (uint32_t)s * kGroups, f[i]);
+        }
+    };
 #pragma unroll
-        for (int i = 0; i < 2 * kMT; ++i) next[i] = __ldg(reinterpret_cast<const uint4 *>(cp[i] + (uint64_t)s2 * 64));
+    for (int d = 0; d < kMvDepth; ++d) fetch(warp + d * kMvWarps, code[d], fac[d]);
+
+    for (int s0 = warp; s0 < segs; s0 += kMvWarps * kMvDepth) {
 #pragma unroll
-        for (int gr = 0; gr < kGroups; ++gr) {
-            float a1[kMT][kNT][4], a2[kMT][kNT][4], xs[kNT][4];
+        for (int d = 0; d < kMvDepth; ++d) {
+            const int s = s0 + d * kMvWarps;
+            if (s >= segs) break;
+            uint4 bx[kNT][4];  // the segment's activations, word j of the lane
 #pragma unroll
-            for (int n = 0; n < kNT; ++n)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    xs[n][c] = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < kMT; ++i) a1[i][n][c] = a2[i][n][c] = 0.0f;
-                }
-#pragma unroll
-            for (int j = gr * kSteps; j < (gr + 1) * kSteps; ++j) {
-                uint32_t bx[kNT][4];
-                const uint64_t k = (uint64_t)s * 128 + j * 32 + t * 8;
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t k = (uint32_t)s * 128 + j * 32;  // (xp starts at the lane's own 8)
 #pragma unroll
                 for (int n = 0; n < kNT; ++n) {
-                    uint4 v = make_uint4(0, 0, 0, 0);
+                    bx[n][j] = make_uint4(0, 0, 0, 0);
                     if (kVec) {
-                        if (xin[n] && k < w.cols) v = __ldg(reinterpret_cast<const uint4 *>(xp[n] + k));
+                        if (xin[n] && k + t * 8 < w.cols) bx[n][j] = __ldg(reinterpret_cast<const uint4 *>(xp[n] + k));
                     } else if (xin[n]) {
-                        uint16_t e[8];
+                        uint32_t e[8];
 #pragma unroll
                         for (int i = 0; i < 8; ++i)
-                            e[i] = k + i < w.cols ? reinterpret_cast<const uint16_t *>(xp[n])[k + i] : uint16_t(0);
-                        v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
-                    }
-                    bx[n][0] = v.x, bx[n][1] = v.y, bx[n][2] = v.z, bx[n][3] = v.w;
-                    constexpr uint32_t one = kHalf ? 0x3c003c00u : 0x3f803f80u;
-                    mma16816<T>(xs[n], one, one, one, one, v.x, v.y);
-                    mma16816<T>(xs[n], one, one, one, one, v.z, v.w);
-                }
-#pragma unroll
-                for (int i = 0; i < kMT; ++i) {
-                    const uint32_t u = j == 0 ? code[2 * i].x : j == 1 ? code[2 * i].y : j == 2 ? code[2 * i].z : code[2 * i].w;
-                    const uint32_t v = j == 0   ? code[2 * i + 1].x
-                                       : j == 1 ? code[2 * i + 1].y
-                                       : j == 2 ? code[2 * i + 1].z
-                                                : code[2 * i + 1].w;
-                    const uint32_t u8 = u >> 8, v8 = v >> 8;
-                    uint32_t f[8];
-                    if constexpr (kHalf) {
-                        f[0] = u & 0x000f000fu, f[1] = v & 0x000f000fu, f[2] = u8 & 0x000f000fu, f[3] = v8 & 0x000f000fu;
-                        f[4] = u & 0x00f000f0u, f[5] = v & 0x00f000f0u, f[6] = u8 & 0x00f000f0u, f[7] = v8 & 0x00f000f0u;
-                    } else {
-                        f[0] = (u & 0x000f000fu) | 0x43004300u, f[1] = (v & 0x000f000fu) | 0x43004300u;
-                        f[2] = (u8 & 0x000f000fu) | 0x43004300u, f[3] = (v8 & 0x000f000fu) | 0x43004300u;
-                        f[4] = ((u >> 4) & 0x000f000fu) | 0x43004300u, f[5] = ((v >> 4) & 0x000f000fu) | 0x43004300u;
-                        f[6] = ((u >> 12) & 0x000f000fu) | 0x43004300u, f[7] = ((v >> 12) & 0x000f000fu) | 0x43004300u;
-                    }
-#pragma unroll
-                    for (int n = 0; n < kNT; ++n) {
-                        mma16816<T>(a1[i][n], f[0], f[1], f[2], f[3], bx[n][0], bx[n][1]);
-                        mma16816<T>(kHalf ? a2[i][n] : a1[i][n], f[4], f[5], f[6], f[7], bx[n][2], bx[n][3]);
+                            e[i] = k + t * 8 + i < w.cols ? reinterpret_cast<const uint16_t *>(xp[n])[k + i] : 0;
+                        bx[n][j] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
                     }
                 }
             }
 #pragma unroll
-            for (int i = 0; i < kMT; ++i) {
-                float2 f0 = __half22float2(__ldg(mp[2 * i] + (uint64_t)s * kGroups + gr));
-                float2 f1 = __half22float2(__ldg(mp[2 * i + 1] + (uint64_t)s * kGroups + gr));
-                if constexpr (kHalf) {  // 2^24 of the subnormal codes
-                    f0.x *= 16777216.0f, f1.x *= 16777216.0f;
-                } else {  // the 128 of 128 + c
-                    f0.y = fmaf(-128.0f, f0.x, f0.y), f1.y = fmaf(-128.0f, f1.x, f1.y);
-                }
+            for (int gr = 0; gr < kGroups; ++gr) {
+                float a1[kMT][kNT][4], a2[kMT][kNT][4], xs[kNT][4];
 #pragma unroll
                 for (int n = 0; n < kNT; ++n)
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        const float2 f = c < 2 ? f0 : f1;
-                        const float sum = kHalf ? fmaf(a2[i][n][c], 0.0625f, a1[i][n][c]) : a1[i][n][c];
-                        y[i][n][c] = fmaf(f.x, sum, fmaf(f.y, xs[n][c], y[i][n][c]));
-                    }
-            }
-        }
+                        xs[n][c] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 2 * kMT; ++i) code[i] = next[i];
+                        for (int i = 0; i < kMT; ++i) a1[i][n][c] = a2[i][n][c] = 0.0f;
+                    }
+#pragma unroll
+                for (int j = gr * kSteps; j < (gr + 1) * kSteps; ++j) {
+                    constexpr uint32_t one = kHalf ? 0x3c003c00u : 0x3f803f80u;
+#pragma unroll
+                    for (int n = 0; n < kNT; ++n) {
+                        mma16816<T>(xs[n], one, one, one, one, bx[n][j].x, bx[n][j].y);
+                        mma16816<T>(xs[n], one, one, one, one, bx[n][j].z, bx[n][j].w);
+                    }
+#pragma unroll
+                    for (int i = 0; i < kMT; ++i) {
+                        const uint4 &cu = code[d][2 * i], &cv = code[d][2 * i + 1];
+                        const uint32_t u = j == 0 ? cu.x : j == 1 ? cu.y : j == 2 ? cu.z : cu.w;
+                        const uint32_t v = j == 0 ? cv.x : j == 1 ? cv.y : j == 2 ? cv.z : cv.w;
+                        const uint32_t u8 = u >> 8, v8 = v >> 8;
+                        uint32_t f[8];
+                        if constexpr (kHalf) {
+                            f[0] = u & 0x000f000fu, f[1] = v & 0x000f000fu, f[2] = u8 & 0x000f000fu, f[3] = v8 & 0x000f000fu;
+                            f[4] = u & 0x00f000f0u, f[5] = v & 0x00f000f0u, f[6] = u8 & 0x00f000f0u, f[7] = v8 & 0x00f000f0u;
+                        } else {
+                            f[0] = (u & 0x000f000fu) | 0x43004300u, f[1] = (v & 0x000f000fu) | 0x43004300u;
+                            f[2] = (u8 & 0x000f000fu) | 0x43004300u, f[3] = (v8 & 0x000f000fu) | 0x43004300u;
+                            f[4] = ((u >> 4) & 0x000f000fu) | 0x43004300u, f[5] = ((v >> 4) & 0x000f000fu) | 0x43004300u;
+                            f[6] = ((u >> 12) & 0x000f000fu) | 0x43004300u, f[7] = ((v >> 12) & 0x000f000fu) | 0x43004300u;
+                        }
+#pragma unroll
+                        for (int n = 0; n < kNT; ++n) {
+                            mma16816<T>(a1[i][n], f[0], f[1], f[2], f[3], bx[n][j].x, bx[n][j].y);
+                            mma16816<T>(kHalf ? a2[i][n] : a1[i][n], f[4], f[5], f[6], f[7], bx[n][j].z, bx[n][j].w);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < kMT; ++i) {
+                    float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&fac[d][2 * i][gr]));
+                    float2 f1 = __half22float2(*reinterpret_cast<const __half2 *>(&fac[d][2 * i + 1][gr]));
+                    if constexpr (kHalf) {  // 2^24 of the subnormal codes
+                        f0.x *= 16777216.0f, f1.x *= 16777216.0f;
+                    } else {  // the 128 of 128 + c
+                        f0.y = fmaf(-128.0f, f0.x, f0.y), f1.y = fmaf(-128.0f, f1.x, f1.y);
+                    }
+#pragma unroll
+                    for (int n = 0; n < kNT; ++n)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const float2 f = c < 2 ? f0 : f1;
+                            const float sum = kHalf ? fmaf(a2[i][n][c], 0.0625f, a1[i][n][c]) : a1[i][n][c];
+                            y[i][n][c] = fmaf(f.x, sum, fmaf(f.y, xs[n][c], y[i][n][c]));
+                        }
+                }
+            }
+            fetch(s + kMvWarps * kMvDepth, code[d], fac[d]);
+        }
     }
 
     // the warps' column shares, added in warp order

@@ -108,11 +108,14 @@ void append(const cora_kv4_cache *c, const cora_kv4_append_args *a, cudaStream_t
 
 // ---- attend ------------------------------------------------------------------------------
 
-// Rows of one key head and sequence: few go to the streaming kernel, more to the tile kernel.
+// Rows of one key head and sequence. Up to 32 the streaming kernel takes tiles of 8, reading the
+// cache again for each (from L2); more go to the tile kernel. Both measured, 16 sequences of 4096
+// tokens, 8 key heads, in us at 8 / 16 / 32 / 64 rows: head size 128, streaming 39 / 55 / 91 / 160,
+// tiles 102 / 102 / 104 / 105; head size 256, 55 / 84 / 145 / 264 against 170 / 172 / 173 / 175.
 uint64_t attend_rows(const cora_kv4_cache &c, uint64_t q_heads, uint64_t max_queries) {
     return std::max<uint64_t>(1, max_queries) * (q_heads / c.kv_heads);
 }
-constexpr uint64_t kFewRows = kAtRows;
+constexpr uint64_t kFewRows = 32;
 uint64_t attend_counters() { return ((uint64_t)sm_count() * 2 * 4 + 255) / 256 * 256; }
 // Workspace: the arrival counters first (they are the part that has to start at zero), then two
 // partial results per block.
@@ -195,6 +198,10 @@ void attend(const cora_kv4_cache *c, const cora_kv4_attend_args *a, cudaStream_t
 
 // ---- matvec ------------------------------------------------------------------------------
 
+// 32 weight rows per warp halve what is done once per activation (its loads, its sums); 16 give
+// twice the blocks, which matrices with fewer rows than fill the SMs twice need more.
+constexpr uint64_t kWideRows = 32 * 2 * 148;
+
 template <typename T, int kGroup, int kMT, int kNT, bool kVec>
 void launch_matvec(const cora_w4_weight &w, const cora_w4_matvec_args &a, cudaStream_t st) {
     const uint64_t bx = (w.rows + 16 * kMT - 1) / (16 * kMT), by = (a.rows + 8 * kNT - 1) / (8 * kNT);
@@ -218,9 +225,14 @@ void matvec(const cora_w4_weight *w, const cora_w4_matvec_args *a, cudaStream_t 
         using T = decltype(z);
         auto go = [&](auto gr) {
             constexpr int G = decltype(gr)::value;
-            if (a->rows <= 8) vec ? launch_matvec<T, G, 1, 1, true>(*w, *a, st) : launch_matvec<T, G, 1, 1, false>(*w, *a, st);
-            else if (a->rows <= 16) vec ? launch_matvec<T, G, 1, 2, true>(*w, *a, st) : launch_matvec<T, G, 1, 2, false>(*w, *a, st);
-            else vec ? launch_matvec<T, G, 1, 4, true>(*w, *a, st) : launch_matvec<T, G, 1, 4, false>(*w, *a, st);
+            auto wide = [&](auto nt, auto mt) {
+                constexpr int NT = decltype(nt)::value, MT = decltype(mt)::value;
+                vec ? launch_matvec<T, G, MT, NT, true>(*w, *a, st) : launch_matvec<T, G, MT, NT, false>(*w, *a, st);
+            };
+            const bool two = w->rows >= kWideRows;
+            if (a->rows <= 8) two ? wide(Int<1>{}, Int<2>{}) : wide(Int<1>{}, Int<1>{});
+            else if (a->rows <= 16) two ? wide(Int<2>{}, Int<2>{}) : wide(Int<2>{}, Int<1>{});
+            else wide(Int<4>{}, Int<1>{});
         };
         if (w->group == 32) go(Int<32>{});
         else if (w->group == 64) go(Int<64>{});

@@ -103,36 +103,52 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(const void *p) {
            (2ull << 61);
 }
 
+// Descriptors of 128-byte swizzled tiles by their low word (the high one, 8-row atoms 1024 bytes
+// apart and the layout, is a constant): 32-bit arithmetic, so that the issuing thread keeps them
+// in few registers. Advancing by `n` bytes adds n / 16.
+constexpr uint32_t kDescHigh = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_low(uint32_t smem, uint32_t block = 16) {
+    return ((smem & 0x3FFFFu) >> 4) | (block >> 4) << 16;
+}
+// One lane of a converged warp. The warp runs the whole issuing loop and only the instructions
+// below are the leader's: operands then stay in uniform registers, where a branch to one lane
+// made the compiler move each of them there for every instruction.
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t r;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+    return r;
+}
 // D[tmem] (+)= A[smem] * B[smem], kind::f16 (A and B fp16), layouts by the descriptors.
-__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
-                                        uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_f16(uint32_t leader, uint32_t d_tmem, uint32_t a_low, uint32_t b_low, uint32_t idesc,
+                                        uint32_t accumulate) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "{\n .reg .pred p, q;\n .reg .b64 a, b;\n mov.b64 a, {%1, %5};\n mov.b64 b, {%2, %5};\n setp.ne.b32 p, %4, 0;\n"
+        " setp.ne.b32 q, %6, 0;\n @q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n}\n" ::"r"(d_tmem),
+        "r"(a_low), "r"(b_low), "r"(idesc), "r"(accumulate), "n"(kDescHigh), "r"(leader)
         : "memory");
 }
 // The same with A in TMEM: row = lane, two fp16 per 32-bit column.
-__device__ __forceinline__ void mma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
-                                           uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_f16_ta(uint32_t leader, uint32_t d_tmem, uint32_t a_tmem, uint32_t b_low, uint32_t idesc,
+                                           uint32_t accumulate) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "{\n .reg .pred p, q;\n .reg .b64 b;\n mov.b64 b, {%2, %5};\n setp.ne.b32 p, %4, 0;\n"
+        " setp.ne.b32 q, %6, 0;\n @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "r"(b_low), "r"(idesc), "r"(accumulate), "n"(kDescHigh), "r"(leader)
+        : "memory");
+}
+// mma_commit by the leader.
+__device__ __forceinline__ void mma_commit_by(uint32_t leader, uint64_t *bar) {
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar)),
+        "r"(leader)
         : "memory");
 }
 // Instruction descriptor: fp32 accumulator, A and B fp16, M x N, A K-major, B K-major or (b_mn)
-// N-major.
+// N-major: rows of 128 bytes then hold 64 columns of N for one k, blocks of 64 columns are `block`
+// bytes apart.
 __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool b_mn) {
     return (1u << 4) | (uint32_t(b_mn) << 16) | (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24);
-}
-// Shared-memory matrix descriptor of an N-major tile with 128-byte swizzle: rows of 128 bytes
-// hold 64 columns of N for one k, 8 rows of k per 1024-byte atom, blocks of 64 columns `block`
-// bytes apart.
-__device__ __forceinline__ uint64_t smem_desc_sw128_mn(const void *p, uint32_t block) {
-    const uint64_t addr = smem_u32(p);
-    return ((addr & 0x3FFFFull) >> 4) | (uint64_t(block >> 4) << 16) | (uint64_t(1024 >> 4) << 32) |
-           (1ull << 46) | (2ull << 61);
 }
 // 32 columns without the wait; tmem_wait_ld orders the uses of up to two such loads.
 __device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t (&r)[32]) {
