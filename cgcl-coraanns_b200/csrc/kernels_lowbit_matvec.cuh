@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(kMvWarps * 32, kNT >= 4 ? 1 : 2) w4_matvec_ker
                                                                                     const cora_w4_matvec_args p) {
     constexpr bool kHalf = std::is_same<T, __half>::value;
     constexpr int kGroups = 128 / kGroup, kSteps = kGroup / 32;
-    constexpr int kMvDepth = kNT >= 4 ? 2 : kMT == 2 ? 3 : 4;
+    constexpr int kMvDepth = kNT == 1 && kMT == 1 ? 3 : 2;
     extern __shared__ float mv_red[];  // [warp][row of x][weight row]
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
     const int n0 = blockIdx.x * 16 * kMT, m0 = blockIdx.y * 8 * kNT;

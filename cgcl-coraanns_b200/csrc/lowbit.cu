@@ -231,7 +231,7 @@ void matvec(const cora_w4_weight *w, const cora_w4_matvec_args *a, cudaStream_t 
             };
             const bool two = w->rows >= kWideRows;
             if (a->rows <= 8) two ? wide(Int<1>{}, Int<2>{}) : wide(Int<1>{}, Int<1>{});
-            else if (a->rows <= 16) two ? wide(Int<2>{}, Int<2>{}) : wide(Int<2>{}, Int<1>{});
+            else if (a->rows <= 16) wide(Int<2>{}, Int<1>{});
             else wide(Int<4>{}, Int<1>{});
         };
         if (w->group == 32) go(Int<32>{});
