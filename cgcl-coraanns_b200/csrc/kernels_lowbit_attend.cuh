@@ -40,14 +40,17 @@
 
 namespace cora {
 
-// One block per SM, of as many warps as leave a thread the registers it needs: spilled variables
-// would go past the little L1 that the ring leaves (they cost 10 of 40 us at 131072 tokens).
-constexpr int at_warps(int D) { return D == 256 ? 8 : 12; }
-constexpr int at_stages(int D) { return D == 256 ? 2 : 3; }  // tiles of a warp's ring
-constexpr int kAtTile = 32;
+// One block of 8 warps per SM: with 255 registers a thread nothing is spilled (spills would go
+// past the little L1 that the ring leaves) and a tile of 64 tokens gives each warp enough
+// independent work. Measured on 131072 tokens x 8 key heads / a ragged batch of 64: 16 warps x 32
+// tokens 57 / 100 us, 12 x 32 53 / 93 us, 9 x 64 58 / 97 us, 8 x 64 47 / 76 us.
+constexpr int at_warps(int D) { return 8; }
+// Tokens of a tile (two tiles per warp have to fit shared memory), and tiles of a warp's ring.
+constexpr int at_tile(int D) { return D == 256 ? 32 : 64; }
+constexpr int at_stages(int D) { return 2; }
 constexpr int kAtRows = 8;         // query rows of a job
 constexpr int kAtMinRun = 2;       // units of a warp, at least
-constexpr int kAtShort = 40;       // tiles of a job that one block takes whole
+constexpr int kAtShort = 1280;     // tokens of a job that one block takes whole, at most
 constexpr int kAtMaxSeqs = 512;    // sequences of one launch (their work is kept in smem)
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -67,7 +70,7 @@ constexpr int kAtPart = kAtRows * (D + 2);
 // The shared memory of a block, in order (each part a multiple of 16 bytes).
 template <int D, int kNG>
 struct AttendSmem {
-    static constexpr int kAtWarps = at_warps(D), kAtStages = at_stages(D);
+    static constexpr int kAtWarps = at_warps(D), kAtStages = at_stages(D), kAtTile = at_tile(D);
     static constexpr uint32_t kCodes = kAtTile * D / 2, kMeta = kAtTile * kNG * 4;
     static constexpr uint32_t kStage = 2 * kCodes + 2 * kMeta;
     static constexpr uint32_t kRing = kAtStages * kStage;   // of a warp; at the end its partial result
@@ -114,7 +117,7 @@ struct SeqWork {
     int len, first;   // cached tokens; first tile-aligned token that any query sees
     int tiles, row_tiles;
 };
-__device__ __forceinline__ SeqWork seq_work(const AttendParams &p, int b, int rows) {
+__device__ __forceinline__ SeqWork seq_work(const AttendParams &p, int b, int rows, int tile) {
     SeqWork s;
     const int seq = p.seq0 + b;
     int q0 = p.a.q_start ? __ldg(p.a.q_start + seq) : seq;
@@ -131,9 +134,9 @@ __device__ __forceinline__ SeqWork seq_work(const AttendParams &p, int b, int ro
     s.n = q1 - q0;
     s.len = len;
     const int w = (int)p.a.window;
-    s.first = w ? max(0, len - s.n - w + 1) / kAtTile * kAtTile : 0;
-    if (s.first > len) s.first = len / kAtTile * kAtTile;
-    s.tiles = max(1, (len - s.first + kAtTile - 1) / kAtTile);  // an empty one still writes zeros
+    s.first = w ? max(0, len - s.n - w + 1) / tile * tile : 0;
+    if (s.first > len) s.first = len / tile * tile;
+    s.tiles = max(1, (len - s.first + tile - 1) / tile);  // an empty one still writes zeros
     s.row_tiles = (s.n * (int)(p.a.q_heads / p.c.kv_heads) + rows - 1) / rows;
     return s;
 }
@@ -141,7 +144,8 @@ __device__ __forceinline__ SeqWork seq_work(const AttendParams &p, int b, int ro
 template <typename T, int D, int kNG>
 __global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const AttendParams p) {
     using S = AttendSmem<D, kNG>;
-    constexpr int kAtWarps = at_warps(D), kAtThreads = kAtWarps * 32, kAtStages = at_stages(D);
+    constexpr int kAtWarps = at_warps(D), kAtThreads = kAtWarps * 32, kAtStages = at_stages(D), kAtTile = at_tile(D);
+    constexpr int kMt = kAtTile / 16;
     constexpr int kG = D / kNG, kWords = kG / 32;  // words of one lane and group
     constexpr int kVB = D / 64;                    // 64-dimension blocks of the values
     extern __shared__ __align__(128) unsigned char at_smem[];
@@ -164,7 +168,7 @@ __global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const A
         fence_barrier_init();
     }
     for (int b = threadIdx.x; b < (int)p.seqs; b += kAtThreads) {
-        const SeqWork s = seq_work(p, b, kAtRows);
+        const SeqWork s = seq_work(p, b, kAtRows, kAtTile);
         work[b] = make_int4(s.q0, s.n, s.len, s.first);
     }
     __syncthreads();
@@ -200,7 +204,7 @@ __global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const A
             jobs += j;
         }
         longest = __reduce_max_sync(0xffffffffu, longest);
-        if (lane == 0) misc[2] = longest <= kAtShort && jobs <= gridDim.x ? (int)jobs : 0;
+        if (lane == 0) misc[2] = (int64_t)longest * kAtTile <= kAtShort && jobs <= gridDim.x ? (int)jobs : 0;
     }
     __syncthreads();
     const int64_t units = base[p.seqs];
@@ -444,16 +448,16 @@ __global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const A
         }
 
         {
-            // ---- a tile: scores of two times 16 tokens x 8 rows ----
+            // ---- a tile: scores of 16 tokens x 8 rows at a time ----
             const int tok0 = sw.first + tile * kAtTile;
             if (pending) {  // (0 only after a wait ran out: nothing more is fetched then)
                 alive = __all_sync(0xffffffffu, mbar_wait_short(bars + stage, phase, p.c.status)) && alive;
                 --pending;
             }
             const unsigned char *st = ring + stage * S::kStage;
-            float s[2][4];
+            float s[kMt][4];
 #pragma unroll
-            for (int mt = 0; mt < 2; ++mt) {
+            for (int mt = 0; mt < kMt; ++mt) {
 #pragma unroll
                 for (int gr = 0; gr < kNG; ++gr) {
                     uint32_t wa[kWords], wb[kWords];
@@ -485,16 +489,16 @@ __global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const A
                 }
             }
             const uint32_t *vm = reinterpret_cast<const uint32_t *>(st + 2 * S::kCodes + S::kMeta);
-            uint32_t vf[2][2][kNG];  // the tokens' value factors
+            uint32_t vf[kMt][2][kNG];  // the tokens' value factors
 #pragma unroll
-            for (int mt = 0; mt < 2; ++mt)
+            for (int mt = 0; mt < kMt; ++mt)
 #pragma unroll
                 for (int r = 0; r < 2; ++r)
 #pragma unroll
                     for (int gr = 0; gr < kNG; ++gr) vf[mt][r][gr] = vm[(mt * 16 + tg + r * 8) * kNG + gr];
             if (tok0 + kAtTile > hi_min || tok0 < lo_max) {  // some row does not see some token
 #pragma unroll
-                for (int mt = 0; mt < 2; ++mt)
+                for (int mt = 0; mt < kMt; ++mt)
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
                         const int tok = tok0 + mt * 16 + tg + r * 8;
@@ -510,7 +514,7 @@ __global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const A
             // ---- maxima, bound of the value scales: the rare way out of the tile's course ----
             __half2 most = __half2half2(__ushort_as_half(0));
 #pragma unroll
-            for (int mt = 0; mt < 2; ++mt)
+            for (int mt = 0; mt < kMt; ++mt)
 #pragma unroll
                 for (int r = 0; r < 2; ++r)
 #pragma unroll
@@ -518,12 +522,16 @@ __global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const A
             const float2 mf = __half22float2(most);
             bool out_of_course = !(mf.x <= vbound) || !(mf.y <= 65504.0f);
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
-                out_of_course |= fmaxf(fmaxf(s[0][c], s[0][c + 2]), fmaxf(s[1][c], s[1][c + 2])) > over[c];
+            for (int c = 0; c < 2; ++c) {
+                float m = fmaxf(s[0][c], s[0][c + 2]);
+#pragma unroll
+                for (int mt = 1; mt < kMt; ++mt) m = fmaxf(m, fmaxf(s[mt][c], s[mt][c + 2]));
+                out_of_course |= m > over[c];
+            }
             if (__any_sync(0xffffffffu, out_of_course)) {
                 float smax = 0.0f;
 #pragma unroll
-                for (int mt = 0; mt < 2; ++mt)
+                for (int mt = 0; mt < kMt; ++mt)
 #pragma unroll
                     for (int r = 0; r < 2; ++r)
 #pragma unroll
@@ -549,7 +557,9 @@ __global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const A
                 }
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    float m = fmaxf(fmaxf(s[0][c], s[0][c + 2]), fmaxf(s[1][c], s[1][c + 2]));
+                    float m = fmaxf(s[0][c], s[0][c + 2]);
+#pragma unroll
+                    for (int mt = 1; mt < kMt; ++mt) m = fmaxf(m, fmaxf(s[mt][c], s[mt][c + 2]));
                     m = max_over_g(m) + ref[c];
                     const bool grew = m > mx[c] + (mx[c] == -INFINITY ? 0.0f : 8.0f);
                     const float k = grew ? ex2(mx[c] - m) : 1.0f, f = k * shrink;
@@ -557,7 +567,7 @@ __global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const A
                         const float shift = ref[c] - m;
                         mx[c] = ref[c] = m, over[c] = 8.0f;
 #pragma unroll
-                        for (int mt = 0; mt < 2; ++mt) s[mt][c] += shift, s[mt][c + 2] += shift;
+                        for (int mt = 0; mt < kMt; ++mt) s[mt][c] += shift, s[mt][c + 2] += shift;
                     }
                     ls[c] *= k;
 #pragma unroll
@@ -570,7 +580,7 @@ __global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const A
             }
             // ---- values: per 16 tokens, p scale' transposed into the 16-deep operand ----
 #pragma unroll
-            for (int mt = 0; mt < 2; ++mt) {
+            for (int mt = 0; mt < kMt; ++mt) {
                 uint32_t pb[kNG][2];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {

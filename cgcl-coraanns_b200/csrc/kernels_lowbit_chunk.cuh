@@ -119,7 +119,7 @@ struct Walker {
                 else lo = mid + 1;
             }
             b = lo;
-            s = seq_work(p, b, kRows);
+            s = seq_work(p, b, kRows, kTN);
         }
         const int64_t per_head = (base[b + 1] - base[b]) / p.c.kv_heads, r = u - base[b];
         g.s = s;
@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
         if (lane == 0) base[0] = 0;
         for (int b0 = 0; b0 < (int)p.seqs; b0 += 32) {
             int64_t v = 0;
-            if (b0 + lane < (int)p.seqs) v = Walk::units_of_head(p, seq_work(p, b0 + lane, kRows)) * H;
+            if (b0 + lane < (int)p.seqs) v = Walk::units_of_head(p, seq_work(p, b0 + lane, kRows, kTN)) * H;
 #pragma unroll
             for (int off = 1; off < 32; off <<= 1) {
                 const int64_t o = __shfl_up_sync(0xffffffffu, v, off);

@@ -110,8 +110,8 @@ void append(const cora_kv4_cache *c, const cora_kv4_append_args *a, cudaStream_t
 
 // Rows of one key head and sequence. Up to 32 the streaming kernel takes tiles of 8, reading the
 // cache again for each (from L2); more go to the tile kernel. Both measured, 16 sequences of 4096
-// tokens, 8 key heads, in us at 8 / 16 / 32 / 64 rows: head size 128, streaming 39 / 55 / 91 / 160,
-// tiles 102 / 102 / 104 / 105; head size 256, 55 / 84 / 145 / 264 against 170 / 172 / 173 / 175.
+// tokens, 8 key heads, in us at 8 / 16 / 32 / 64 rows: head size 128, streaming 35 / 51 / 80 / 160,
+// tiles 102 / 102 / 104 / 104; head size 256, 55 / 84 / 145 / 264 against 170 / 172 / 173 / 175.
 uint64_t attend_rows(const cora_kv4_cache &c, uint64_t q_heads, uint64_t max_queries) {
     return std::max<uint64_t>(1, max_queries) * (q_heads / c.kv_heads);
 }
@@ -174,6 +174,10 @@ void attend(const cora_kv4_cache *c, const cora_kv4_attend_args *a, cudaStream_t
     const uint64_t rows = attend_rows(*c, a->q_heads, a->max_queries);
     need(a->workspace && aligned16(a->workspace) && a->workspace_bytes >= attend_workspace(*c, rows),
          "the workspace is smaller than cora_kv4_attend_workspace()");
+    // units (token tiles x row tiles x key heads) of a sequence are counted in 32 bits
+    const double tiles = (double)a->table_width * c->page_size / 32 + 2;
+    const double row_tiles = (double)a->q_tokens * (a->q_heads / c->kv_heads) / kAtRows + 1;
+    need(tiles * row_tiles * c->kv_heads < 4.0e9, "too much work for one call: split the queries");
     AttendParams p{};
     p.c = *c;
     p.a = *a;
