@@ -538,3 +538,19 @@ def test_refusals(lb):
         with pytest.raises(InvalidArgument):
             f()
     cache.check()
+
+
+# ---- together ------------------------------------------------------------------------------
+
+
+def test_reader_example_searches_and_reads():
+    """The example's decoder agrees with plain torch on the same 4-bit values: activations are
+    rounded to bf16 (2^-8) some 8 times per layer on the way to the logits, so 10 % is far above
+    what two layers leave, and far below what a wrong operator gives."""
+    import importlib.util
+    from conftest import ROOT
+    spec = importlib.util.spec_from_file_location("reader", ROOT / "cgcl-coraanns_b200" / "apps" / "reader.py")
+    reader = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(reader)
+    ids, off = reader.main(["--passages", "600", "--tokens", "5"])
+    assert ids[0] == 17 and off < 0.1
