@@ -69,9 +69,11 @@ def _library():
     return _bound
 
 
-try:  # the current stream's handle without a Stream object around it
-    from torch._C import _cuda_getCurrentRawStream as _stream
+try:  # the current stream's handle without a Stream object around it, the current device
+    from torch._C import _cuda_getCurrentRawStream as _stream, _cuda_getDevice as _current_device
 except ImportError:
+    _current_device = torch.cuda.current_device
+
     def _stream(index):
         return torch.cuda.current_stream(index).cuda_stream
 
@@ -87,7 +89,7 @@ def _need(ok, what):
 
 def _call(f, index, *args):
     """f(*args, stream) on device `index` and its current stream."""
-    if index == torch.cuda.current_device():
+    if index == _current_device():
         rc = f(*args, _stream(index))
     else:
         with torch.cuda.device(index):
@@ -97,7 +99,7 @@ def _call(f, index, *args):
 
 
 def _index(t, what, dtype, shape, device):
-    if t.dtype is not dtype or t.shape != shape or t.device != device or not t.is_contiguous():
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != device.index or not t.is_contiguous():
         _refuse(f"{what} must be a contiguous {dtype} tensor of shape {shape} on {device}")
     return t.data_ptr()
 
@@ -158,7 +160,7 @@ class Cache4:
 
     def _heads(self, x, what, shape):
         """The type code of a (tokens, heads, head_dim) tensor."""
-        if x.shape != shape or x.device != self.device or x.stride(2) != 1:
+        if x.shape != shape or x.get_device() != self._dev or x.stride(2) != 1:
             _refuse(f"{what} must be {shape} on {self.device}, its last stride 1")
         return _DTYPES.get(x.dtype, 99)
 
@@ -224,7 +226,7 @@ class Cache4:
         dt = self._heads(q, "q", (T, Hq, self.head_dim))
         B, width = page_table.shape
         stride, last = page_table.stride()
-        if page_table.dtype is not torch.int32 or page_table.device != dev or last != 1:
+        if page_table.dtype is not torch.int32 or page_table.get_device() != self._dev or last != 1:
             _refuse(f"page_table must be int32 (sequences, width) on {dev}")
         if window < 0 or max_queries < 1:
             _refuse("window must not be negative, max_queries must be positive")
@@ -326,7 +328,7 @@ def matvec(x: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = None
     """x (..., cols) times the 4-bit weight, plus bias: (..., rows) in x's type. Meant for the few
     rows of decoding (1 to 64); more are correct, 32 rows at a time."""
     dev, N, dims = weight.device, weight.rows, x.dim()
-    if not dims or x.shape[-1] != weight.cols or x.device != dev or x.stride(-1) != 1:
+    if not dims or x.shape[-1] != weight.cols or x.get_device() != weight._dev or x.stride(-1) != 1:
         _refuse(f"x must be (..., {weight.cols}) on {dev}, its last stride 1")
     x2 = x if dims == 2 else x.reshape(-1, weight.cols)
     M = x2.shape[0]
