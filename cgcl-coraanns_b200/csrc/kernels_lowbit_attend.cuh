@@ -10,7 +10,7 @@
 //    side: the query heads that share a key head fill one instruction;
 //  - a code becomes an fp16 operand by one AND: nibble 0 of a 16-bit half is the subnormal
 //    c 2^-24, nibble 1 is c 2^-20, both exact in the tensor core. The powers of two go into q
-//    (a common power of two per block, so fp16 holds every bit of a bf16 or fp16 q that is
+//    (a common power of two per job, so fp16 holds every bit of a bf16 or fp16 q that is
 //    within 2^-24 of the largest) and into the final scaling of the output;
 //  - w = fp16(p scale') is the operand of the second product (11 bits; scaled by a power of two
 //    that follows the largest scale' met, so it uses the normal range). What the rounding of w
@@ -30,6 +30,8 @@
 //    A job inside one run is written by its warp; one cut over the warps of a block is joined in
 //    shared memory; one cut over blocks by the last block to arrive, from partial results in
 //    the workspace. Where all jobs are short, each block takes one instead (no join over blocks).
+// Measured, 8 key heads of 128: 131072 tokens 47 us (3.0 TB/s over the call, near 5 in the stream),
+// 64 ragged sequences of 200 to 16384 tokens in two groups 76 us (2.8 TB/s).
 #pragma once
 #include <cuda_fp16.h>
 

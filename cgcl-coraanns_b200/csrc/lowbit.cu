@@ -149,6 +149,13 @@ void launch_chunk(AttendParams p, cudaStream_t st) {
     using S = ChunkSmem<D, kNG, kNQ>;
     static_assert(S::bytes(kAtMaxSeqs) <= 232448, "");
     static int seen[64] = {};
+    static const int regs = [&] {
+        cudaFuncAttributes at{};
+        CUDA_TRY(cudaFuncGetAttributes(&at, kern));
+        return at.numRegs;
+    }();
+    // The roles' shares are drawn from what the block is launched with; with less they would wait.
+    if (regs < 96) fail(CORA_ERUNTIME, "kv4_chunk_kernel was compiled to fewer registers than its roles share");
     allow_smem(kern, S::bytes(kAtMaxSeqs), seen);
     const uint32_t seqs = p.a.seqs;
     for (uint32_t s0 = 0; s0 < seqs; s0 += kAtMaxSeqs) {
@@ -203,7 +210,8 @@ void attend(const cora_kv4_cache *c, const cora_kv4_attend_args *a, cudaStream_t
 // ---- matvec ------------------------------------------------------------------------------
 
 // 32 weight rows per warp halve what is done once per activation (its loads, its sums); 16 give
-// twice the blocks, which matrices with fewer rows than fill the SMs twice need more.
+// twice the blocks, which matrices with fewer rows than fill the SMs twice need more. 32768 x 8192,
+// one row: 39 us with 32, 43 us with 16; 10007 x 5000, 13 rows: 27 us with 32 (spills), 20 with 16.
 constexpr uint64_t kWideRows = 32 * 2 * 148;
 
 template <typename T, int kGroup, int kMT, int kNT, bool kVec>

@@ -366,7 +366,7 @@ int cora_kv4_append(const cora_kv4_cache *cache, const cora_kv4_append_args *arg
  * contiguous. max_queries: an upper bound on the query tokens of a sequence.
  * workspace: cora_kv4_attend_workspace() bytes for this q_heads and max_queries, zero before its
  * first use; left ready for the next call (of any shape it is large enough for). Calls that
- * overlap in time need workspaces of their own. With more than 8 rows (query tokens x heads of a
+ * overlap in time need workspaces of their own. With more than 32 rows (query tokens x heads of a
  * group) per key head, cached values are rounded to fp16 (past 65504 they become infinite). */
 typedef struct {
     const void *q;
