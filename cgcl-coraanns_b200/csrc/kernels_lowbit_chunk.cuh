@@ -16,13 +16,16 @@
 //             stay below 2^8, which fp16 holds.
 //   8-15      unpack, into 128-byte swizzled tiles: key codes as the fp16 subnormals c 2^-24 and
 //             c 2^-20, exact (the scores keep fp32 accuracy); value codes to fp16 scale c + low,
-//             one rounding each (2^-12 of the value, as of the probability; values past 65504
-//             do not fit).
+//             one rounding each (2^-12 of the value, as of the probability). The format goes up to
+//             16 x 65504: from a tile that holds a value past 65504 on, a stretch's values are
+//             unpacked under 2^-5 (values below 2^-9 then keep an absolute 2^-20) and the sums follow.
 //   16        copies code tiles from the cache's pages (bulk copies into a ring).
 //   17        issues the tcgen05 products: S_g = Q_g C_g^T per factor group (keys K-major) and
 //             O += P V (P in TMEM, values as stored, token-major: the N-major operand). The whole
 //             warp runs the loop; from a branch to one lane the issue itself was the bound
-//             (802 against 730 us). Warps 18 and 19 are idle.
+//             (802 against 730 us).
+//   18        looks for values past 65504 in a copied tile's factors before it is unpacked (by the
+//             unpacking warps themselves it cost 80 cycles a tile). Warp 19 is idle.
 // Units (sequence, key head, row tile, token tile) are cut into equal runs, one per block; a job
 // cut over blocks is joined by the last to arrive. Every wait is bounded.
 //
@@ -73,8 +76,14 @@ struct ChunkSmem {
     static constexpr uint32_t poison = fac + kTables * 2 * kNG * kTN * 4;  // [kTables][4] bits: value is not finite
     static constexpr uint32_t misc = poison + kTables * 16;                   // tmem slot, last-to-arrive flags
     static constexpr uint32_t bars = misc + 32;
-    static constexpr uint32_t walk = bars + 288;                    // [warp] Walker
-    static constexpr uint32_t base = walk + 18 * 160;               // int64[seqs + 1]
+    static constexpr uint32_t kBarBytes = 304;
+    static constexpr uint32_t walk = bars + kBarBytes;              // [warp] Walker
+    // Marks of tiles whose values are under 2^-5. That of tile t is written once tile t - kRaw is
+    // unpacked, its values' slot thus free of tile t - kRaw - 2 (t - kRaw - 3 with 6 slots or, by the
+    // scores ahead, with 3), which softmax has then left: it reads marks from t - 5 on.
+    static constexpr int kLarge = 8;
+    static constexpr uint32_t large = walk + 19 * 160;              // [kLarge]
+    static constexpr uint32_t base = large + kLarge * 4;            // int64[seqs + 1]
     static constexpr size_t bytes(uint32_t seqs) { return 1024 + base + 8 * (size_t)(seqs + 1); }
 };
 
@@ -185,6 +194,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
     unsigned char *sm = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(ck_raw) + 1023) & ~uintptr_t(1023));
     float *fac = reinterpret_cast<float *>(sm + S::fac);
     volatile uint32_t *poison = reinterpret_cast<volatile uint32_t *>(sm + S::poison);
+    volatile uint32_t *large = reinterpret_cast<volatile uint32_t *>(sm + S::large);
     volatile uint32_t *misc = reinterpret_cast<volatile uint32_t *>(sm + S::misc);
     uint64_t *bars = reinterpret_cast<uint64_t *>(sm + S::bars);
     uint64_t *raw_full = bars, *raw_empty = raw_full + S::kRaw;
@@ -193,7 +203,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
     // (pv_done has a barrier per tile parity: a wait on one knows a phase by its parity alone, and
     // the softmax may be two second products ahead)
     uint64_t *s_full = o_free + 2, *p_full = s_full + 4, *pv_done = p_full + 4, *mma_done = pv_done + 4;
-    static_assert((2 * S::kRaw + 2 * S::kSlots + 17) * 8 <= 288, "");
+    uint64_t *looked = mma_done + 1;
+    static_assert((3 * S::kRaw + 2 * S::kSlots + 17) * 8 <= S::kBarBytes, "");
     int64_t *base = reinterpret_cast<int64_t *>(sm + S::base);
     int *err = p.c.status;
 
@@ -202,7 +213,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
     using Walk = Walker<kTN, kRows>;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < S::kRaw; ++i) mbar_init(raw_full + i, 1), mbar_init(raw_empty + i, 8);
+        for (int i = 0; i < S::kRaw; ++i) mbar_init(raw_full + i, 1), mbar_init(raw_empty + i, 8), mbar_init(looked + i, 1);
         for (int i = 0; i < S::kSlots; ++i) mbar_init(deq_full + i, 8), mbar_init(deq_empty + i, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(q_full + i, 4), mbar_init(o_free + i, 4);  // (an arrival per warp)
@@ -233,9 +244,9 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
     const uint32_t tmem = misc[0];
     const int64_t units = base[p.seqs], blocks = max((int64_t)1, min((int64_t)gridDim.x, units / kCkMinRun));
     static_assert(sizeof(Walk) <= 160, "");
-    Walk &walk = *reinterpret_cast<Walk *>(sm + S::walk + (warp < 18 ? warp : 0) * 160);
+    Walk &walk = *reinterpret_cast<Walk *>(sm + S::walk + (warp < 19 ? warp : 0) * 160);
     const Segment &g = walk.g;
-    if (lane == 0 && warp < 18) {
+    if (lane == 0 && warp < 19) {
         walk.u = blockIdx.x < blocks ? blockIdx.x * units / blocks : 0;
         walk.end = blockIdx.x < blocks ? (blockIdx.x + 1) * units / blocks : 0;
         walk.b = -1;
@@ -326,6 +337,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
             float fr[4], qr[4][kNG], m[4], over[4];  // unit of the scores; sums of q; maximum, room above it
             int lo[4], hi[4];                        // tokens that the row sees
             float2 l2[4];                            // sum of p, over even and odd columns
+            float unit = 1.0f;                       // of the sums of p v: 1, or 2^5 from a large tile on
             int hi_min = 0x7fffffff, lo_max = 0;
             {
                 // scale 0: scores 0, whatever the products are
@@ -346,6 +358,27 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
                     l2[k] = make_float2(0.0f, 0.0f);
                 }
             }
+            // The sums of p v so far, times a factor for each of the thread's rows.
+            auto rescale_o = [&](float k0, float k1, float k2, float k3) {
+                if (!__all_sync(0xffffffffu, mbar_wait_short(pv_done + 2 * q + ((tile_no - 1) & 1), (tile_no - 1) >> 1 & 1, err)))
+                    return false;
+                tc_fence_after();
+#pragma unroll 1
+                for (int d = 0; d < D; d += 32) {
+                    uint32_t x[16], y[16];
+                    tmem_ld_frag(t_o + d, x);
+                    tmem_ld_frag(t_o + d + (16u << 16), y);
+                    tmem_wait_frag(x, y);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        x[e] = __float_as_uint(__uint_as_float(x[e]) * (e & 2 ? k1 : k0));
+                        y[e] = __float_as_uint(__uint_as_float(y[e]) * (e & 2 ? k3 : k2));
+                    }
+                    tmem_st_frag(t_o + d, x);
+                    tmem_st_frag(t_o + d + (16u << 16), y);
+                }
+                return true;
+            };
             for (int j = 0; j < g.tiles && ok; ++j, ++tile_no) {
                 const int buf = q * kBufs + (int)(tile_no % kBufs);
                 const uint32_t sph = tile_no / kBufs & 1;
@@ -431,23 +464,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
                             }
                         }
                         if (j > 0) {
-                            ok = __all_sync(0xffffffffu, mbar_wait_short(pv_done + 2 * q + ((tile_no - 1) & 1), (tile_no - 1) >> 1 & 1, err));
+                            ok = rescale_o(kf[0], kf[1], kf[2], kf[3]);
                             if (!ok) break;
-                            tc_fence_after();
-#pragma unroll 1
-                            for (int d = 0; d < D; d += 32) {
-                                uint32_t x[16], y[16];
-                                tmem_ld_frag(t_o + d, x);
-                                tmem_ld_frag(t_o + d + (16u << 16), y);
-                                tmem_wait_frag(x, y);
-#pragma unroll
-                                for (int e = 0; e < 16; ++e) {
-                                    x[e] = __float_as_uint(__uint_as_float(x[e]) * kf[e >> 1 & 1]);
-                                    y[e] = __float_as_uint(__uint_as_float(y[e]) * kf[2 + (e >> 1 & 1)]);
-                                }
-                                tmem_st_frag(t_o + d, x);
-                                tmem_st_frag(t_o + d + (16u << 16), y);
-                            }
                         }
                         tmem_wait_st();
                     }
@@ -470,13 +488,19 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
                     }
                 }
                 if (!ok) break;
-                // values that are not finite are kept out of the product: rows that see one say so here
+                // values that are not finite are kept out of the product: rows that see one say so here;
+                // from the first large tile on the sums are under 2^-5
                 {
                     const volatile uint32_t *bits = poison + 4 * (tile_no % S::kTables);
-                    uint32_t any = 0;
+                    uint32_t any = large[tile_no % S::kLarge];
 #pragma unroll
                     for (int c = 0; c < kTN / 32; ++c) any |= bits[c];
                     if (any) {
+                        if (large[tile_no % S::kLarge] && unit == 1.0f) {
+                            unit = 32.0f;
+                            if (j > 0) ok = rescale_o(0.03125f, 0.03125f, 0.03125f, 0.03125f);
+                            if (!ok) break;
+                        }
                         for (int e = 0; e < kTN; ++e)
                             if (bits[e / 32] >> (e % 32) & 1) {
 #pragma unroll
@@ -510,7 +534,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
             const size_t sl = (size_t)(2 * blockIdx.x + (g.first ? 1 : 0)) * kNQ + q;
             float *po = p.part + sl * D * 128 + row;
             float2 *ps = reinterpret_cast<float2 *>(p.part + slots * D * 128) + sl * 128 + row;
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const float inv = l == 0.0f ? 0.0f : unit / l;
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
                 uint32_t x[32];
@@ -518,7 +542,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
                 tmem_wait_ld(x);
                 if (!whole) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) __stcg(po + (c + e) * 128, __uint_as_float(x[e]));
+                    for (int e = 0; e < 32; ++e) __stcg(po + (c + e) * 128, __uint_as_float(x[e]) * unit);
                 } else if (in) {
 #pragma unroll
                     for (int e = 0; e < 32; e += 8) {
@@ -592,9 +616,16 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
             for (int j = 0; j < g.tiles && ok; ++j, ++raw_no) {
                 const int rs = raw_no % S::kRaw, tok0 = g.tok0 + j * kTN;
                 const unsigned char *rw = sm + S::raw + rs * S::kRawBytes;
-                ok = mbar_wait_short(raw_full + rs, (raw_no / S::kRaw) & 1, err);
+                ok = mbar_wait_short(looked + rs, (raw_no / S::kRaw) & 1, err);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
+                // Value codes become k c (and lows k low), k = 1 or 2^-5: fma(1024 + c, k, -1024 k) and,
+                // from the odd nibbles, fma(1024 + 16 c, k / 16, -64 k), exact.
+                const bool big = large[raw_no % S::kLarge] != 0;
+                const __half2 k1 = __half2half2(__ushort_as_half(big ? 0x2800 : 0x3c00));
+                const __half2 k1024 = __half2half2(__ushort_as_half(big ? 0xd000 : 0xe400));
+                const __half2 k16 = __half2half2(__ushort_as_half(big ? 0x1800 : 0x2c00));
+                const __half2 k64 = __half2half2(__ushort_as_half(big ? 0xc000 : 0xd400));
 #pragma unroll
                 for (int kv = 0; kv < 2; ++kv, ++item) {
                     const int sl = item % S::kSlots;
@@ -647,20 +678,18 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
                             const bool bad = (fu & 0x7c00u) == 0x7c00u || (fu & 0x7c000000u) == 0x7c000000u;
                             // unseen tokens count as 0, and so do values that are marked above
                             if (tok < see_lo || tok >= see_hi || bad) f = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
-                            sc = __low2half2(f), lw = __high2half2(f);
+                            sc = __low2half2(f), lw = __hmul2(__high2half2(f), k1);
                         }
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             const uint32_t w = ws[k], w8 = w >> 8;
                             uint32_t o[4] = {w & 0x000f000fu, w & 0x00f000f0u, w8 & 0x000f000fu, w8 & 0x00f000f0u};
                             if (kv) {
-                                const __half2 k1024 = __half2half2(__ushort_as_half(0x6400)), k64 = __half2half2(__ushort_as_half(0xd400));
-                                const __half2 sixteenth = __half2half2(__ushort_as_half(0x2c00));
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) {
                                     o[e] |= 0x64006400u;  // 1024 + c or 1024 + 16 c
                                     __half2 v = *reinterpret_cast<__half2 *>(&o[e]);
-                                    v = e & 1 ? __hfma2(v, sixteenth, k64) : __hsub2(v, k1024);
+                                    v = e & 1 ? __hfma2(v, k16, k64) : __hfma2(v, k1, k1024);
                                     v = __hfma2(v, sc, lw);
                                     o[e] = *reinterpret_cast<uint32_t *>(&v);
                                 }
@@ -719,6 +748,34 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
         // the last copy into each stage has landed before the block exits
         for (uint32_t k = raw_no > S::kRaw ? raw_no - S::kRaw : 0; k < raw_no; ++k)
             mbar_wait_short(raw_full + k % S::kRaw, (k / S::kRaw) & 1, err);
+        } else if (warp == 18) {
+        // ---------------- values past 65504 ----------------
+        uint32_t raw_no = 0;
+        bool ok = true;
+        while (ok && next()) {
+            const int2 see = Walk::sees(p, g.s, g.row0 / kRows);
+            bool big = false;  // from the first such tile of a stretch on
+            for (int j = 0; j < g.tiles; ++j, ++raw_no) {
+                const int rs = raw_no % S::kRaw, tok0 = g.tok0 + j * kTN;
+                ok = __all_sync(0xffffffffu, mbar_wait_short(raw_full + rs, (raw_no / S::kRaw) & 1, err));
+                if (!ok) break;
+                const uint4 f4 = reinterpret_cast<const uint4 *>(sm + S::raw + rs * S::kRawBytes + 2 * S::kCodes + S::kMeta)[lane];
+                const uint32_t f[4] = {f4.x, f4.y, f4.z, f4.w};
+                bool past = false;  // some row sees it, its factors are finite, its largest value rounds to infinity
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&f[e]));
+                    const int tok = tok0 + (lane * 4 + e) / kNG;
+                    past |= tok >= see.x && tok < see.y && fabsf(v.x) <= 65504.0f && fabsf(v.y) <= 65504.0f &&
+                            fabsf(fmaf(15.0f, v.x, v.y)) >= 65520.0f;
+                }
+                big |= __any_sync(0xffffffffu, past) != 0;
+                if (lane == 0) {
+                    large[raw_no % S::kLarge] = big;
+                    mbar_arrive(looked + rs);
+                }
+            }
+        }
         } else if (warp == 17) {
         // ---------------- products ----------------
         constexpr uint32_t id_qk = idesc_f16(128, kTN, false), id_pv = idesc_f16(128, D, true);
