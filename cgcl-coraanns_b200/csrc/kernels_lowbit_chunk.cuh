@@ -12,8 +12,9 @@
 //             at a time (accumulator fragments), so that a factor it reads serves 4 rows: with a
 //             thread per row the factors alone took 2048 of 7200 cycles of shared memory a tile.
 //             One pass: probabilities refer to the maximum met before; only where it grows by more than
-//             2^8 are the sums (and the tile's earlier probabilities) rescaled, so that they
-//             stay below 2^8, which fp16 holds.
+//             2^8 are the sums (and the tile's earlier probabilities) rescaled. All are times 2^7, so
+//             that they stay below 2^15, which fp16 holds, and that of a token is off by at most
+//             2^-32 of the largest: a long tail of tiny ones keeps its share.
 //   8-15      unpack, into 128-byte swizzled tiles: key codes as the fp16 subnormals c 2^-24 and
 //             c 2^-20, exact (the scores keep fp32 accuracy); value codes to fp16 scale c + low,
 //             one rounding each (2^-12 of the value, as of the probability). The format goes up to
@@ -43,6 +44,7 @@ namespace cora {
 constexpr int kCkThreads = 640, kCkMinRun = 2;
 constexpr int kCkRegsSoftmax = 144, kCkRegsUnpack = 72, kCkRegsRest = 48;
 static_assert(256 * kCkRegsSoftmax + 256 * kCkRegsUnpack + 128 * kCkRegsRest <= kCkThreads * 96, "");
+constexpr float kCkShift = 7.0f;  // probabilities are 2^(score - m), m = maximum - kCkShift
 template <int kRegs>
 __device__ __forceinline__ void more_registers() {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
@@ -334,7 +336,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full + q);
             // From here a thread holds rows 8 k + lane / 4 of its warp, k = 0..3.
-            float fr[4], qr[4][kNG], m[4], over[4];  // unit of the scores; sums of q; maximum, room above it
+            float fr[4], qr[4][kNG], m[4], over[4];  // unit of the scores; sums of q; maximum - kCkShift, room above it
             int lo[4], hi[4];                        // tokens that the row sees
             float2 l2[4];                            // sum of p, over even and odd columns
             float unit = 1.0f;                       // of the sums of p v: 1, or 2^5 from a large tile on
@@ -441,8 +443,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
                             kf[k] = 1.0f;
                             if (tm[k] > over[k]) {
                                 const float to = tm[k] * fr[k];
-                                kf[k] = ex2(m[k] - to);
-                                m[k] = to;
+                                kf[k] = ex2(m[k] + kCkShift - to);
+                                m[k] = to - kCkShift;
                                 over[k] = tm[k] + 8.0f / fr[k];
                                 l2[k].x *= kf[k], l2[k].y *= kf[k];
                             }

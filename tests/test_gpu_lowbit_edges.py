@@ -51,3 +51,40 @@ def test_attend_values_past_fp16_cut_over_blocks(lb):
     v = torch.linspace(-65504, 65504, 128, device="cuda").to(torch.float16)[None, None].expand(2, 1, 128)
     cache.append(k, v, slots_of(cache, lens, seed, [11000, 29999]))
     check_attend(lb, cache, lens, 4, [10], "fp16", seed=seed)
+
+
+# ---- long flat tails --------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("per,n,L,H", [(4, 1, 16384, 1184), (4, 20, 16384, 148), (4, 40, 32768, 148), (2, 17, 65536, 148)])
+def test_attend_flat_tail_behind_a_sink(lb, per, n, L, H):
+    """One early token 17.7 nats above all others, its value 0: what remains of the output is the
+    sum of L tiny probabilities. As many key heads as give each block (streaming: warp) a whole
+    sequence, so that all its tokens are weighed against that one.
+
+    A probability is an fp16 operand times 2^7 relative to the maximum: below the normal range it
+    is off by half of 2^-24, that is 2^-32 of the maximum's, per token and unit of value (the
+    streaming kernel's operand p scale likewise, times half the range of a group). So L 2^-32
+    max |v| is added to the bound."""
+    D, page = 128, 64
+    one = lb.Cache4(L // page, 1, D, page_size=page)
+    gen = torch.Generator(device="cuda").manual_seed(L)
+    direction = torch.randn(D, generator=gen, device="cuda")
+    k = torch.zeros(L, 1, D, device="cuda")
+    v = 1.0 + 0.25 * torch.randn(L, 1, D, generator=gen, device="cuda")
+    k[5, 0] = direction * (17.7 / (direction.square().sum() * D ** -0.5))
+    v[5] = 0.0
+    one.append(k.to(torch.bfloat16), v.to(torch.bfloat16), torch.arange(L, device="cuda"))
+    cache = lb.Cache4.from_pool(one.pool.expand(-1, H, -1).contiguous(), page, D)
+    q = direction.expand(n, per * H, D).to(torch.bfloat16)
+    table = torch.arange(L // page, dtype=torch.int32, device="cuda")[None]
+    dl = torch.tensor([L], dtype=torch.int32, device="cuda")
+    qs = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    got, lse = cache.attend(q, table, dl, q_start=qs, max_queries=n, return_lse=True)
+    cache.check()
+    want, mass, wlse = attend64(one, q[:, :per], table.cpu().numpy(), [L], [0, n], True, 0, D ** -0.5)
+    bound = TOL_OUT["bf16"] * np.abs(want) + TOL_MASS * mass + L * 2.0 ** -32 * float(v.abs().max())
+    got, lse = (x.double().cpu().numpy() for x in (got.view(n, H, per, D), lse.view(n, H, per)))
+    for h in range(H):
+        assert (np.abs(got[:, h] - want) <= bound).all(), (h, (np.abs(got[:, h] - want) / bound).max())
+        assert np.abs(lse[:, h] - wlse).max() <= 2e-4
