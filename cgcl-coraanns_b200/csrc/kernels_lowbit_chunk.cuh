@@ -78,7 +78,7 @@ struct ChunkSmem {
     static constexpr uint32_t poison = fac + kTables * 2 * kNG * kTN * 4;  // [kTables][4] bits: value is not finite
     static constexpr uint32_t misc = poison + kTables * 16;                   // tmem slot, last-to-arrive flags
     static constexpr uint32_t bars = misc + 32;
-    static constexpr uint32_t kBarBytes = 304;
+    static constexpr uint32_t kBarBytes = 320;
     static constexpr uint32_t walk = bars + kBarBytes;              // [warp] Walker
     // Marks of tiles whose values are under 2^-5. That of tile t is written once tile t - kRaw is
     // unpacked, its values' slot thus free of tile t - kRaw - 2 (t - kRaw - 3 with 6 slots or, by the
@@ -205,8 +205,8 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
     // (pv_done has a barrier per tile parity: a wait on one knows a phase by its parity alone, and
     // the softmax may be two second products ahead)
     uint64_t *s_full = o_free + 2, *p_full = s_full + 4, *pv_done = p_full + 4, *mma_done = pv_done + 4;
-    uint64_t *looked = mma_done + 1;
-    static_assert((3 * S::kRaw + 2 * S::kSlots + 17) * 8 <= S::kBarBytes, "");
+    uint64_t *looked = mma_done + 1, *joined = looked + S::kRaw;
+    static_assert((3 * S::kRaw + 2 * S::kSlots + 19) * 8 <= S::kBarBytes, "");
     int64_t *base = reinterpret_cast<int64_t *>(sm + S::base);
     int *err = p.c.status;
 
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
         for (int i = 0; i < S::kRaw; ++i) mbar_init(raw_full + i, 1), mbar_init(raw_empty + i, 8), mbar_init(looked + i, 1);
         for (int i = 0; i < S::kSlots; ++i) mbar_init(deq_full + i, 8), mbar_init(deq_empty + i, 1);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(q_full + i, 4), mbar_init(o_free + i, 4);  // (an arrival per warp)
+            mbar_init(q_full + i, 4), mbar_init(o_free + i, 4), mbar_init(joined + i, 4);  // (an arrival per warp)
         }
         for (int i = 0; i < 4; ++i) mbar_init(s_full + i, 1), mbar_init(p_full + i, 4), mbar_init(pv_done + i, 1);
         mbar_init(mma_done, 1);
@@ -273,6 +273,13 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
         T *out = static_cast<T *>(p.a.out);
         uint32_t tile_no = 0;  // tiles this thread has done (phases of the barriers)
         bool ok = true;
+        // The four warps of this row tile meet, twice for each part of a cut job (so that the phases
+        // are known); false once one of them has given up (it does not come: the wait is bounded).
+        auto meet = [&](uint32_t parity) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(joined + q);
+            return __all_sync(0xffffffffu, mbar_wait_short(joined + q, parity, err)) != 0;
+        };
         while (ok && next()) {
             const int r = q * 128 + row, grow = g.row0 + r;
             const bool in = r < g.rows;
@@ -565,11 +572,11 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
             }
             __stcg(ps, make_float2(mrow, l));
             __threadfence();
-            named_barrier_sync(1 + q, 128);
+            if (!meet(0)) break;
             const int first = (int)(((g.job_u0 + 1) * blocks - 1) / units), last = (int)((g.job_u1 * blocks - 1) / units);
             uint32_t *count = p.arrived + first * kNQ + q;
             if (row == 0) misc[1 + q] = atomicAdd(count, 1u) == (uint32_t)(last - first);
-            named_barrier_sync(1 + q, 128);
+            if (!meet(1)) break;
             if (misc[1 + q]) {
                 __threadfence();
                 if (row == 0) *count = 0;
@@ -599,7 +606,7 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
                 if (in && p.a.lse)
                     p.a.lse[(int64_t)(g.s.q0 + i) * p.a.q_heads + hh] = jl == 0.0f ? -INFINITY : (jm + log2f(jl)) / kLog2e;
             }
-            named_barrier_sync(1 + q, 128);  // misc is free again
+            // (misc is written again after the next part's first meeting, when all have read it)
         }
     } else if (warp >= 8 && warp < 16) {
         // ---------------- unpack ----------------
