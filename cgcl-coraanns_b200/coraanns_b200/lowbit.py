@@ -18,6 +18,8 @@ from __future__ import annotations
 
 import ctypes as C
 import struct
+import threading
+import weakref
 from typing import NamedTuple, Optional
 
 import torch
@@ -76,6 +78,24 @@ except ImportError:
 
     def _stream(index):
         return torch.cuda.current_stream(index).cuda_stream
+
+try:  # whether the current device's current stream is being captured
+    from torch._C import _cuda_isCurrentStreamCapturing as _capturing
+except ImportError:
+    _capturing = torch.cuda.is_current_stream_capturing
+
+
+class _Workspace:
+    """Scratch memory of the attention calls of one stream, which run one after another: all caches
+    share it. Never part of a captured graph."""
+    __slots__ = ("held", "__weakref__")
+
+    def __init__(self):
+        self.held = (0, 0, None)  # address, bytes, the tensor: replaced as a whole
+
+
+_workspaces = weakref.WeakValueDictionary()  # (device, stream handle) -> _Workspace, alive while a cache uses it
+_workspaces_lock = threading.Lock()
 
 
 def _refuse(what):
@@ -156,7 +176,8 @@ class Cache4:
                               self.status.data_ptr())
         self._ref = C.addressof(self._arg)
         self._dev = self.device.index
-        self._work = {}  # attend's workspaces, one per stream (calls on different streams may overlap)
+        self._spaces = {}  # stream handle -> _Workspace (calls on different streams may overlap)
+        self._bytes = {}   # bits of the rows per key head -> bytes of a workspace
 
     def _heads(self, x, what, shape):
         """The type code of a (tokens, heads, head_dim) tensor."""
@@ -219,6 +240,9 @@ class Cache4:
         last `window` of them. scale: of the scores, default head_dim ** -0.5. A token that sees
         nothing gets zeros (and lse -inf). Returns out, or (out, lse): lse is fp32 (rows, heads).
         """
+        if self._dev != _current_device():
+            with torch.cuda.device(self._dev):
+                return self.attend(q, page_table, lens, q_start, max_queries, causal, window, scale, return_lse, out)
         dev = self.device
         if q.dim() != 3 or page_table.dim() != 2:
             _refuse("q must be (rows, heads, head_dim), page_table (sequences, width)")
@@ -243,28 +267,45 @@ class Cache4:
         if return_lse:
             lse = torch.empty((T, Hq), dtype=torch.float32, device=dev)
             lp = lse.data_ptr()
-        key = (_stream(self._dev), Hq, max_queries)
-        work, size = self._work.get(key) or self._workspace(key)
+        stream = _stream(self._dev)
+        bits = (max_queries * (Hq // self.kv_heads) - 1).bit_length()  # of the rows per key head
+        space, size = self._spaces.get(stream), self._bytes.get(bits)
+        held = (0, 0, None) if space is None or size is None else space.held  # (kept until the call is enqueued)
+        if not held[1] or held[1] < size or _capturing():
+            held = self._workspace(bits, stream)
+        work, size, _ = held
         qt, qh, _ = q.stride()
-        _call(self._lib.cora_kv4_attend, self._dev, self._ref, _ATTEND(
+        rc = self._lib.cora_kv4_attend(self._ref, _ATTEND(
             q.data_ptr(), out.data_ptr(), lp, qt, qh, page_table.data_ptr(),
             _index(lens, "lens", torch.int32, (B,), dev), qs, stride, T, size, work,
-            D ** -0.5 if scale is None else scale, B, width, Hq, max_queries, window, bool(causal), dt))
+            D ** -0.5 if scale is None else scale, B, width, Hq, max_queries, window, bool(causal), dt), stream)
+        if rc:
+            _check(rc)
         return (out, lse) if return_lse else out
 
-    def _workspace(self, key):
-        """The stream's workspace, made larger where this shape of call needs more."""
-        stream, heads, queries = key
-        with torch.cuda.device(self.device):
-            size = int(self._lib.cora_kv4_attend_workspace(self._ref, heads, queries))
-        _need(size > 0, "q_heads must be a multiple of kv_heads")
-        buf = self._work.get(stream)
-        if buf is None or buf.numel() < size:
-            self._work[stream] = buf = torch.zeros(size, dtype=torch.uint8, device=self.device)
-            for k in [k for k in self._work if isinstance(k, tuple) and k[0] == stream]:
-                del self._work[k]
-        self._work[key] = work = (buf.data_ptr(), buf.numel())
-        return work
+    def _workspace(self, bits, stream):
+        """(address, bytes, tensor) for a call of up to 2^bits rows per key head on the current stream."""
+        size = self._bytes.get(bits)
+        if size is None:
+            size = int(self._lib.cora_kv4_attend_workspace(self._ref, self.kv_heads, min(1 << bits, 0xffffffff)))
+            if not size:
+                raise CoraRuntimeError(load_library().cora_last_error().decode())
+            self._bytes[bits] = size
+        if _capturing():
+            # A graph's own: its replays may overlap calls, and other graphs, of this stream, and outlive
+            # what is kept here. The call itself adds the node that readies it.
+            buf = torch.empty(size, dtype=torch.uint8, device=self.device)
+            return buf.data_ptr(), size, buf
+        dev = self._dev
+        with _workspaces_lock:
+            space = _workspaces.get((dev, stream))
+            if space is None:
+                _workspaces[dev, stream] = space = _Workspace()
+            if space.held[1] < size:
+                buf = torch.zeros(size, dtype=torch.uint8, device=self.device)
+                space.held = (buf.data_ptr(), size, buf)
+            self._spaces[stream] = space
+            return space.held
 
     def check(self):
         """Synchronise the current stream; raise if a call met a bad slot, page, position or row
@@ -272,7 +313,11 @@ class Cache4:
         try:
             _call(self._lib.cora_kv4_status, self._dev, self._ref)
         except CoraRuntimeError:
-            self._work.clear()  # a call that gave up may have left its workspace unready
+            # a call that gave up may have left a workspace unready: the next ones take fresh memory
+            with _workspaces_lock:
+                for (dev, _), space in list(_workspaces.items()):
+                    if dev == self._dev:
+                        space.held = (0, 0, None)
             raise
 
 

@@ -185,6 +185,11 @@ void attend(const cora_kv4_cache *c, const cora_kv4_attend_args *a, cudaStream_t
     const double tiles = (double)a->table_width * c->page_size / 32 + 2;
     const double row_tiles = (double)a->q_tokens * (a->q_heads / c->kv_heads) / kAtRows + 1;
     need(tiles * row_tiles * c->kv_heads < 4.0e9, "too much work for one call: split the queries");
+    // A captured call readies its counters itself: whoever ran before a replay of the graph, and
+    // whether the memory was ever zeroed outside it, is not known here.
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    CUDA_TRY(cudaStreamIsCapturing(st, &capture));
+    if (capture != cudaStreamCaptureStatusNone) CUDA_TRY(cudaMemsetAsync(a->workspace, 0, attend_counters(), st));
     AttendParams p{};
     p.c = *c;
     p.a = *a;

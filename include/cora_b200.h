@@ -366,7 +366,9 @@ int cora_kv4_append(const cora_kv4_cache *cache, const cora_kv4_append_args *arg
  * contiguous. max_queries: an upper bound on the query tokens of a sequence.
  * workspace: cora_kv4_attend_workspace() bytes for this q_heads and max_queries, zero before its
  * first use; left ready for the next call (of any shape it is large enough for). Calls that
- * overlap in time need workspaces of their own. With more than 32 rows (query tokens x heads of a
+ * overlap in time need workspaces of their own. A call on a stream that is being captured readies its
+ * workspace in the graph: it need not be zero, but belongs to that graph (its replays must not overlap
+ * other users of it) and has to stay allocated as long as the graph. With more than 32 rows (query tokens x heads of a
  * group) per key head, cached values are rounded to fp16 (where values pass 65504, up to the
  * format's 16 times that, under 2^-5: those below 2^-9 then keep an absolute 2^-20). */
 typedef struct {

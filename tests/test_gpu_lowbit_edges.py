@@ -88,3 +88,79 @@ def test_attend_flat_tail_behind_a_sink(lb, per, n, L, H):
     for h in range(H):
         assert (np.abs(got[:, h] - want) <= bound).all(), (h, (np.abs(got[:, h] - want) / bound).max())
         assert np.abs(lse[:, h] - wlse).max() <= 2e-4
+
+
+# ---- captured graphs ------------------------------------------------------------------------------
+
+
+def graph_inputs(lb, lens, n, per=4, H=2, D=128, seed=1):
+    cache = random_cache(lb, 700, H, D, 16, 128, seed=seed)
+    _, table = page_tables(lens, 16, 700, seed)
+    dl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    qs = torch.arange(len(lens) + 1, dtype=torch.int32, device="cuda") * n
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    q = torch.randn(len(lens) * n, H * per, D, generator=gen, device="cuda").to(torch.bfloat16)
+    return cache, lambda out=None: cache.attend(q, table, dl, q_start=qs, max_queries=n, out=out)
+
+
+@pytest.mark.parametrize("warm", [True, False])
+def test_captured_steps_survive_larger_calls(lb, warm):
+    """Decoding steps of two caches captured on a stream, then larger eager calls there and memory
+    that others take: the replays give the eager results."""
+    a, step_a = graph_inputs(lb, [3000, 40, 5000], 1, seed=1)
+    b, step_b = graph_inputs(lb, [2000, 700], 1, seed=2)
+    _, chunk = graph_inputs(lb, [1500], 64, seed=3)
+    want, more = [step_a(), step_b()], chunk()
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    if warm:
+        with torch.cuda.stream(s):
+            step_a(), step_b()
+        s.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        got = [step_a(), step_b()]
+    with torch.cuda.stream(s):
+        first = chunk()
+        junk = [torch.full((size,), 0xff, dtype=torch.uint8, device="cuda") for size in (1 << 20, 6 << 20, 7 << 20, 20 << 20)]
+        for _ in range(3):
+            graph.replay()
+            second = chunk()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    assert torch.equal(first, more) and torch.equal(second, more)
+    assert all((j == 0xff).all() for j in junk)
+    a.check(), b.check()
+
+
+def test_graphs_of_one_stream_replayed_in_any_order(lb):
+    """Two graphs captured on a stream that never ran a call eagerly, of both kernels; the second is
+    replayed first, then both at once on two streams."""
+    a, step = graph_inputs(lb, [9000], 1, seed=4)
+    b, chunk = graph_inputs(lb, [2500], 100, seed=5)
+    want, more = step(), chunk()
+    torch.cuda.synchronize()
+    s, t = torch.cuda.Stream(), torch.cuda.Stream()
+    graphs, outs = [], []
+    for f in (step, chunk, step):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            outs.append(f())
+        graphs.append(g)
+    for g in reversed(graphs):
+        g.replay()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            graphs[0].replay()
+            graphs[1].replay()
+        with torch.cuda.stream(t):
+            graphs[2].replay()
+        eager = step()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want) and torch.equal(outs[1], more) and torch.equal(outs[2], want)
+        assert torch.equal(eager, want)
+    a.check(), b.check()
