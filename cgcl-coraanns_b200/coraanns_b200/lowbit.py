@@ -309,7 +309,8 @@ class Cache4:
 
     def check(self):
         """Synchronise the current stream; raise if a call met a bad slot, page, position or row
-        range, or if a wait ran out, since the last check."""
+        range, or if a wait ran out, since the last check. Calls on other streams are covered where
+        they are ordered before this one."""
         try:
             _call(self._lib.cora_kv4_status, self._dev, self._ref)
         except CoraRuntimeError:

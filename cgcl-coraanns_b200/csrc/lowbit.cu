@@ -52,6 +52,9 @@ void by_dtype(uint32_t dtype, F &&f) {
 template <int N>
 using Int = std::integral_constant<int, N>;
 
+// Takes back the bits that were reported, and only those: calls on other streams may set more.
+__global__ void clear_bits_kernel(int32_t *status, int32_t bits) { atomicAnd(status, ~bits); }
+
 // Raises a kernel's dynamic shared memory limit, once per device and kernel.
 template <typename K>
 void allow_smem(K kernel, size_t bytes, int (&seen)[64]) {
@@ -273,8 +276,12 @@ int cora_kv4_status(const cora_kv4_cache *cache, void *stream) {
         int32_t word = 0;
         auto st = static_cast<cudaStream_t>(stream);
         CUDA_TRY(cudaMemcpyAsync(&word, cache->status, sizeof word, cudaMemcpyDeviceToHost, st));
-        CUDA_TRY(cudaMemsetAsync(cache->status, 0, sizeof word, st));
         CUDA_TRY(cudaStreamSynchronize(st));
+        if (word) {
+            cora::clear_bits_kernel<<<1, 1, 0, st>>>(cache->status, word);
+            CUDA_TRY(cudaGetLastError());
+            CUDA_TRY(cudaStreamSynchronize(st));
+        }
         if (word & cora::kDevWaitTimeout) cora::fail(CORA_ERUNTIME, "a device-side wait timed out");
         if (word & cora::kDevBadInput)
             cora::fail(CORA_ERUNTIME, "a slot, position, page or row range lies outside its tensor");

@@ -334,7 +334,8 @@ typedef struct {
 } cora_kv4_cache;
 
 uint64_t cora_kv4_block_bytes(uint32_t page_size, uint32_t head_dim, uint32_t group);
-/* Synchronises `stream`, reports and clears the status word: CORA_ERUNTIME if a bit is set. */
+/* Synchronises `stream`, reports the status word and clears what it reports: CORA_ERUNTIME if a bit is
+ * set. Covers the calls ordered before it on `stream`; bits of others are kept for the next report. */
 int cora_kv4_status(const cora_kv4_cache *cache, void *stream);
 
 /* Rotates keys and queries by position, quantises keys and values, stores them at their slots

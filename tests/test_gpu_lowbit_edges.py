@@ -164,3 +164,37 @@ def test_graphs_of_one_stream_replayed_in_any_order(lb):
         assert torch.equal(outs[0], want) and torch.equal(outs[1], more) and torch.equal(outs[2], want)
         assert torch.equal(eager, want)
     a.check(), b.check()
+
+
+# ---- errors found on the device -------------------------------------------------------------------
+
+
+def test_check_loses_no_error(lb):
+    """Calls on one stream set the status word while check() reads and clears it on another: each
+    error is reported."""
+    import threading
+    cache = lb.Cache4(2, 1, 64, page_size=16)
+    k = torch.zeros(1, 1, 64, dtype=torch.bfloat16, device="cuda")
+    bad = torch.tensor([32], device="cuda")
+    torch.cuda.synchronize()
+    raised, lost = threading.Event(), []
+
+    def caller():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for i in range(400):
+                raised.clear()
+                cache.append(k, k, bad)
+                torch.cuda.current_stream().synchronize()
+                if not raised.wait(2):
+                    lost.append(i)
+                    return
+
+    thread = threading.Thread(target=caller)
+    thread.start()
+    while thread.is_alive():
+        try:
+            cache.check()
+        except Exception:
+            raised.set()
+    thread.join()
+    assert not lost
