@@ -10,8 +10,8 @@
 //    side: the query heads that share a key head fill one instruction;
 //  - a code becomes an fp16 operand by one AND: nibble 0 of a 16-bit half is the subnormal
 //    c 2^-24, nibble 1 is c 2^-20, both exact in the tensor core. The powers of two go into q
-//    (a common power of two per job, so fp16 holds every bit of a bf16 or fp16 q that is
-//    within 2^-24 of the largest) and into the final scaling of the output;
+//    (a power of two per row, so fp16 holds every bit of a bf16 or fp16 q that is within 2^-24 of
+//    its row's largest) and into the final scaling of the output;
 //  - w = fp16(p scale') is the operand of the second product (11 bits; scaled by a power of two
 //    that follows the largest scale' met, so it uses the normal range). What the rounding of w
 //    loses would be multiplied by codes of 0..15 although values spread around the middle of
@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const A
     float acc[kVB][4][4], om[2][kNG], ws[kNG][4];  // sum w c'; sum p (low' + 7.5 scale'); sum w (rows alike)
     float mx[2], ref[2], over[2], ls[2];           // per row: maximum, what scores are relative to, how far
                                                    // they may exceed it, sum of p
-    float qs[2][kNG], raw = 0.0f;                  // sums of q; the unit of q . c
+    float qs[2][kNG], raw[2] = {};                 // sums of q; the unit of these and of q . c
     int2 lm[2];                                    // tokens that rows 2 t and 2 t + 1 see
     int lo_max = 0, hi_min = 0;
     int vexp = 0;                                  // 2^-vexp bounds the value scales met
@@ -378,20 +378,48 @@ __global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const A
         }
         if (fresh) {
         fresh = false;
-        // queries: rows are (token, head of the group); fp16 under a common power of two
-        float big = 0.0f;
+        // queries: rows are (token, head of the group); fp16 under a power of two per row: 2^qe brings
+        // the row's largest |q| into [2^13, 2^14). qe[i] is that of the lane's row of load i
+        int qe[kLoads];
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i)
+        for (int i = 0; i < kLoads; ++i) {
+            float big = 0.0f;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float m = fabsf(to_f32(qv[i][e]));
-                big = m < 3.4e38f ? fmaxf(big, m) : big;  // infinities and NaN keep to their rows
+                big = m < 3.4e38f ? fmaxf(big, m) : big;  // infinities and NaN have no say
             }
-        big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));
-        // 2^qe brings the largest |q| into [2^13, 2^14)
-        const int qe = big > 0.0f ? max(-100, min(126, 13 - ilogbf(big))) : 0;
-        const float qpow = ldexpf(1.0f, qe), qf = p.a.scale * kLog2e;
-        raw = ldexpf(qf, 24 - qe);  // of q . c as the tensor core sums it
+            uint32_t top = __float_as_uint(big);
+            if constexpr (D == 64) {  // a row is half a load
+#pragma unroll
+                for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+            } else {
+                top = __reduce_max_sync(0xffffffffu, top);
+            }
+            qe[i] = (int)(top >> 23);
+        }
+        if constexpr (D == 256) {  // a row is two loads
+#pragma unroll
+            for (int i = 0; i < kLoads; i += 2) qe[i] = qe[i + 1] = max(qe[i], qe[i + 1]);
+        }
+        const float qf = p.a.scale * kLog2e;
+        float qpow[kLoads];
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            qe[i] = max(-100, min(126, 13 + 127 - qe[i]));
+            qpow[i] = __int_as_float((qe[i] + 127) << 23);
+        }
+        int qe2[2];  // of rows 2 t and 2 t + 1
+        if constexpr (D == 64) {
+            const int mine = t == 0 ? qe[0] : t == 1 ? qe[1] : t == 2 ? qe[2] : qe[3], other = __shfl_xor_sync(0xffffffffu, mine, 16);
+            qe2[0] = lane < 16 ? mine : other, qe2[1] = lane < 16 ? other : mine;
+        } else {
+            constexpr int kPer = D / 128;  // loads of a row
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+                qe2[c] = t == 0 ? qe[c * kPer] : t == 1 ? qe[(2 + c) * kPer] : t == 2 ? qe[(4 + c) * kPer] : qe[(6 + c) * kPer];
+        }
+        raw[0] = ldexpf(qf, 24 - qe2[0]), raw[1] = ldexpf(qf, 24 - qe2[1]);  // of q . c as the tensor core sums it
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
@@ -401,7 +429,7 @@ __global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const A
             // 2^-4: neighbouring lanes swap halves, and each stores two pairs.
             float x[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = r < nrows ? to_f32(qv[i][e]) * qpow * (e & 1 ? 0.0625f : 1.0f) : 0.0f;
+            for (int e = 0; e < 4; ++e) x[e] = r < nrows ? to_f32(qv[i][e]) * qpow[i] * (e & 1 ? 0.0625f : 1.0f) : 0.0f;
             const uint32_t lo = pack_half2(x[0], x[1]), hi = pack_half2(x[2], x[3]);
             const uint32_t other = __shfl_xor_sync(0xffffffffu, lane & 1 ? lo : hi, 1);
             uint2 w;
@@ -423,8 +451,7 @@ __global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const A
                 mma16816<__half>(d, one, one, sixteen, sixteen, q.x, q.y);
                 mma16816<__half>(d, one, one, sixteen, sixteen, q.z, q.w);
             }
-            const float f = ldexpf(qf, -qe);
-            qs[0][gr] = d[0] * f, qs[1][gr] = d[1] * f;
+            qs[0][gr] = d[0] * 5.9604644775390625e-8f, qs[1][gr] = d[1] * 5.9604644775390625e-8f;  // 2^-24
         }
         lo_max = 0, hi_min = 0x7fffffff;
 #pragma unroll
@@ -484,11 +511,12 @@ __global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const A
                     const __half2 *km = reinterpret_cast<const __half2 *>(st + 2 * S::kCodes);
                     const float2 f0 = __half22float2(km[(mt * 16 + tg) * kNG + gr]);
                     const float2 f1 = __half22float2(km[(mt * 16 + 8 + tg) * kNG + gr]);
-                    const float r0 = f0.x * raw, r1 = f1.x * raw;
 #pragma unroll
                     for (int c = 0; c < 4; ++c)
-                        s[mt][c] = fmaf(c < 2 ? r0 : r1, d[c], fmaf(c < 2 ? f0.y : f1.y, qs[c & 1][gr], gr ? s[mt][c] : -ref[c & 1]));
+                        s[mt][c] = fmaf(c < 2 ? f0.x : f1.x, d[c], fmaf(c < 2 ? f0.y : f1.y, qs[c & 1][gr], gr ? s[mt][c] : 0.0f));
                 }
+#pragma unroll
+                for (int c = 0; c < 4; ++c) s[mt][c] = fmaf(s[mt][c], raw[c & 1], -ref[c & 1]);
             }
             const uint32_t *vm = reinterpret_cast<const uint32_t *>(st + 2 * S::kCodes + S::kMeta);
             uint32_t vf[kMt][2][kNG];  // the tokens' value factors

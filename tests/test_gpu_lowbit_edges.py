@@ -90,6 +90,28 @@ def test_attend_flat_tail_behind_a_sink(lb, per, n, L, H):
         assert np.abs(lse[:, h] - wlse).max() <= 2e-4
 
 
+# ---- rows and tokens that must not touch one another ------------------------------------------
+
+
+@pytest.mark.parametrize("D,G", [(64, 64), (128, 64), (128, 128), (256, 128)])
+@pytest.mark.parametrize("n", [1, 3, 12])
+def test_attend_huge_query_keeps_to_its_row(lb, D, G, n):
+    """A finite but huge query changes nothing in the rows that share its instructions."""
+    cache = random_cache(lb, 12, 1, D, 16, G, seed=2)
+    table, dtable = page_tables([90], 16, 12, 3)
+    q = torch.randn(n, 4, D, device="cuda").to(torch.bfloat16)
+    dl = torch.tensor([90], dtype=torch.int32, device="cuda")
+    qs = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    want = cache.attend(q, dtable, dl, q_start=qs, max_queries=n)
+    big = q.clone()
+    big[0, 1] *= 2.0 ** 60
+    big[n - 1, 3, 5] = 1e30
+    got = cache.attend(big, dtable, dl, q_start=qs, max_queries=n)
+    touched = torch.zeros(n, 4, dtype=torch.bool, device="cuda")
+    touched[0, 1] = touched[n - 1, 3] = True
+    assert torch.equal(got[~touched], want[~touched])
+
+
 # ---- captured graphs ------------------------------------------------------------------------------
 
 
