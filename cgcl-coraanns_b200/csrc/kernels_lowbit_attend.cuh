@@ -527,6 +527,10 @@ __global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const A
 #pragma unroll
                     for (int gr = 0; gr < kNG; ++gr) vf[mt][r][gr] = vm[(mt * 16 + tg + r * 8) * kNG + gr];
             if (tok0 + kAtTile > hi_min || tok0 < lo_max) {  // some row does not see some token
+                // tokens that the job's rows see between them
+                const int past = sw.len - sw.n, first = past + row0 / heads, last = past + (row0 + nrows - 1) / heads;
+                const int job_hi = p.a.causal ? min(sw.len, last + 1) : sw.len;
+                const int job_lo = p.a.window ? first - (int)p.a.window + 1 : 0;
 #pragma unroll
                 for (int mt = 0; mt < kMt; ++mt)
 #pragma unroll
@@ -535,7 +539,8 @@ __global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const A
 #pragma unroll
                         for (int c = 0; c < 2; ++c)
                             if (tok < lm[c].x || tok >= lm[c].y) s[mt][2 * r + c] = -INFINITY;
-                        if (tok >= sw.len) {  // nobody does: the bytes may be anything
+                        if (tok < job_lo || tok >= job_hi) {  // nobody does: the bytes may be anything, and have no
+                                                              // part in the bound of the value scales
 #pragma unroll
                             for (int gr = 0; gr < kNG; ++gr) vf[mt][r][gr] = 0;
                         }

@@ -112,6 +112,30 @@ def test_attend_huge_query_keeps_to_its_row(lb, D, G, n):
     assert torch.equal(got[~touched], want[~touched])
 
 
+@pytest.mark.parametrize("per,n", [(4, 1), (8, 3), (2, 4)])
+def test_attend_hidden_tokens_of_wide_range(lb, per, n):
+    """Value factors of the largest finite size in tokens that no query sees (outside the window,
+    past the end) or only the last query does: the others keep their accuracy, for values that are
+    small beside them."""
+    D, page, L, window, seed = 128, 16, 90, 20, 40
+    lens = [L]
+    cache = lb.Cache4(8, 1, D, page_size=page)
+    k, v = (torch.randn(8 * page, 1, D, device="cuda") for _ in range(2))
+    cache.append(k.to(torch.bfloat16), (1e-3 * v).to(torch.bfloat16), torch.arange(8 * page, device="cuda"))
+    hidden = list(range(L - n - window + 1)) + list(range(L, 96)) + ([L - 1] if n > 1 and per == 8 else [])
+    wide = torch.linspace(-6e4, 6e4, D, device="cuda").to(torch.bfloat16)[None, None].expand(len(hidden), 1, D)
+    cache.append(wide, wide, slots_of(cache, [96], seed, hidden))
+    table, dtable = page_tables([96], page, 8, seed + 1)
+    q = torch.randn(n, per, D, device="cuda").to(torch.bfloat16)
+    got = cache.attend(q, dtable, torch.tensor(lens, dtype=torch.int32, device="cuda"),
+                       q_start=torch.tensor([0, n], dtype=torch.int32, device="cuda"), max_queries=n, window=window)
+    cache.check()
+    want, mass, _ = attend64(cache, q, table, lens, [0, n], True, window, D ** -0.5)
+    err = np.abs(got.double().cpu().numpy() - want)
+    bound = TOL_OUT["bf16"] * np.abs(want) + TOL_MASS * mass
+    assert (err <= bound).all(), (err / bound).max()
+
+
 # ---- captured graphs ------------------------------------------------------------------------------
 
 
