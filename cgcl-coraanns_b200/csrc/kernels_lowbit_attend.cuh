@@ -13,7 +13,8 @@
 //    (a power of two per row, so fp16 holds every bit of a bf16 or fp16 q that is within 2^-24 of
 //    its row's largest) and into the final scaling of the output;
 //  - w = fp16(p scale') is the operand of the second product (11 bits; scaled by a power of two
-//    that follows the largest scale' met, so it uses the normal range). What the rounding of w
+//    per row that follows the largest scale' met, or the largest p scale' where that is far less, so
+//    it uses the normal range). What the rounding of w
 //    loses would be multiplied by codes of 0..15 although values spread around the middle of
 //    their group's range; so the sum is taken as sum w (c' - 7.5) + sum p (low' + 7.5 scale'),
 //    sum w by one more product with ones: the loss is then 2^-12 of |value - middle|.
@@ -101,6 +102,9 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
+// 2^e, and the e of the largest 2^e up to x (-127 for 0 and what is below the normal range).
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
+__device__ __forceinline__ int exponent_of(float x) { return (__float_as_int(x) >> 23) - 127; }
 // Largest and sum over the eight lanes of one column pair (lane = 4 g + t, over g).
 __device__ __forceinline__ float max_over_g(float v) {
     v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
@@ -326,8 +330,8 @@ __global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const A
     float qs[2][kNG], raw[2] = {};                 // sums of q; the unit of these and of q . c
     int2 lm[2];                                    // tokens that rows 2 t and 2 t + 1 see
     int lo_max = 0, hi_min = 0;
-    int vexp = 0;                                  // 2^-vexp bounds the value scales met
-    float vbound = 0.0f, vmul = 0.0f;              // w = p scale' vmul = p scale' 2^(7 + vexp)
+    float vmul[2] = {};                            // w = p scale' vmul, a power of two: 2^7 / vmul bounds the value
+    float vbound = 0.0f;                           // scales met (0: none yet); the less of both rows' bounds
     int b = -1, head = 0, row0 = 0, nrows = 0, tile = 0, tile_end = 0;
     int64_t u = u0, seg_end = 0, job_u0 = 0, job_u1 = 0;
     SeqWork sw{};
@@ -407,7 +411,7 @@ __global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const A
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             qe[i] = max(-100, min(126, 13 + 127 - qe[i]));
-            qpow[i] = __int_as_float((qe[i] + 127) << 23);
+            qpow[i] = power_of_two(qe[i]);
         }
         int qe2[2];  // of rows 2 t and 2 t + 1
         if constexpr (D == 64) {
@@ -473,7 +477,7 @@ __global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const A
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) acc[v][i][c] = 0.0f;
-        vexp = 119, vbound = vmul = 0.0f;
+        vbound = vmul[0] = vmul[1] = 0.0f;
         }
 
         {
@@ -564,32 +568,7 @@ __global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const A
                 out_of_course |= m > over[c];
             }
             if (__any_sync(0xffffffffu, out_of_course)) {
-                float smax = 0.0f;
-#pragma unroll
-                for (int mt = 0; mt < kMt; ++mt)
-#pragma unroll
-                    for (int r = 0; r < 2; ++r)
-#pragma unroll
-                        for (int gr = 0; gr < kNG; ++gr) {
-                            const float2 f = __half22float2(*reinterpret_cast<__half2 *>(&vf[mt][r][gr]));
-                            if (fabsf(f.x) <= 65504.0f && fabsf(f.y) <= 65504.0f) {
-                                smax = fmaxf(smax, fabsf(f.x));
-                                continue;
-                            }
-                            vf[mt][r][gr] = 0;
-#pragma unroll
-                            for (int c = 0; c < 2; ++c)
-                                if (s[mt][2 * r + c] != -INFINITY) ls[c] = __int_as_float(0x7fc00000);
-                        }
-                smax = max_over_g(smax);
-                float shrink = 1.0f;
-                if (smax > vbound) {
-                    const int e = -(ilogbf(smax) + 1);  // smax < 2^-e
-                    if (vbound > 0.0f) shrink = ldexpf(1.0f, e - vexp);
-                    vexp = e;
-                    vbound = ldexpf(1.0f, -e);
-                    vmul = ldexpf(1.0f, 7 + e);
-                }
+                float k[2];
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     float m = fmaxf(s[0][c], s[0][c + 2]);
@@ -597,16 +576,51 @@ __global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const A
                     for (int mt = 1; mt < kMt; ++mt) m = fmaxf(m, fmaxf(s[mt][c], s[mt][c + 2]));
                     m = max_over_g(m) + ref[c];
                     const bool grew = m > mx[c] + (mx[c] == -INFINITY ? 0.0f : 8.0f);
-                    const float k = grew ? ex2(mx[c] - m) : 1.0f, f = k * shrink;
+                    k[c] = grew ? ex2(mx[c] - m) : 1.0f;
                     if (grew) {
                         const float shift = ref[c] - m;
                         mx[c] = ref[c] = m, over[c] = 8.0f;
 #pragma unroll
                         for (int mt = 0; mt < kMt; ++mt) s[mt][c] += shift, s[mt][c + 2] += shift;
                     }
-                    ls[c] *= k;
+                }
+                // A row's bound: the largest value scale, or 2^6 times its largest p scale (p up to 1)
+                // where that is less: a token that it all but ignores does not cost it its bits.
+                float smax = 0.0f, pmax[2] = {};
 #pragma unroll
-                    for (int gr = 0; gr < kNG; ++gr) om[c][gr] *= k, ws[gr][c] *= f;
+                for (int mt = 0; mt < kMt; ++mt)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const float p0 = ex2(fminf(0.0f, s[mt][2 * r])), p1 = ex2(fminf(0.0f, s[mt][2 * r + 1]));
+#pragma unroll
+                        for (int gr = 0; gr < kNG; ++gr) {
+                            const float2 f = __half22float2(*reinterpret_cast<__half2 *>(&vf[mt][r][gr]));
+                            if (fabsf(f.x) <= 65504.0f && fabsf(f.y) <= 65504.0f) {
+                                smax = fmaxf(smax, fabsf(f.x));
+                                pmax[0] = fmaxf(pmax[0], fabsf(f.x) * p0), pmax[1] = fmaxf(pmax[1], fabsf(f.x) * p1);
+                                continue;
+                            }
+                            vf[mt][r][gr] = 0;
+#pragma unroll
+                            for (int c = 0; c < 2; ++c)
+                                if (s[mt][2 * r + c] != -INFINITY) ls[c] = __int_as_float(0x7fc00000);
+                        }
+                    }
+                smax = max_over_g(smax);
+                vbound = 65504.0f;  // (of rows that saw a token; another comes this way with its first)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const float most = fminf(smax, 64.0f * max_over_g(pmax[c]));
+                    float f = k[c];
+                    if (most * vmul[c] > 128.0f || (vmul[c] == 0.0f && most > 0.0f)) {
+                        const float to = power_of_two(min(100, 6 - exponent_of(most)));  // most < 2^7 / to
+                        if (vmul[c] > 0.0f) f *= to * power_of_two(-exponent_of(vmul[c]));
+                        vmul[c] = to;
+                    }
+                    if (mx[c] != -INFINITY) vbound = fminf(vbound, vmul[c] > 0.0f ? power_of_two(7 - exponent_of(vmul[c])) : 0.0f);
+                    ls[c] *= k[c];
+#pragma unroll
+                    for (int gr = 0; gr < kNG; ++gr) om[c][gr] *= k[c], ws[gr][c] *= f;
 #pragma unroll
                     for (int v = 0; v < kVB; ++v)
 #pragma unroll
@@ -617,10 +631,12 @@ __global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const A
 #pragma unroll
             for (int mt = 0; mt < kMt; ++mt) {
                 uint32_t pb[kNG][2];
+                float sv[4];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     s[mt][c] = ex2(s[mt][c]);
                     ls[c & 1] += s[mt][c];
+                    sv[c] = s[mt][c] * vmul[c & 1];
                 }
 #pragma unroll
                 for (int gr = 0; gr < kNG; ++gr) {
@@ -628,10 +644,10 @@ __global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const A
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
                         const float2 f = __half22float2(*reinterpret_cast<__half2 *>(&vf[mt][r][gr]));
-                        const float fw = f.x * vmul, fm = fmaf(7.5f, f.x, f.y);
+                        const float fm = fmaf(7.5f, f.x, f.y);
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            x[2 * r + c] = s[mt][2 * r + c] * fw;
+                            x[2 * r + c] = sv[2 * r + c] * f.x;
                             om[c][gr] = fmaf(s[mt][2 * r + c], fm, om[c][gr]);
                         }
                     }
@@ -672,9 +688,9 @@ __global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const A
         fresh = true;
 
         // ---- the warp's result of this job: acc becomes sum p v, ls the sum over its tokens ----
-        const float opow = ldexpf(1.0f, 17 - vexp);  // 2^24 of the codes, 2^-(7 + vexp) of the operand
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
+            const float opow = vmul[c] > 0.0f ? power_of_two(24 - exponent_of(vmul[c])) : 0.0f;  // 2^24 of the codes, the operand's factor
             ls[c] = sum_over_g(ls[c]);
 #pragma unroll
             for (int gr = 0; gr < kNG; ++gr) {
