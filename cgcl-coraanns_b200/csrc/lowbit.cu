@@ -178,7 +178,10 @@ void attend(const cora_kv4_cache *c, const cora_kv4_attend_args *a, cudaStream_t
     need(a->q_heads >= 1 && a->q_heads % c->kv_heads == 0, "q_heads must be a multiple of kv_heads");
     need(a->q_tokens <= INT_MAX && a->seqs <= INT_MAX, "too many rows");
     need(a->q_start || a->q_tokens >= a->seqs, "q needs a row per sequence where q_start is null");
-    need((uint64_t)a->table_width * c->page_size <= INT_MAX, "table_width * page_size must fit an int");
+    // Positions, from -q_tokens to the table's last token, and up to 32 pages read ahead are ints in the
+    // kernels.
+    const uint64_t room = (uint64_t)a->table_width * c->page_size;
+    need(room + 32ull * c->page_size + a->q_tokens <= INT_MAX, "table_width * page_size must fit an int, with q_tokens and 32 pages");
     need(!a->window || a->causal, "a window needs causal attention");
     need(a->window <= INT_MAX, "window must fit an int");
     const uint64_t rows = attend_rows(*c, a->q_heads, a->max_queries);

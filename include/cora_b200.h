@@ -365,6 +365,7 @@ int cora_kv4_append(const cora_kv4_cache *cache, const cora_kv4_append_args *arg
  * -inf). Query heads h * q_heads / kv_heads .. share key head h. out is q_tokens x q_heads x
  * head_dim, lse (natural log of the sum of exponentials; may be null) q_tokens x q_heads, both
  * contiguous. max_queries: an upper bound on the query tokens of a sequence.
+ * (table_width + 32) * page_size + q_tokens has to fit an int.
  * workspace: cora_kv4_attend_workspace() bytes for this q_heads and max_queries, zero before its
  * first use; left ready for the next call (of any shape it is large enough for). Calls that
  * overlap in time need workspaces of their own. A call on a stream that is being captured readies its

@@ -36,6 +36,18 @@ def test_roles_of_the_tile_kernel_meet_with_a_limit():
     assert "mbar_wait_short" in roles
 
 
+@pytest.mark.parametrize("width,page,tokens", [((1 << 31) // 64 - 1, 64, 2), ((1 << 31) // 1024 - 8, 1024, 2),
+                                               ((1 << 31) // 16 - 33, 16, 100), (1 << 20, 1024, (1 << 30))])
+def test_tables_whose_positions_pass_an_int_are_refused(width, page, tokens):
+    """The kernels hold positions, and pages up to 32 ahead, as ints."""
+    from test_lowbit_abi import attend_args, cache_arg
+    from coraanns_b200 import CORA_EINVAL, lowbit
+    lib = lowbit._library()
+    c = cache_arg(page_size=page)
+    assert lib.cora_kv4_attend(C.addressof(c), attend_args(width=width, tokens=tokens), None) == CORA_EINVAL
+    assert b"table_width" in lib.cora_last_error()
+
+
 # ---- attention's workspaces, on host memory with the C calls replaced -----------------------------
 
 
