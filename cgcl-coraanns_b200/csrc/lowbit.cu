@@ -199,6 +199,9 @@ void attend(const cora_kv4_cache *c, const cora_kv4_attend_args *a, cudaStream_t
     AttendParams p{};
     p.c = *c;
     p.a = *a;
+    // No sequence is longer than its table: a wider window hides nothing, and position - window would
+    // wrap for the queries of a sequence that has more of them than cached tokens.
+    if (a->window >= room) p.a.window = 0;
     p.q_tokens = (int64_t)a->q_tokens;
     p.arrived = static_cast<uint32_t *>(a->workspace);
     p.part = reinterpret_cast<float *>(static_cast<char *>(a->workspace) + attend_counters());

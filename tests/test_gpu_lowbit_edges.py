@@ -136,6 +136,13 @@ def test_attend_hidden_tokens_of_wide_range(lb, per, n):
     assert (err <= bound).all(), (err / bound).max()
 
 
+def test_attend_window_of_any_size(lb):
+    """A window as large as an int holds, with more queries than cached tokens."""
+    for D, G, per in ((128, 128, 2), (64, 64, 4), (256, 128, 1)):
+        cache = random_cache(lb, 20, 1, D, 16, G, seed=6)
+        check_attend(lb, cache, [100, 70], per, [200, 80], "bf16", window=2 ** 31 - 1, seed=50)
+
+
 # ---- captured graphs ------------------------------------------------------------------------------
 
 
