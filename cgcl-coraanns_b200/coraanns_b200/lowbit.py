@@ -238,7 +238,7 @@ class Cache4:
         q_start[b + 1] - 1 (q_start int32 (sequences + 1,), at most max_queries each; without it
         row b), its last tokens. causal: a token sees those up to itself, with a window only the
         last `window` of them. scale: of the scores, default head_dim ** -0.5. A token that sees
-        nothing gets zeros (and lse -inf). Returns out, or (out, lse): lse is fp32 (rows, heads).
+        nothing gets zeros (and lse -inf), as do rows of q outside all ranges. Returns out, or (out, lse): lse is fp32 (rows, heads).
         """
         if self._dev != _current_device():
             with torch.cuda.device(self._dev):

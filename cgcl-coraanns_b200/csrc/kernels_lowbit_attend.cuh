@@ -147,6 +147,24 @@ __device__ __forceinline__ SeqWork seq_work(const AttendParams &p, int b, int ro
     return s;
 }
 
+// Rows [from, to) that no sequence asks for: zeros, log-sums -inf. By all threads of the grid.
+__device__ __forceinline__ void clear_rows(const AttendParams &p, int64_t from, int64_t to, uint32_t thread, uint32_t threads) {
+    const int64_t heads = p.a.q_heads, chunks = p.c.head_dim / 8;
+    uint4 *const out = static_cast<uint4 *>(p.a.out);
+    for (int64_t i = from * heads * chunks + thread; i < to * heads * chunks; i += threads) out[i] = make_uint4(0, 0, 0, 0);
+    if (p.a.lse)
+        for (int64_t i = from * heads + thread; i < to * heads; i += threads) p.a.lse[i] = -INFINITY;
+}
+// Those of a launch: before the first range (first launch), after the last (last launch).
+__device__ __forceinline__ void clear_gaps(const AttendParams &p, int64_t q0, int64_t q1, uint32_t thread, uint32_t threads) {
+    if (p.seq0 == 0 && q0 > 0) clear_rows(p, 0, q0, thread, threads);
+    if (p.seq0 + p.seqs == p.a.seqs && q1 < p.q_tokens) clear_rows(p, q1, p.q_tokens, thread, threads);
+}
+// A call without sequences.
+__global__ void kv4_clear_kernel(const AttendParams p) {
+    clear_rows(p, 0, p.q_tokens, blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x);
+}
+
 template <typename T, int D, int kNG>
 __global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const AttendParams p) {
     using S = AttendSmem<D, kNG>;
@@ -211,6 +229,8 @@ __global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const A
         }
         longest = __reduce_max_sync(0xffffffffu, longest);
         if (lane == 0) misc[2] = (int64_t)longest * kAtTile <= kAtShort && jobs <= gridDim.x ? (int)jobs : 0;
+    } else if (warp == 1) {  // (meanwhile)
+        clear_gaps(p, work[0].x, (int64_t)work[p.seqs - 1].x + work[p.seqs - 1].y, blockIdx.x * 32 + lane, gridDim.x * 32);
     }
     __syncthreads();
     const int64_t units = base[p.seqs];

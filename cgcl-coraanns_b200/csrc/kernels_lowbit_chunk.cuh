@@ -26,7 +26,8 @@
 //             warp runs the loop; from a branch to one lane the issue itself was the bound
 //             (802 against 730 us).
 //   18        looks for values past 65504 in a copied tile's factors before it is unpacked (by the
-//             unpacking warps themselves it cost 80 cycles a tile). Warp 19 is idle.
+//             unpacking warps themselves it cost 80 cycles a tile).
+//   19        clears rows of the output that no sequence asks for.
 // Units (sequence, key head, row tile, token tile) are cut into equal runs, one per block; a job
 // cut over blocks is joined by the last to arrive. Every wait is bounded.
 //
@@ -785,6 +786,10 @@ __global__ void __launch_bounds__(kCkThreads, 1) kv4_chunk_kernel(const AttendPa
                 }
             }
         }
+        } else if (warp == 19) {
+        // ---------------- rows that no sequence asks for ----------------
+        const SeqWork head = seq_work(p, 0, kRows, kTN), tail = seq_work(p, (int)p.seqs - 1, kRows, kTN);
+        clear_gaps(p, head.q0, (int64_t)tail.q0 + tail.n, blockIdx.x * 32 + lane, gridDim.x * 32);
         } else if (warp == 17) {
         // ---------------- products ----------------
         constexpr uint32_t id_qk = idesc_f16(128, kTN, false), id_pv = idesc_f16(128, D, true);

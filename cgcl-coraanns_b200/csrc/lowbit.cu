@@ -172,8 +172,8 @@ void launch_chunk(AttendParams p, cudaStream_t st) {
 void attend(const cora_kv4_cache *c, const cora_kv4_attend_args *a, cudaStream_t st) {
     check_cache(c);
     need(a, "null arguments");
-    if (a->seqs == 0 || a->q_tokens == 0) return;
-    need(a->q && a->out && a->page_table && a->lens, "q, out, page_table and lens are needed");
+    if (a->q_tokens == 0) return;
+    need(a->q && a->out && (!a->seqs || (a->page_table && a->lens)), "q, out, page_table and lens are needed");
     need(aligned16(a->out), "out must be 16-byte aligned");
     need(a->q_heads >= 1 && a->q_heads % c->kv_heads == 0, "q_heads must be a multiple of kv_heads");
     need(a->q_tokens <= INT_MAX && a->seqs <= INT_MAX, "too many rows");
@@ -184,6 +184,16 @@ void attend(const cora_kv4_cache *c, const cora_kv4_attend_args *a, cudaStream_t
     need(room + 32ull * c->page_size + a->q_tokens <= INT_MAX, "table_width * page_size must fit an int, with q_tokens and 32 pages");
     need(!a->window || a->causal, "a window needs causal attention");
     need(a->window <= INT_MAX, "window must fit an int");
+    AttendParams p{};
+    p.c = *c;
+    p.a = *a;
+    p.q_tokens = (int64_t)a->q_tokens;
+    if (!a->seqs) {
+        by_dtype(a->dtype, [](auto) {});
+        kv4_clear_kernel<<<sm_count(), 256, 0, st>>>(p);
+        CUDA_TRY(cudaGetLastError());
+        return;
+    }
     const uint64_t rows = attend_rows(*c, a->q_heads, a->max_queries);
     need(a->workspace && aligned16(a->workspace) && a->workspace_bytes >= attend_workspace(*c, rows),
          "the workspace is smaller than cora_kv4_attend_workspace()");
@@ -196,13 +206,9 @@ void attend(const cora_kv4_cache *c, const cora_kv4_attend_args *a, cudaStream_t
     cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
     CUDA_TRY(cudaStreamIsCapturing(st, &capture));
     if (capture != cudaStreamCaptureStatusNone) CUDA_TRY(cudaMemsetAsync(a->workspace, 0, attend_counters(), st));
-    AttendParams p{};
-    p.c = *c;
-    p.a = *a;
     // No sequence is longer than its table: a wider window hides nothing, and position - window would
     // wrap for the queries of a sequence that has more of them than cached tokens.
     if (a->window >= room) p.a.window = 0;
-    p.q_tokens = (int64_t)a->q_tokens;
     p.arrived = static_cast<uint32_t *>(a->workspace);
     p.part = reinterpret_cast<float *>(static_cast<char *>(a->workspace) + attend_counters());
     by_dtype(a->dtype, [&](auto z) {

@@ -362,7 +362,7 @@ int cora_kv4_append(const cora_kv4_cache *cache, const cora_kv4_append_args *arg
  * [q_start[b], q_start[b + 1]) of q (q_start null: row b), the last ones of the sequence: the
  * i-th of n is at position lens[b] - n + i. causal: a query sees tokens up to its position;
  * window w > 0 (causal only): the last w of those. A query that sees none gives zeros (lse
- * -inf). Query heads h * q_heads / kv_heads .. share key head h. out is q_tokens x q_heads x
+ * -inf), and so do rows of q before the first range and after the last. Query heads h * q_heads / kv_heads .. share key head h. out is q_tokens x q_heads x
  * head_dim, lse (natural log of the sum of exponentials; may be null) q_tokens x q_heads, both
  * contiguous. max_queries: an upper bound on the query tokens of a sequence.
  * (table_width + 32) * page_size + q_tokens has to fit an int.

@@ -143,6 +143,54 @@ def test_attend_window_of_any_size(lb):
         check_attend(lb, cache, [100, 70], per, [200, 80], "bf16", window=2 ** 31 - 1, seed=50)
 
 
+# ---- rows that no sequence asks for -------------------------------------------------------------
+
+
+@pytest.mark.parametrize("D,G,n", [(64, 64, 2), (128, 128, 2), (256, 64, 2), (64, 64, 50), (128, 64, 50), (256, 128, 50)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_attend_rows_outside_every_range(lb, D, G, n, dtype):
+    """Padding rows before the first range and after the last give zeros and a log-sum of -inf."""
+    cache = random_cache(lb, 30, 2, D, 16, G, seed=7)
+    _, table = page_tables([100, 33], 16, 30, 8)
+    lens = torch.tensor([100, 33], dtype=torch.int32, device="cuda")
+    q = torch.randn(3 + 2 * n + 5, 8, D, device="cuda").to(DT[dtype])
+    qs = torch.tensor([3, 3 + n, 3 + 2 * n], dtype=torch.int32, device="cuda")
+    out = torch.full_like(q, 7.0)
+    got, lse = cache.attend(q, table, lens, q_start=qs, max_queries=n, out=out, return_lse=True)
+    cache.check()
+    inside = slice(3, 3 + 2 * n)
+    want, wlse = cache.attend(q[inside], table, lens, q_start=qs - 3, max_queries=n, return_lse=True)
+    assert torch.equal(got[inside], want) and torch.equal(lse[inside], wlse)
+    rest = torch.ones(len(q), dtype=torch.bool, device="cuda")
+    rest[inside] = False
+    assert (got[rest] == 0).all() and torch.isneginf(lse[rest]).all()
+
+
+def test_attend_rows_outside_every_range_of_many_sequences(lb):
+    """More sequences than one launch takes: the gaps are those of the whole call."""
+    lens = [5] * 700
+    cache = random_cache(lb, 700, 1, 64, 16, 64, seed=5)
+    _, table = page_tables(lens, 16, 700, 3)
+    q = torch.randn(712, 2, 64, device="cuda").to(torch.bfloat16)
+    dl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    qs = torch.arange(701, dtype=torch.int32, device="cuda") + 4
+    for most in (1, 40):  # both kernels
+        got = cache.attend(q, table, dl, q_start=qs, max_queries=most, out=torch.full_like(q, 7.0))
+        cache.check()
+        want = cache.attend(q[4:704], table, dl, q_start=qs - 4, max_queries=most)
+        assert torch.equal(got[4:704], want)
+        assert (got[:4] == 0).all() and (got[704:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_attend_without_sequences(lb, dtype):
+    cache = random_cache(lb, 2, 1, 64, 16, 64, seed=5)
+    q = torch.randn(3, 2, 64, device="cuda").to(DT[dtype])
+    got, lse = cache.attend(q, torch.zeros(0, 1, dtype=torch.int32, device="cuda"), torch.zeros(0, dtype=torch.int32, device="cuda"),
+                            q_start=torch.zeros(1, dtype=torch.int32, device="cuda"), out=torch.full_like(q, 7.0), return_lse=True)
+    assert (got == 0).all() and torch.isneginf(lse).all()
+
+
 # ---- captured graphs ------------------------------------------------------------------------------
 
 
