@@ -47,6 +47,8 @@ class _WeightArg(C.Structure):
 _APPEND = struct.Struct("6Q6q4Q2Q4I").pack
 _ATTEND = struct.Struct("3Q2q3Qq3Qf7I").pack
 _MATVEC = struct.Struct("3Q2qQI4x").pack
+_INF = float("inf")
+_FLOAT_PAST = 2.0 ** 128 - 2.0 ** 103  # the least that rounds past fp32
 
 
 def _bind(L):
@@ -252,8 +254,12 @@ class Cache4:
         stride, last = page_table.stride()
         if page_table.dtype is not torch.int32 or page_table.get_device() != self._dev or last != 1:
             _refuse(f"page_table must be int32 (sequences, width) on {dev}")
-        if window < 0 or max_queries < 1:
-            _refuse("window must not be negative, max_queries must be positive")
+        if not 0 <= window <= 0x7fffffff or not 1 <= max_queries <= 0xffffffff:
+            _refuse("window must fit an int and not be negative, max_queries must be positive and fit 32 bits")
+        if scale is None:
+            scale = D ** -0.5
+        elif _FLOAT_PAST <= abs(scale) < _INF:
+            _refuse("scale must fit fp32")
         qs = 0
         if q_start is not None:
             qs = _index(q_start, "q_start", torch.int32, (B + 1,), dev)
@@ -278,7 +284,7 @@ class Cache4:
         rc = self._lib.cora_kv4_attend(self._ref, _ATTEND(
             q.data_ptr(), out.data_ptr(), lp, qt, qh, page_table.data_ptr(),
             _index(lens, "lens", torch.int32, (B,), dev), qs, stride, T, size, work,
-            D ** -0.5 if scale is None else scale, B, width, Hq, max_queries, window, bool(causal), dt), stream)
+            scale, B, width, Hq, max_queries, window, bool(causal), dt), stream)
         if rc:
             _check(rc)
         return (out, lse) if return_lse else out

@@ -172,3 +172,20 @@ def test_threads_share_the_first_workspace_of_a_stream(fake, monkeypatch):
     for t in threads:
         t.join()
     assert len({work for work, _, _ in fake.calls}) == 1 and len(fake.calls) == 2
+
+
+@pytest.mark.parametrize("kw", [dict(window=1 << 31), dict(window=1 << 40), dict(window=-1), dict(max_queries=1 << 32),
+                                dict(max_queries=0), dict(scale=3.5e38), dict(scale=-1e300)])
+def test_numbers_past_their_fields_are_refused(fake, kw):
+    from coraanns_b200 import InvalidArgument
+    one = torch.ones(1, dtype=torch.int32)
+    with pytest.raises(InvalidArgument):
+        fake.cache().attend(torch.zeros(1, 2, 64, dtype=torch.bfloat16), one[None], one, **kw)
+    assert not fake.calls
+
+
+def test_largest_numbers_are_taken(fake):
+    one = torch.ones(1, dtype=torch.int32)
+    for kw in (dict(window=(1 << 31) - 1), dict(max_queries=(1 << 32) - 1), dict(scale=3.4028234e38)):
+        fake.cache().attend(torch.zeros(1, 2, 64, dtype=torch.bfloat16), one[None], one, **kw)
+    assert len(fake.calls) == 3
