@@ -240,7 +240,8 @@ class Cache4:
         q_start[b + 1] - 1 (q_start int32 (sequences + 1,), at most max_queries each; without it
         row b), its last tokens. causal: a token sees those up to itself, with a window only the
         last `window` of them. scale: of the scores, default head_dim ** -0.5. A token that sees
-        nothing gets zeros (and lse -inf), as do rows of q outside all ranges. Returns out, or (out, lse): lse is fp32 (rows, heads).
+        nothing gets zeros (and lse -inf), as do rows of q outside all ranges. Returns out, or (out, lse): lse is fp32 (rows, heads). out
+        may be q itself (a row is written once all that read it have), else it must not overlap q.
         """
         if self._dev != _current_device():
             with torch.cuda.device(self._dev):
@@ -378,7 +379,7 @@ class Weight4:
 def matvec(x: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = None,
            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x (..., cols) times the 4-bit weight, plus bias: (..., rows) in x's type. Meant for the few
-    rows of decoding (1 to 64); more are correct, 32 rows at a time."""
+    rows of decoding (1 to 64); more are correct, 32 rows at a time. out must not overlap x."""
     dev, N, dims = weight.device, weight.rows, x.dim()
     if not dims or x.shape[-1] != weight.cols or x.get_device() != weight._dev or x.stride(-1) != 1:
         _refuse(f"x must be (..., {weight.cols}) on {dev}, its last stride 1")
@@ -392,6 +393,10 @@ def matvec(x: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = None
         out = torch.empty(shape, dtype=x.dtype, device=dev)
     elif out.shape != shape or out.dtype != x.dtype or out.device != dev or not out.is_contiguous():
         _refuse("out must be contiguous, of x's type, (..., rows)")
+    elif M and N:  # (blocks read x while others write)
+        first, end = x2.data_ptr(), x2.data_ptr() + 2 * ((M - 1) * x2.stride(0) + weight.cols)
+        if out.data_ptr() < end and first < out.data_ptr() + 2 * M * N:
+            _refuse("out must not overlap x")
     _call(weight._lib.cora_w4_matvec, weight._dev, weight._ref, _MATVEC(
         x2.data_ptr(), bp, out.data_ptr(), x2.stride(0), N, M, _DTYPES.get(x.dtype, 99)))
     return out

@@ -364,7 +364,8 @@ int cora_kv4_append(const cora_kv4_cache *cache, const cora_kv4_append_args *arg
  * window w > 0 (causal only): the last w of those. A query that sees none gives zeros (lse
  * -inf), and so do rows of q before the first range and after the last. Query heads h * q_heads / kv_heads .. share key head h. out is q_tokens x q_heads x
  * head_dim, lse (natural log of the sum of exponentials; may be null) q_tokens x q_heads, both
- * contiguous. max_queries: an upper bound on the query tokens of a sequence.
+ * contiguous; out may be q itself (with the same strides), else it must not overlap q.
+ * max_queries: an upper bound on the query tokens of a sequence.
  * (table_width + 32) * page_size + q_tokens has to fit an int.
  * workspace: cora_kv4_attend_workspace() bytes for this q_heads and max_queries, zero before its
  * first use; left ready for the next call (of any shape it is large enough for). Calls that
@@ -400,7 +401,7 @@ typedef struct {
     uint32_t group;
 } cora_w4_weight;
 /* y[m] = weight x[m] (+ bias) for `rows` activation rows (fp32 sums, rounded once); strides in
- * elements. */
+ * elements. y must not overlap x. */
 typedef struct {
     const void *x, *bias;
     void *y;

@@ -299,3 +299,33 @@ def test_check_loses_no_error(lb):
             raised.set()
     thread.join()
     assert not lost
+
+
+# ---- outputs over inputs ------------------------------------------------------------------------
+
+
+def test_matvec_refuses_an_output_over_its_input(lb):
+    from coraanns_b200 import InvalidArgument
+    w = lb.Weight4.quantize(torch.randn(256, 256, device="cuda"))
+    buf = torch.randn(9, 256, device="cuda").to(torch.bfloat16)
+    for x, out in ((buf, buf), (buf[:4], buf[3:7]), (buf[3:7], buf[:4]), (buf[4], buf[4]), (buf[::2], buf[4:])):
+        with pytest.raises(InvalidArgument):
+            lb.matvec(x, w, out=out)
+    x = buf[:4].clone()
+    assert torch.equal(lb.matvec(buf[:4], w, out=buf[4:8]), lb.matvec(x, w)) and torch.equal(buf[:4], x)
+    assert torch.equal(lb.matvec(buf[4:8].clone(), w, out=buf[:4]), lb.matvec(buf[4:8], w))
+
+
+@pytest.mark.parametrize("n,lens,H,per", [(1, [30000], 2, 4), (5, [700, 300], 2, 4), (200, [3000, 900], 2, 4), (64, [500] * 20, 4, 1)])
+def test_attend_in_place(lb, n, lens, H, per):
+    """Over its own queries, jobs whole and cut over blocks."""
+    pages = sum(-(-x // 32) for x in lens)
+    cache = random_cache(lb, pages, H, 128, 32, 128, seed=8)
+    _, table = page_tables(lens, 32, pages, 9)
+    dl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    qs = torch.arange(len(lens) + 1, dtype=torch.int32, device="cuda") * n
+    q = torch.randn(n * len(lens), H * per, 128, device="cuda").to(torch.bfloat16)
+    want = cache.attend(q, table, dl, q_start=qs, max_queries=n)
+    for _ in range(20):
+        x = q.clone()
+        assert cache.attend(x, table, dl, q_start=qs, max_queries=n, out=x) is x and torch.equal(x, want)
