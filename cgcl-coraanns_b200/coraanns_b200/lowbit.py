@@ -253,7 +253,7 @@ class Cache4:
         dt = self._heads(q, "q", (T, Hq, self.head_dim))
         B, width = page_table.shape
         stride, last = page_table.stride()
-        if page_table.dtype is not torch.int32 or page_table.get_device() != self._dev or last != 1:
+        if page_table.dtype is not torch.int32 or page_table.get_device() != self._dev or (last != 1 and width > 1):
             _refuse(f"page_table must be int32 (sequences, width) on {dev}")
         if not 0 <= window <= 0x7fffffff or not 1 <= max_queries <= 0xffffffff:
             _refuse("window must fit an int and not be negative, max_queries must be positive and fit 32 bits")
@@ -381,7 +381,7 @@ def matvec(x: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = None
     """x (..., cols) times the 4-bit weight, plus bias: (..., rows) in x's type. Meant for the few
     rows of decoding (1 to 64); more are correct, 32 rows at a time. out must not overlap x."""
     dev, N, dims = weight.device, weight.rows, x.dim()
-    if not dims or x.shape[-1] != weight.cols or x.get_device() != weight._dev or x.stride(-1) != 1:
+    if not dims or x.shape[-1] != weight.cols or x.get_device() != weight._dev or (x.stride(-1) != 1 and weight.cols > 1):
         _refuse(f"x must be (..., {weight.cols}) on {dev}, its last stride 1")
     x2 = x if dims == 2 else x.reshape(-1, weight.cols)
     M = x2.shape[0]

@@ -329,3 +329,19 @@ def test_attend_in_place(lb, n, lens, H, per):
     for _ in range(20):
         x = q.clone()
         assert cache.attend(x, table, dl, q_start=qs, max_queries=n, out=x) is x and torch.equal(x, want)
+
+
+# ---- sizes of one and none ------------------------------------------------------------------------
+
+
+def test_strides_of_sizes_of_one_do_not_matter(lb):
+    cache = random_cache(lb, 4, 1, 64, 16, 64, seed=2)
+    q = torch.randn(3, 2, 64, device="cuda").to(torch.bfloat16)
+    lens = torch.tensor([3, 16, 9], dtype=torch.int32, device="cuda")
+    table = torch.tensor([[2, 0, 1]], dtype=torch.int32, device="cuda").t()  # (3, 1), strides (1, 3)
+    assert table.stride(1) != 1
+    assert torch.equal(cache.attend(q, table, lens), cache.attend(q, table.contiguous().view(3, 1), lens))
+    w = lb.Weight4.quantize(torch.randn(70, 1, device="cuda"))
+    x = torch.randn(1, 5, device="cuda").to(torch.float16).t()  # (5, 1), strides (1, 5)
+    assert x.stride(1) != 1
+    assert torch.equal(lb.matvec(x, w), lb.matvec(x.clone(memory_format=torch.contiguous_format).reshape(5).view(5, 1), w))
