@@ -356,10 +356,11 @@ class Weight4:
         """Quantise a dense (rows, cols) matrix, as a model is loaded (plain torch, in row blocks)."""
         _need(dense.dim() == 2 and dense.is_cuda and group in (32, 64, 128), "dense must be a CUDA matrix, group 32, 64 or 128")
         rows, cols = dense.shape
+        _need(cols >= 1, "dense must have columns")
         pad = -cols % 128
         step = max(1, (1 << 26) // (cols + pad))
         codes, meta = [], []
-        for r in range(0, rows, step):
+        for r in range(0, max(1, rows), step):
             x = torch.nn.functional.pad(dense[r:r + step].float(), (0, pad)).unflatten(1, (-1, group))
             low = x.amin(-1, keepdim=True)
             scale = ((x.amax(-1, keepdim=True) - low) * (1 / 15)).clamp(max=65504.0).half().float()
@@ -367,11 +368,11 @@ class Weight4:
             inv = torch.where(scale > 0, 1.0 / scale, torch.zeros_like(scale))
             c = ((x - low) * inv).round().clamp(0, 15).to(torch.int32)
             # 128 columns = 4 j x 4 t x 8 e -> words (t, j), nibbles by e
-            c = c.view(x.shape[0], -1, 4, 4, 8).transpose(2, 3)
+            c = c.view(x.shape[0], (cols + pad) // 128, 4, 4, 8).transpose(2, 3)
             word = torch.zeros(c.shape[:-1], dtype=torch.int32, device=dense.device)
             for e, nib in enumerate(NIBBLE_OF):
                 word |= c[..., e] << (4 * nib)
-            codes.append(word.reshape(x.shape[0], -1).view(torch.uint8))
+            codes.append(word.reshape(x.shape[0], (cols + pad) // 8).view(torch.uint8))
             meta.append(torch.cat((scale, low), -1).half())
         return cls(torch.cat(codes), torch.cat(meta), cols)
 

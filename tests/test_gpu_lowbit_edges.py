@@ -345,3 +345,13 @@ def test_strides_of_sizes_of_one_do_not_matter(lb):
     x = torch.randn(1, 5, device="cuda").to(torch.float16).t()  # (5, 1), strides (1, 5)
     assert x.stride(1) != 1
     assert torch.equal(lb.matvec(x, w), lb.matvec(x.clone(memory_format=torch.contiguous_format).reshape(5).view(5, 1), w))
+
+
+def test_weights_without_rows_or_columns(lb):
+    from coraanns_b200 import InvalidArgument
+    w = lb.Weight4.quantize(torch.zeros(0, 200, device="cuda"))
+    assert w.rows == 0 and lb.matvec(torch.zeros(3, 200, device="cuda", dtype=torch.float16), w).shape == (3, 0)
+    with pytest.raises(InvalidArgument):
+        lb.Weight4.quantize(torch.zeros(5, 0, device="cuda"))
+    with pytest.raises(InvalidArgument):
+        lb.Weight4.quantize(torch.zeros(5, 4, device="cuda"), group=48)
