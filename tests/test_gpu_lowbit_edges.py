@@ -191,6 +191,48 @@ def test_attend_without_sequences(lb, dtype):
     assert (got == 0).all() and torch.isneginf(lse).all()
 
 
+# ---- the kernels' rarer paths -------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("D,G", [(64, 64), (128, 128), (128, 64), (256, 128), (256, 64)])
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 37), (True, 1), (False, 0)])
+@pytest.mark.parametrize("per,counts", [(4, [5, 0, 8, 7, 3, 1]), (1, [32, 9, 10, 2, 31, 1]), (7, [4, 1, 2, 3, 0, 4])])
+def test_attend_several_tokens_streamed(lb, D, G, causal, window, per, counts):
+    """2 to 32 rows per key head: several query tokens through the streaming kernel, one sequence
+    with more of them than it has cached tokens."""
+    cache = random_cache(lb, 60, 2, D, 16, G, seed=D)
+    check_attend(lb, cache, [100, 64, 9, 3, 333, 20], per, counts, "fp16" if per == 4 else "bf16", causal=causal, window=window,
+                 seed=4)
+
+
+@pytest.mark.parametrize("D,G", [(64, 64), (128, 128), (128, 64), (256, 128), (256, 64)])
+@pytest.mark.parametrize("n,scale", [(4, 0.1), (40, 0.1), (4, -0.1), (40, -0.1), (40, 0.0), (150, 0.1)])
+def test_attend_maxima_that_keep_growing(lb, D, G, n, scale):
+    """Keys that grow from token to token (and scales of either sign): the running maximum is
+    raised, and the sums rescaled, many times along a sequence. |score| stays under 60."""
+    seed, L = 60, 500
+    cache = random_cache(lb, 40, 1, D, 16, G, seed=D)
+    gen = torch.Generator(device="cuda").manual_seed(D)
+    k = torch.randn(L, 1, D, generator=gen, device="cuda") * torch.linspace(0.05, 10.0 * (64 / D) ** 0.5, L, device="cuda")[:, None, None]
+    v = torch.randn(L, 1, D, generator=gen, device="cuda")
+    cache.append(k.to(torch.bfloat16), v.to(torch.bfloat16), slots_of(cache, [L], seed, np.arange(L)))
+    check_attend(lb, cache, [L], 3, [n], "fp16", scale=scale, seed=seed, q_scale=1.2)
+
+
+@pytest.mark.parametrize("D,G", [(64, 64), (128, 64), (256, 128)])
+def test_attend_value_scales_that_grow(lb, D, G):
+    """Values whose size doubles every 20 tokens: the streaming kernel's bound on the value scales is
+    raised, and its sums shrunk, along the sequence."""
+    seed, L = 70, 320
+    cache = random_cache(lb, 24, 1, D, 16, G, seed=D)
+    gen = torch.Generator(device="cuda").manual_seed(D)
+    v = torch.randn(L, 1, D, generator=gen, device="cuda") * 2.0 ** (torch.arange(L, device="cuda") / 20 - 8)[:, None, None]
+    k = torch.randn(L, 1, D, generator=gen, device="cuda")
+    cache.append(k.to(torch.bfloat16), v.to(torch.bfloat16), slots_of(cache, [L], seed, np.arange(L)))
+    check_attend(lb, cache, [L], 4, [1], "bf16", seed=seed)
+    check_attend(lb, cache, [L], 4, [7], "fp16", seed=seed)
+
+
 # ---- captured graphs ------------------------------------------------------------------------------
 
 
