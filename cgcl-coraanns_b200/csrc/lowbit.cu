@@ -230,9 +230,11 @@ void attend(const cora_kv4_cache *c, const cora_kv4_attend_args *a, cudaStream_t
 // ---- matvec ------------------------------------------------------------------------------
 
 // 32 weight rows per warp halve what is done once per activation (its loads, its sums); 16 give
-// twice the blocks, which matrices with fewer rows than fill the SMs twice need more. 32768 x 8192,
-// one row: 39 us with 32, 43 us with 16; 10007 x 5000, 13 rows: 27 us with 32 (spills), 20 with 16.
-constexpr uint64_t kWideRows = 32 * 2 * 148;
+// twice the blocks, which matrices with fewer rows than fill the SMs twice need more. One bf16 row,
+// weights from HBM, us with 16 / 32 rows per warp: 4736 x 4096 6.1 / 6.8, 7000 x 4096 8.5 / 8.4,
+// 9472 x 4096 10.0 / 8.8, 18944 x 4096 17.1 / 15.2, 32768 x 8192 46.5 / 42.2; eight rows alike. From
+// 9 rows of x on the products' registers spill with 32 (10007 x 5000, 13 rows: 27 us against 20).
+uint64_t wide_rows() { return 32ull * 2 * sm_count(); }
 
 template <typename T, int kGroup, int kMT, int kNT, bool kVec>
 void launch_matvec(const cora_w4_weight &w, const cora_w4_matvec_args &a, cudaStream_t st) {
@@ -261,7 +263,7 @@ void matvec(const cora_w4_weight *w, const cora_w4_matvec_args *a, cudaStream_t 
                 constexpr int NT = decltype(nt)::value, MT = decltype(mt)::value;
                 vec ? launch_matvec<T, G, MT, NT, true>(*w, *a, st) : launch_matvec<T, G, MT, NT, false>(*w, *a, st);
             };
-            const bool two = w->rows >= kWideRows;
+            const bool two = w->rows >= wide_rows();
             if (a->rows <= 8) two ? wide(Int<1>{}, Int<2>{}) : wide(Int<1>{}, Int<1>{});
             else if (a->rows <= 16) wide(Int<2>{}, Int<1>{});
             else wide(Int<4>{}, Int<1>{});

@@ -343,6 +343,34 @@ def test_check_loses_no_error(lb):
     assert not lost
 
 
+# ---- products: the variant for matrices of many rows ------------------------------------------------
+
+
+def wide_rows():
+    return 2 * 32 * torch.cuda.get_device_properties(0).multi_processor_count
+
+
+@pytest.mark.parametrize("M", [1, 5, 8])
+@pytest.mark.parametrize("over,K,G", [(-1, 200, 64), (0, 128, 128), (1, 7, 32), (31, 260, 64), (535, 384, 32), (535, 1003, 128)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_matvec_of_many_rows(lb, M, over, K, G, dtype):
+    """Row counts on both sides of where a warp takes two row tiles, with ragged last blocks, and few
+    columns (warps without a segment). Bound as in test_matvec."""
+    from test_gpu_lowbit import weight64
+    N = wide_rows() + over
+    gen = torch.Generator(device="cuda").manual_seed(M + N + K)
+    w = lb.Weight4.quantize(torch.randn(N, K, generator=gen, device="cuda") + 0.3, group=G)
+    x = torch.randn(M, K, generator=gen, device="cuda").to(DT[dtype])
+    bias = torch.randn(N, generator=gen, device="cuda").to(DT[dtype]) if M != 5 else None
+    y = lb.matvec(x, w, bias=bias).double().cpu().numpy()
+    x64 = x.double().cpu().numpy()
+    want = x64 @ weight64(w).T + (0 if bias is None else bias.double().cpu().numpy())
+    meta = np.repeat(w.meta.cpu().numpy().astype(np.float64), w.group, 1)[:, :K]
+    mass = np.abs(x64) @ (128 * meta[..., 0] + np.abs(meta[..., 1])).T
+    bound = TOL_OUT[dtype] * np.abs(want) + 2.0 ** -20 * mass + 1e-7
+    assert (np.abs(y - want) <= bound).all(), (np.abs(y - want) / bound).max()
+
+
 # ---- outputs over inputs ------------------------------------------------------------------------
 
 
