@@ -12,7 +12,8 @@ Tensors are CUDA tensors of torch, bf16 or fp16. Calls enqueue on the current st
 tensors' device and return without synchronising; tensors made on another stream have to be ready
 on it, as for any torch call. Errors in the arguments raise ``InvalidArgument``; what only the
 device can see (a slot, page, position or row range outside its tensor) is skipped there and
-reported by ``Cache4.check``. There is no CPU fallback.
+reported by ``Cache4.check``. There is no CPU fallback, and there are no gradients: results are
+detached from inputs that require them.
 """
 from __future__ import annotations
 

@@ -4,8 +4,9 @@
 //   out     = sum_t p_t (scale'_t c'_t + low'_t),   p = softmax(score)
 //
 // so codes enter the matrix instructions as integers and a token's factors are applied once per
-// (token, query), to fp32 sums. What bounds it: reading the cache once; instruction issue is
-// next (4 bits arrive at 48 codes per clock and SM). Hence:
+// (token, query), to fp32 sums. What has to be done is to read the cache once; what bounds it is
+// instruction latency (two warps per scheduler, 1080 warp instructions per 64 tokens and key head in one
+// group, issue slots 42% used), then memory. Hence:
 //  - tokens (then value dimensions) are the 16-row side of m16n8k16, query rows the 8-column
 //    side: the query heads that share a key head fill one instruction;
 //  - a code becomes an fp16 operand by one AND: nibble 0 of a 16-bit half is the subnormal
@@ -31,8 +32,9 @@
 //    A job inside one run is written by its warp; one cut over the warps of a block is joined in
 //    shared memory; one cut over blocks by the last block to arrive, from partial results in
 //    the workspace. Where all jobs are short, each block takes one instead (no join over blocks).
-// Measured, 8 key heads of 128: 131072 tokens 47 us (3.0 TB/s over the call, near 5 in the stream),
-// 64 ragged sequences of 200 to 16384 tokens in two groups 76 us (2.8 TB/s).
+// Measured, 8 key heads of 128: 131072 tokens 47 us (3.0 TB/s over the call; from 65536 to 262144
+// tokens 34 -> 77 us, 4.9 TB/s, so some 18 us are start and joins), 64 ragged sequences of 200 to
+// 16384 tokens in two groups 77 us (2.8 TB/s).
 #pragma once
 #include <cuda_fp16.h>
 
@@ -47,13 +49,16 @@ namespace cora {
 // past the little L1 that the ring leaves) and a tile of 64 tokens gives each warp enough
 // independent work. Measured on 131072 tokens x 8 key heads / a ragged batch of 64: 16 warps x 32
 // tokens 57 / 100 us, 12 x 32 53 / 93 us, 9 x 64 58 / 97 us, 8 x 64 47 / 76 us.
-constexpr int at_warps(int D) { return 8; }
-// Tokens of a tile (two tiles per warp have to fit shared memory), and tiles of a warp's ring.
+constexpr int kAtWarps = 8;
+// Tiles of a warp's ring, and tokens of a tile (two tiles per warp have to fit shared memory).
+constexpr int kAtStages = 2;
 constexpr int at_tile(int D) { return D == 256 ? 32 : 64; }
-constexpr int at_stages(int D) { return 2; }
 constexpr int kAtRows = 8;         // query rows of a job
 constexpr int kAtMinRun = 2;       // units of a warp, at least
-constexpr int kAtShort = 1280;     // tokens of a job that one block takes whole, at most
+// Tokens of a job that one block takes whole, at most, where the grid has a block for each job. Cut
+// over blocks, whole, in us, heads of 128: 8 jobs of 512 / 1280 / 2048 / 3072 tokens 17.0, 22.5, 19.5,
+// 19.5 against 14.2, 16.6, 20.7, 24.7; 64 jobs 22.7, 22.6, 23.0, 24.9 against 14.6, 18.4, 22.3, 25.6.
+constexpr int kAtShort = 1280;
 constexpr int kAtMaxSeqs = 512;    // sequences of one launch (their work is kept in smem)
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -73,7 +78,7 @@ constexpr int kAtPart = kAtRows * (D + 2);
 // The shared memory of a block, in order (each part a multiple of 16 bytes).
 template <int D, int kNG>
 struct AttendSmem {
-    static constexpr int kAtWarps = at_warps(D), kAtStages = at_stages(D), kAtTile = at_tile(D);
+    static constexpr int kAtTile = at_tile(D);
     static constexpr uint32_t kCodes = kAtTile * D / 2, kMeta = kAtTile * kNG * 4;
     static constexpr uint32_t kStage = 2 * kCodes + 2 * kMeta;
     static constexpr uint32_t kRing = kAtStages * kStage;   // of a warp; at the end its partial result
@@ -166,9 +171,9 @@ __global__ void kv4_clear_kernel(const AttendParams p) {
 }
 
 template <typename T, int D, int kNG>
-__global__ void __launch_bounds__(at_warps(D) * 32, 1) kv4_attend_kernel(const AttendParams p) {
+__global__ void __launch_bounds__(kAtWarps * 32, 1) kv4_attend_kernel(const AttendParams p) {
     using S = AttendSmem<D, kNG>;
-    constexpr int kAtWarps = at_warps(D), kAtThreads = kAtWarps * 32, kAtStages = at_stages(D), kAtTile = at_tile(D);
+    constexpr int kAtThreads = kAtWarps * 32, kAtTile = at_tile(D);
     constexpr int kMt = kAtTile / 16;
     constexpr int kG = D / kNG, kWords = kG / 32;  // words of one lane and group
     constexpr int kVB = D / 64;                    // 64-dimension blocks of the values

@@ -1,9 +1,11 @@
 // Attention of many query rows per key head over the paged 4-bit cache: cora_kv4_attend for
 // chunks of a prompt and wide head groups (more than 32 rows per key head). Measured: 2048 queries
-// x 32 heads of 128 on 16384 tokens (8 key heads) 731 us, 705 TFLOP/s.
+// x 32 heads of 128 on 16384 tokens (8 key heads) 756 us, 682 TFLOP/s (in turn with variants on
+// unchanged inputs 745; 730 when the other figures below were taken).
 //
-// Bound by the tensor cores and, next to them, by exponentials (16 a clock and SM) and by shared
-// memory. Rows (query token, head of the group) fill tiles of 128; one block takes kNQ = 2 tiles
+// Tensor cores and exponentials are each a third busy, issue slots 46%: what bounds it is the chain of
+// one row tile (softmax, hand-over, second product, next scores), of which the other row tile's
+// work covers a part. Rows (query token, head of the group) fill tiles of 128; one block takes kNQ = 2 tiles
 // (1 for few rows or head size 256) against the same keys, so each unpacked key tile serves 256
 // rows. Warp roles:
 //   0-3, 4-7  softmax of row tile 0 / 1, 32 rows per warp: sums of q . c from TMEM, the token's

@@ -66,9 +66,10 @@ __device__ __forceinline__ void ld_factors(const uint32_t *p, uint32_t (&f)[kWor
 //           24 bits, of which the offset costs about five, and the result keeps eight.
 // sum(x) of a group comes from one more product with a matrix of ones.
 //
-// What bounds it: reading the weights. Codes and factors of the next kMvDepth segments are in
-// flight in registers (a warp and segment: 1 or 2 KB). Measured: 32768 x 8192, one fp16 row, 39 us
-// (3.6 TB/s); 10007 x 5000, 13 bf16 rows, 20 us.
+// What has to be done is to read the weights: codes and factors of the next kMvDepth segments are in
+// flight in registers (a warp and segment: 1 or 2 KB). What bounds it is the wait for the activations,
+// which are loaded where they are used (long scoreboard first, issue slots 42% used). Measured:
+// 32768 x 8192, one fp16 row, 39 us (3.6 TB/s); 10007 x 5000, 13 bf16 rows, 20 us.
 template <typename T, int kGroup, int kMT, int kNT, bool kVec>
 __global__ void __launch_bounds__(kMvWarps * 32, kNT >= 4 ? 1 : 2) w4_matvec_kernel(const cora_w4_weight w,
                                                                                     const cora_w4_matvec_args p) {

@@ -113,8 +113,9 @@ void append(const cora_kv4_cache *c, const cora_kv4_append_args *a, cudaStream_t
 
 // Rows of one key head and sequence. Up to 32 the streaming kernel takes tiles of 8, reading the
 // cache again for each (from L2); more go to the tile kernel. Both measured, 16 sequences of 4096
-// tokens, 8 key heads, in us at 8 / 16 / 32 / 64 rows: head size 128, streaming 35 / 51 / 80 / 160,
-// tiles 102 / 102 / 104 / 104; head size 256, 55 / 84 / 145 / 264 against 170 / 172 / 173 / 175.
+// tokens, 8 key heads, in us at 8 / 16 / 32 / 40 / 48 / 64 rows: head size 64, streaming 29 / 41 / 65 /
+// 76 / 87 / 111, tiles 92 throughout; head size 128, 35 / 50 / 80 / 95 / 109 / 139 against 107 to 109;
+// head size 256, 55 / 84 / 144 / 175 / 205 / 264 against 172 to 177.
 uint64_t attend_rows(const cora_kv4_cache &c, uint64_t q_heads, uint64_t max_queries) {
     return std::max<uint64_t>(1, max_queries) * (q_heads / c.kv_heads);
 }
@@ -125,7 +126,7 @@ uint64_t attend_counters() { return ((uint64_t)sm_count() * 2 * 4 + 255) / 256 *
 uint64_t attend_workspace(const cora_kv4_cache &c, uint64_t rows) {
     const uint64_t blocks = sm_count();
     // few rows: two parts of 8 rows per block and one per warp
-    const uint64_t parts = rows <= kFewRows ? blocks * (2 + at_warps(c.head_dim)) * kAtRows
+    const uint64_t parts = rows <= kFewRows ? blocks * (2 + kAtWarps) * kAtRows
                                             : 2 * blocks * (rows <= 128 || c.head_dim == 256 ? 128 : 256);
     return attend_counters() + parts * (c.head_dim + 2) * 4;
 }
@@ -141,7 +142,7 @@ void launch_attend(AttendParams p, cudaStream_t st) {
     for (uint32_t s0 = 0; s0 < seqs; s0 += kAtMaxSeqs) {
         p.seq0 = s0;
         p.seqs = std::min<uint32_t>(kAtMaxSeqs, seqs - s0);
-        kern<<<sm_count(), at_warps(D) * 32, S::bytes(p.seqs), st>>>(p);
+        kern<<<sm_count(), kAtWarps * 32, S::bytes(p.seqs), st>>>(p);
         CUDA_TRY(cudaGetLastError());
     }
 }
